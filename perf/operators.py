@@ -177,21 +177,21 @@ def _mx_values(v, e):
 
 def _mx_pack(v, e):
     """Stored form: two codes a byte (the even column in the low half), and the scale bytes in the product's order:
-    [blocks of 512 columns][4][rows][4], where byte 2 j + q of entry g is that of columns 32 (8 j + 2 g + q) ..."""
+    [512-column blocks][4][rows, to a multiple of 4][4], where byte b of entry g is that of columns 32 (4 b + g) .. of
+    the 512; zero where there is no such column or row."""
     index = torch.tensor([0, 1, 2, 3, 4, 0, 5, 0, 6, 0, 0, 0, 7], dtype=torch.uint8, device=v.device)
     code = index[(v.abs() * 2).long()] | (torch.signbit(v).to(torch.uint8) << 3)
     rows, nb = e.shape
-    scale = torch.zeros(rows, -(-nb // 16) * 16, dtype=torch.uint8, device=v.device)
-    scale[:, :nb] = (e + 127).to(torch.uint8)
-    scale = scale.view(rows, -1, 2, 4, 2).permute(1, 3, 0, 2, 4).reshape(-1, 4, rows, 4).contiguous()
+    scale = torch.zeros(-(-rows // 4) * 4, -(-nb // 16) * 16, dtype=torch.uint8, device=v.device)
+    scale[:rows, :nb] = (e + 127).to(torch.uint8)
+    scale = scale.view(scale.shape[0], -1, 4, 4).permute(1, 3, 0, 2).contiguous()
     return (code[:, 0::2] | (code[:, 1::2] << 4)).contiguous(), scale
 
 
 def _mx_unpack(codes, scale):
     table = torch.tensor([*E2M1, *(-t for t in E2M1)], device=codes.device)
     v = torch.stack((table[(codes & 15).long()], table[(codes >> 4).long()]), -1).flatten(-2)
-    rows = codes.shape[0]
-    e = scale.view(-1, 4, rows, 2, 2).permute(2, 0, 3, 1, 4).reshape(rows, -1)[:, : v.shape[1] // 32].int() - 127
+    e = scale.permute(2, 0, 3, 1).flatten(1)[: v.shape[0], : v.shape[1] // 32].int() - 127
     return _mx_values(v, e)
 
 
