@@ -1,0 +1,288 @@
+// MXFP4 projections for gfx950: row quantization to e2m1 codes with a
+// power-of-two scale for each 32 values, its inverse, and the product of two
+// such matrices on the block-scaled MFMA (formats: include/tmhd_lowbit.h).
+#include <type_traits>
+
+#include <algorithm>
+
+#include "tmhd_internal.h"
+#include "tmhd_lowbit.h"
+
+namespace tmhd {
+namespace {
+
+using i32x8 = int __attribute__((ext_vector_type(8)));
+using u16x2 = unsigned short __attribute__((ext_vector_type(2)));
+
+constexpr int kSuper = 512;  // columns that a scale word spans
+
+// Scale word of (512-column block s, column group g, row): R4 rows, a multiple of 4.
+__device__ __forceinline__ int64_t scale_word(int s, int g, int row, int32_t r4) {
+  return ((int64_t)s * 4 + g) * r4 + row;
+}
+
+// ---------------------------------------------------------------------------
+// Row quantization: bound by HBM.  A wave takes one 512-column block of RQ
+// consecutive rows: per row a 16-byte load of 8 values per lane (1 KiB in all),
+// four lanes to a block of 32.  The maximum is taken on the magnitudes' bits
+// (packed 16-bit integers), so a block's exponent is that maximum's exponent
+// field and an infinity or NaN shows as a maximum of 0x7f80 and more.  The
+// conversion instruction divides by the scale, rounds to nearest even and
+// saturates.
+constexpr int RQ = 4;
+
+// max of the magnitudes of 8 bf16, in both halves of the result
+__device__ __forceinline__ uint32_t amax8(const i32x4 &v) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, (uint32_t)v[e] & 0x7fff7fffu));
+  return max((uint32_t)m[0], (uint32_t)m[1]);
+}
+
+// scale byte of a block whose largest magnitude has the bf16 bits amax
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  const uint32_t e = amax >> 7;  // exponent field
+  return e == 255u ? 255u : (uint32_t)max((int)e - 2, 2);
+}
+
+// 8 bf16 -> 8 codes; a block without finite values (byte 255) gives codes 0
+__device__ __forceinline__ uint32_t codes8(const i32x4 &v, uint32_t byte) {
+  const float scale = __uint_as_float(byte << 23);
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, (uint32_t)v[0]), scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, (uint32_t)v[1]), scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, (uint32_t)v[2]), scale, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, (uint32_t)v[3]), scale, 3);
+  return byte == 255u ? 0u : c;
+}
+
+__global__ void __launch_bounds__(256) mxfp4_quant_kernel(uint8_t *__restrict__ q, uint32_t *__restrict__ scale,
+                                                          const uint16_t *__restrict__ x, int32_t rows, int32_t r4,
+                                                          int32_t cols, int64_t xs, int32_t blocks) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int s = blockIdx.x % blocks, row0 = (blockIdx.x / blocks * 4 + w) * RQ;
+  if (row0 >= r4) return;
+  const int col = s * kSuper + lane * 8;
+  const bool live = col < cols;
+  i32x4 v[RQ];
+#pragma unroll
+  for (int i = 0; i < RQ; ++i)
+    v[i] = live && row0 + i < rows ? *(const i32x4 *)(x + (int64_t)(row0 + i) * xs + col) : i32x4{0, 0, 0, 0};
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    uint32_t m = amax8(v[i]);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+    const bool there = live && row0 + i < rows;
+    uint32_t byte = scale_byte(m);
+    if (there) *(uint32_t *)(q + (int64_t)(row0 + i) * (cols >> 1) + (col >> 1)) = codes8(v[i], byte);
+    byte = there ? byte : 0u;
+    // block 4 b + g of the 512 columns sits in lanes 16 b + 4 g ..: word g of
+    // the row gathers lanes 4 g + 16 b
+    uint32_t gathered = byte | (uint32_t)__shfl_xor((int)byte, 16) << 8;
+    gathered |= (uint32_t)__shfl_xor((int)gathered, 32) << 16;
+    if ((lane & 3) == i) word = gathered;  // lanes 4 g + i of the first 16 keep row i's word g
+  }
+  if (lane < 16) scale[scale_word(s, lane >> 2, row0 + (lane & 3), r4)] = word;
+}
+
+// The inverse: a lane reads 8 codes and their scale byte, writes 16 bytes.
+__global__ void __launch_bounds__(256) mxfp4_dequant_kernel(uint16_t *__restrict__ x, const uint8_t *__restrict__ q,
+                                                            const uint32_t *__restrict__ scale, int32_t rows,
+                                                            int32_t r4, int32_t cols, int32_t blocks) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int s = blockIdx.x % blocks, row0 = (blockIdx.x / blocks * 4 + w) * RQ;
+  const int col = s * kSuper + lane * 8;
+  if (col >= cols) return;
+  uint32_t c[RQ], sw[RQ];
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    const int row = min(row0 + i, rows - 1);
+    c[i] = *(const uint32_t *)(q + (int64_t)row * (cols >> 1) + (col >> 1));
+    sw[i] = scale[scale_word(s, (lane >> 2) & 3, row, r4)];
+  }
+#pragma unroll
+  for (int i = 0; i < RQ; ++i) {
+    if (row0 + i >= rows) break;
+    const uint32_t byte = (sw[i] >> (8 * (lane >> 4))) & 255u;
+    const float f = __uint_as_float(byte << 23);
+    i32x4 o;
+    o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[i], f, 0));
+    o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[i], f, 1));
+    o[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[i], f, 2));
+    o[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[i], f, 3));
+    if (byte == 255u) o = i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
+    *(i32x4 *)(x + (int64_t)(row0 + i) * cols + col) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Products.  D[n][m] = B rows x A rows on v_mfma_scale_f32_16x16x128_f8f6f4: a
+// lane (i, g) = (lane % 16, lane / 16) holds the 16 bytes of columns 32 g .. of
+// row i for each 128 columns, so a 32-column block and its scale belong to one
+// lane, and word g of a row's scales serves four MFMAs (byte b for columns 128 b
+// .. of 512).  It gets four consecutive n of one m.
+struct XArgs {
+  const uint8_t *a;
+  const uint8_t *b;
+  const uint32_t *as;
+  const uint32_t *bs;
+  uint16_t *out;
+  const uint16_t *bias;
+  int32_t m, n, k;
+  int32_t am4, bn4;  // rows of the scale arrays
+  int64_t lda, ldb, ldo;
+  int32_t st_ok;     // 8-byte stores of 4 columns
+};
+
+template <int B>
+__device__ __forceinline__ f32x4 mfma_fp4(const i32x4 &b, const i32x4 &a, const f32x4 &c, int sb, int sa) {
+  const i32x8 bb = {b[0], b[1], b[2], b[3]}, aa = {a[0], a[1], a[2], a[3]};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bb, aa, c, 4, 4, B, sb, B, sa);
+}
+
+// Four columns n .. n + 3 of row m, bias added, rounded once.
+__device__ __forceinline__ void store_quad(const XArgs &xa, const f32x4 &v, int m, int n) {
+  if (m >= xa.m || n >= xa.n) return;
+  float t[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] = v[e] + (xa.bias ? bf16_bits_to_f32(xa.bias[min(n + e, xa.n - 1)]) : 0.0f);
+  const i32x2 o = {(int)pack_bf16_rne(t[0], t[1]), (int)pack_bf16_rne(t[2], t[3])};
+  uint16_t *op = xa.out + (int64_t)m * xa.ldo + n;
+  if (xa.st_ok && n + 3 < xa.n)
+    *(i32x2 *)op = o;
+  else
+    for (int e = 0; e < 4 && n + e < xa.n; ++e) op[e] = (uint16_t)((uint32_t)o[e >> 1] >> (16 * (e & 1)));
+}
+
+// Few rows: 16 columns of n and 16 MB rows of m a workgroup, its W waves take
+// the 512-column blocks of k in turn, straight from global memory to the MFMA
+// (each code is used once or by MB MFMAs), and add their sums through LDS in
+// wave order.
+template <int MB, int W>
+__global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
+  __shared__ f32x4 part[W][MB][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
+  const int chunks = xa.k >> 5, blocks = (xa.k + kSuper - 1) / kSuper;
+  const int brow = min(n0 + li, xa.n - 1);
+  const uint8_t *bp = xa.b + (int64_t)brow * xa.ldb + lg * 16;
+  const uint8_t *ap[MB];
+  int arow[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) {
+    arow[j] = min(m0 + j * 16 + li, xa.m - 1);
+    ap[j] = xa.a + (int64_t)arow[j] * xa.lda + lg * 16;
+  }
+  f32x4 acc[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = w; s < blocks; s += W) {
+    // chunk 16 s + 4 t + lg; behind the last column: zero codes (their scale bytes are zero too)
+    const int64_t at = (int64_t)s * (kSuper / 2);
+    i32x4 bv[4], av[MB][4];
+    int sa[MB];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bool in = 16 * s + 4 * t + lg < chunks;
+      bv[t] = in ? *(const i32x4 *)(bp + at + 64 * t) : i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < MB; ++j) av[j][t] = in ? *(const i32x4 *)(ap[j] + at + 64 * t) : i32x4{0, 0, 0, 0};
+    }
+    const int sb = (int)xa.bs[scale_word(s, lg, brow, xa.bn4)];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) sa[j] = (int)xa.as[scale_word(s, lg, arow[j], xa.am4)];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      acc[j] = mfma_fp4<0>(bv[0], av[j][0], acc[j], sb, sa[j]);
+      acc[j] = mfma_fp4<1>(bv[1], av[j][1], acc[j], sb, sa[j]);
+      acc[j] = mfma_fp4<2>(bv[2], av[j][2], acc[j], sb, sa[j]);
+      acc[j] = mfma_fp4<3>(bv[3], av[j][3], acc[j], sb, sa[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j) part[w][j][lane] = acc[j];
+  __syncthreads();
+  for (int j = w; j < MB; j += W) {
+    f32x4 sum = part[0][j][lane];
+#pragma unroll
+    for (int i = 1; i < W; ++i) sum += part[i][j][lane];
+    store_quad(xa, sum, m0 + j * 16 + li, n0 + 4 * lg);
+  }
+}
+
+int round4(int32_t rows) { return (int)(((int64_t)rows + 3) / 4 * 4); }
+
+int check_matrix(const char *what, int32_t rows, int32_t cols) {
+  if (rows < 0 || rows > INT32_MAX - 64) return set_error(TMHD_ERR_INVALID, "%s: rows %d", what, rows);
+  if (cols <= 0 || cols % 32) return set_error(TMHD_ERR_UNSUPPORTED, "%s: columns %d must be a positive multiple of 32", what, cols);
+  return TMHD_OK;
+}
+
+// Workgroups of 4 RQ rows x 512 columns; 0: more than a launch holds.
+unsigned quant_grid(int32_t rows, int32_t cols) {
+  const int64_t g = (((int64_t)rows + 4 * RQ - 1) / (4 * RQ)) * ((cols + kSuper - 1) / kSuper);
+  return g <= INT32_MAX ? (unsigned)g : 0u;
+}
+
+}  // namespace
+}  // namespace tmhd
+
+extern "C" int tmhd_mxfp4_quant(uint8_t *q, uint8_t *scale, const void *x, int32_t rows, int32_t cols,
+                                int64_t x_stride, void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_mxfp4_quant";
+  if (int st = check_matrix(what, rows, cols)) return st;
+  if (rows == 0) return TMHD_OK;
+  if (!q || !scale || !x || (uintptr_t)x % 16 || (uintptr_t)q % 16 || (uintptr_t)scale % 16)
+    return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
+  if (x_stride < cols || x_stride % 8) return set_error(TMHD_ERR_INVALID, "%s: row stride %lld", what, (long long)x_stride);
+  const unsigned grid = quant_grid(rows, cols);
+  if (!grid) return set_error(TMHD_ERR_UNSUPPORTED, "%s: %d x %d is too large", what, rows, cols);
+  hipLaunchKernelGGL(mxfp4_quant_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, q, (uint32_t *)scale,
+                     (const uint16_t *)x, rows, round4(rows), cols, x_stride, (cols + kSuper - 1) / kSuper);
+  return check_launch(what);
+}
+
+extern "C" int tmhd_mxfp4_dequant(void *x, const uint8_t *q, const uint8_t *scale, int32_t rows, int32_t cols,
+                                  void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_mxfp4_dequant";
+  if (int st = check_matrix(what, rows, cols)) return st;
+  if (rows == 0) return TMHD_OK;
+  if (!q || !scale || !x || (uintptr_t)x % 16 || (uintptr_t)q % 16 || (uintptr_t)scale % 16)
+    return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
+  const unsigned grid = quant_grid(rows, cols);
+  if (!grid) return set_error(TMHD_ERR_UNSUPPORTED, "%s: %d x %d is too large", what, rows, cols);
+  hipLaunchKernelGGL(mxfp4_dequant_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, (uint16_t *)x, q,
+                     (const uint32_t *)scale, rows, round4(rows), cols, (cols + kSuper - 1) / kSuper);
+  return check_launch(what);
+}
+
+extern "C" int tmhd_gemm_mxfp4(void *out, const uint8_t *a, const uint8_t *b, const uint8_t *a_scale,
+                               const uint8_t *b_scale, const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda,
+                               int64_t ldb, int64_t ldo, void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_gemm_mxfp4";
+  if (int st = check_matrix(what, m, k)) return st;
+  if (n <= 0 || n > INT32_MAX - 64) return set_error(TMHD_ERR_INVALID, "%s: n %d", what, n);
+  if (m == 0) return TMHD_OK;
+  if (!out || !a || !b || !a_scale || !b_scale || (uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)a_scale % 16 ||
+      (uintptr_t)b_scale % 16 || (uintptr_t)out % 2 || (uintptr_t)bias % 2)
+    return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
+  if (lda % 16 || ldb % 16 || lda < k / 2 || ldb < k / 2 || ldo < n)
+    return set_error(TMHD_ERR_INVALID, "%s: row strides %lld, %lld, %lld", what, (long long)lda, (long long)ldb, (long long)ldo);
+  const XArgs xa{a, b, (const uint32_t *)a_scale, (const uint32_t *)b_scale, (uint16_t *)out, (const uint16_t *)bias,
+                 m, n, k, round4(m), round4(n), lda, ldb, ldo,
+                 (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0)};
+  hipStream_t s = (hipStream_t)stream;
+  const unsigned nt = (unsigned)((n + 15) / 16);
+  if ((m + 63) / 64 > 65535) return set_error(TMHD_ERR_UNSUPPORTED, "%s: m %d is too large", what, m);
+  if (m <= 16)
+    hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4>), dim3(nt, 1), dim3(256), 0, s, xa);
+  else
+    hipLaunchKernelGGL((mxfp4_rows_kernel<4, 4>), dim3(nt, (unsigned)((m + 63) / 64)), dim3(256), 0, s, xa);
+  return check_launch(what);
+}

@@ -12,7 +12,7 @@ the hand-written HIP kernels of libtmhd.so; nothing falls back to the CPU.
 """
 
 from . import _native, condition
-from .attention import QKQuantWorkspace, segment_attention
+from .attention import AttentionCall, QKQuantWorkspace, segment_attention, segment_attention_batch
 from .capability import (
     STREAM_HOOK_ABI,
     native_stream_attention_hook,
@@ -42,6 +42,16 @@ from .adaln import (
 )
 from .packed import packed_sdpa
 from .rope import fused_apply_rope, fused_qk_norm_rope, fused_qkv_qk_norm_rope_, fused_qkv_qk_norm_rope_stage_
+from .mxfp4 import (
+    mxfp4_dequant,
+    mxfp4_linear,
+    mxfp4_quant,
+    mxfp4_quant_into,
+    mxfp4_scale_from_rows,
+    mxfp4_scale_to_rows,
+    mxfp4_scaled_mm,
+    mxfp4_scaled_mm_out,
+)
 from .quant import (
     cutlass_scaled_mm,
     cutlass_scaled_mm_out,
@@ -86,6 +96,7 @@ __all__ = [
     "_native",
     "AVKV",
     "AUDIO_TOKEN_TAG",
+    "AttentionCall",
     "CleanAVKVCache",
     "CutlassW8A8Workspace",
     "H3StreamingAttentionHook",
@@ -115,6 +126,14 @@ __all__ = [
     "int8_mm_i32",
     "kv_contract_from_model",
     "linear",
+    "mxfp4_dequant",
+    "mxfp4_linear",
+    "mxfp4_quant",
+    "mxfp4_quant_into",
+    "mxfp4_scale_from_rows",
+    "mxfp4_scale_to_rows",
+    "mxfp4_scaled_mm",
+    "mxfp4_scaled_mm_out",
     "load_cutlass_w8a8_stream_weight_",
     "native_stream_attention_hook",
     "native_stream_attention_metadata",
@@ -129,6 +148,7 @@ __all__ = [
     "resolve_h3_cutlass_w8a8_policy",
     "scaled_int8_quant",
     "segment_attention",
+    "segment_attention_batch",
     "set_native_stream_attention_hook",
     "set_official_attention_hook",
     "streaming_capability",

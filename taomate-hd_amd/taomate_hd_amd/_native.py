@@ -1,5 +1,5 @@
-"""ctypes binding of libtmhd.so (the C ABI declared in include/tmhd.h, tmhd_batch.h
-and tmhd_forms.h).
+"""ctypes binding of libtmhd.so (the C ABI declared in include/tmhd.h, tmhd_batch.h,
+tmhd_forms.h and tmhd_lowbit.h).
 
 The library is the only compute path of this package: every operator raises
 if it is not built or no GPU is present.  There is no CPU fallback.
@@ -7,6 +7,7 @@ if it is not built or no GPU is present.  There is no CPU fallback.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
@@ -221,6 +222,17 @@ _MORE_SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     ),
 }
 
+# include/tmhd_lowbit.h
+_LOWBIT_SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
+    "tmhd_mxfp4_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int64, c_void_p]),
+    "tmhd_mxfp4_dequant": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    "tmhd_gemm_mxfp4": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_int64,
+         c_int64, c_void_p],
+    ),
+}
+
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)  # of include/tmhd.h
 
 _lock = threading.Lock()
@@ -240,7 +252,8 @@ def load() -> ctypes.CDLL:
                     "(hipcc --offload-arch=gfx950) before using the HIP operators"
                 )
             lib = ctypes.CDLL(str(LIB_PATH))
-            for name, (restype, argtypes) in (*_SIGNATURES.items(), *_MORE_SIGNATURES.items()):
+            for name, (restype, argtypes) in (*_SIGNATURES.items(), *_MORE_SIGNATURES.items(),
+                                              *_LOWBIT_SIGNATURES.items()):
                 fn = getattr(lib, name)
                 fn.restype = restype
                 fn.argtypes = argtypes
@@ -298,6 +311,16 @@ def stream_ptr(torch: Any, device: Any) -> int:
         else:
             _gpu_index[given] = index
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_ON_DEVICE = contextlib.nullcontext()
+
+
+def device_of(torch: Any, tensor: Any) -> Any:
+    """A context in which the GPU of ``tensor`` is the current one (a launch goes
+    to the current device; the guard costs host time only where it changes)."""
+    index = tensor.device.index
+    return _ON_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def ptr(tensor: Any) -> int:
