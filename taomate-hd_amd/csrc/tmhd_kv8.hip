@@ -1,0 +1,793 @@
+// K/V slots held in 8 bits (e4m3 or int8 codes, a power-of-two scale for each 64
+// tokens of a head; formats: include/tmhd_lowbit.h): the quantizing pack, the
+// exact expansion to bf16 and attention of few query rows that reads the codes.
+#include <type_traits>
+
+#include <algorithm>
+
+#include "tmhd_internal.h"
+#include "tmhd_lowbit.h"
+
+namespace tmhd {
+namespace {
+
+using u16x2 = unsigned short __attribute__((ext_vector_type(2)));
+using i16x2 = short __attribute__((ext_vector_type(2)));
+
+constexpr int kBlock = 64;  // tokens of a scale
+constexpr int kMaxRanges = 32, kMaxCalls = 16, kMaxSegs = 24;
+constexpr int kMinByte = 10;  // 2^-117: the least code times it is a normal number
+
+// ---- codes
+
+// 2^(byte - 127); NaN for 255 (byte >= kMinByte)
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+}
+
+// scale byte of a block whose largest magnitude has the bf16 bits amax: the
+// least power of two with amax <= 448 (1.75 * 2^8) or 127 (1.984375 * 2^6) times it
+template <bool E4M3>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  if (amax >= 0x7f80u) return 255u;
+  const int e = (int)(amax >> 7), m = (int)(amax & 0x7fu);
+  return (uint32_t)max(E4M3 ? e - 8 + (m > 0x60) : e - 6 + (m > 0x7e), kMinByte);
+}
+
+// 8 bf16 -> 8 codes (2 words)
+template <bool E4M3>
+__device__ __forceinline__ i32x2 encode8(const i32x4 &v, uint32_t byte) {
+  i32x2 c;
+  if (byte == 255u) return i32x2{0, 0};
+  if constexpr (E4M3) {
+    const float s = __uint_as_float(byte << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i16x2 p = {0, 0};
+      const uint32_t lo = (uint32_t)v[2 * h], hi = (uint32_t)v[2 * h + 1];
+      p = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(p, __builtin_bit_cast(bf16x2, lo), s, false);
+      p = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(p, __builtin_bit_cast(bf16x2, hi), s, true);
+      c[h] = __builtin_bit_cast(int, p);
+    }
+  } else {
+    const float inv = __uint_as_float((254u - byte) << 23);  // exact: the byte is 10 .. 248
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t p = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t w = (uint32_t)v[2 * h + (e >> 1)];
+        const float x = bf16_bits_to_f32((e & 1) ? w >> 16 : w & 0xffffu);
+        p |= ((uint32_t)(int)__builtin_rintf(x * inv) & 255u) << (8 * e);
+      }
+      c[h] = (int)p;
+    }
+  }
+  return c;
+}
+
+// 4 codes -> 4 bf16 (2 words), times `scale` (a power of two or NaN)
+template <bool E4M3>
+__device__ __forceinline__ i32x2 decode4(uint32_t c, float scale, bool nan) {
+  if constexpr (E4M3) {
+    i32x2 o;
+    o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false));
+    o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true));
+    return nan ? i32x2{0x7fc07fc0, 0x7fc07fc0} : o;
+  } else {
+    const float a = (float)(int8_t)c, b = (float)(int8_t)(c >> 8), d = (float)(int8_t)(c >> 16), e = (float)(int8_t)(c >> 24);
+    return i32x2{(int)pack_bf16_rne(a * scale, b * scale), (int)pack_bf16_rne(d * scale, e * scale)};
+  }
+}
+
+// ---- pack
+
+struct PackArgs {
+  const uint16_t *k, *v;
+  int64_t ts, hs;
+  uint8_t *ko, *vo, *kso, *vso;
+  int32_t cap, n_ranges;
+  struct {
+    const int32_t *rows;
+    int32_t row0, n, dst, first;  // first: of the launch's 64-token blocks
+  } r[kMaxRanges];
+};
+
+// bytes of a word -> word i holds byte i of the four words
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// Quantizing pack of one 64-token block of K or of V of one head; bound by HBM.
+// 2 D threads: thread (tg, dl) holds channels 8 dl .. of tokens 4 tg .. (four
+// 16-byte loads, whole rows of a head per wave), the workgroup's maximum gives
+// the scale, and the codes go through LDS into the slot's chunk order, so that
+// the block leaves as 64 D contiguous bytes.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(2 * D) kv8_pack_kernel(const PackArgs pa) {
+  constexpr int T = 2 * D, L = D / 8;  // threads; lanes of a token row
+  __shared__ uint32_t img[16 * D];
+  __shared__ uint32_t part[T / 64];
+  const int tid = threadIdx.x, dl = tid % L, tg = tid / L;
+  const bool is_v = blockIdx.y & 1;
+  const int h = blockIdx.y >> 1;
+  int ri = 0;
+  while (ri + 1 < pa.n_ranges && (int)blockIdx.x >= pa.r[ri + 1].first) ++ri;
+  const int b = (int)blockIdx.x - pa.r[ri].first, n = pa.r[ri].n;  // block of the range; n > 64 b
+  const int32_t *rows = pa.r[ri].rows;
+  const uint16_t *src = (is_v ? pa.v : pa.k) + (int64_t)h * pa.hs + dl * 8;
+  i32x4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 64 * b + 4 * tg + i, tc = min(t, n - 1);
+    const int64_t row = rows ? rows[tc] : pa.r[ri].row0 + tc;
+    v[i] = *(const i32x4 *)(src + row * pa.ts);
+    if (t >= n) v[i] = i32x4{0, 0, 0, 0};
+  }
+  u16x2 mx = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(u16x2, (uint32_t)v[i][e] & 0x7fff7fffu));
+  int m = max((int)mx[0], (int)mx[1]);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) m = max(m, __shfl_xor(m, off));
+  if ((tid & 63) == 0) part[tid >> 6] = (uint32_t)m;
+  __syncthreads();
+  uint32_t amax = part[0];
+#pragma unroll
+  for (int i = 1; i < T / 64; ++i) amax = max(amax, part[i]);
+  const uint32_t byte = scale_byte<E4M3>(amax);
+  const int64_t blk = pa.r[ri].dst / kBlock + b;  // of the slot
+  if (tid == 0) (is_v ? pa.vso : pa.kso)[(int64_t)h * (pa.cap / kBlock) + blk] = (uint8_t)byte;
+  i32x2 c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = encode8<E4M3>(v[i], byte);
+  if (is_v) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t w[4] = {(uint32_t)c[0][half], (uint32_t)c[1][half], (uint32_t)c[2][half], (uint32_t)c[3][half]};
+      transpose4(w);  // word e: channel 8 dl + 4 half + e of the four tokens
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 8 * dl + 4 * half + e;
+        img[(tg >> 3) * (8 * D) + (d >> 5) * 256 + (tg & 1) * 128 + (d & 31) * 4 + ((tg >> 1) & 3)] = w[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * tg + i;
+      *(i32x2 *)&img[(t >> 5) * (8 * D) + (dl >> 1) * 128 + (t & 31) * 4 + (dl & 1) * 2] = c[i];
+    }
+  }
+  __syncthreads();
+  uint8_t *out = (is_v ? pa.vo : pa.ko) + ((int64_t)h * pa.cap + blk * kBlock) * D;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) *(i32x4 *)(out + (i * T + tid) * 16) = *(const i32x4 *)&img[(i * T + tid) * 4];
+}
+
+// ---- expansion
+
+struct View {
+  const uint8_t *k, *v, *ks, *vs;  // at the view's first row
+  int32_t cap, tokens, dst, first;
+};
+struct ExpandArgs {
+  uint16_t *k, *vt;
+  int64_t khs, vhs;
+  int32_t vrs, n_views;
+  View view[kMaxSegs];
+};
+
+// One 64-token block of K or V of one head into the bf16 slot format; bound by
+// HBM.  K: lanes run along a token row, so that rows are written whole.  V: the
+// 16 codes of a chunk are two runs of 8 consecutive positions of a transposed row.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(2 * D) kv8_expand_kernel(const ExpandArgs ea) {
+  constexpr int T = 2 * D, C = D / 16;
+  const int tid = threadIdx.x, h = blockIdx.y >> 1;
+  const bool is_v = blockIdx.y & 1;
+  int vi = 0;
+  while (vi + 1 < ea.n_views && (int)blockIdx.x >= ea.view[vi + 1].first) ++vi;
+  const View &vw = ea.view[vi];
+  const int b = (int)blockIdx.x - vw.first;
+  const int64_t in_at = ((int64_t)h * vw.cap + b * kBlock) * D;
+  const uint32_t byte = (is_v ? vw.vs : vw.ks)[(int64_t)h * (vw.cap / kBlock) + b];
+  const float s = scale_of(byte);
+  const bool nan = byte == 255u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = i * T + tid;
+    if (is_v) {
+      const int g = c & 1, tile = (c >> 1) & 1, d = c >> 2;
+      const i32x4 w = *(const i32x4 *)(vw.v + in_at + tile * (32 * D) + (d >> 5) * 1024 + g * 512 + (d & 31) * 16);
+      uint16_t *o = ea.vt + (int64_t)h * ea.vhs + (int64_t)d * ea.vrs + vw.dst + b * kBlock + tile * 32 + g * 8;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const i32x2 lo = decode4<E4M3>((uint32_t)w[2 * m], s, nan), hi = decode4<E4M3>((uint32_t)w[2 * m + 1], s, nan);
+        *(i32x4 *)(o + 16 * m) = i32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    } else {
+      const int dc = c % C, t = c / C;
+      const i32x4 w = *(const i32x4 *)(vw.k + in_at + (t >> 5) * (32 * D) + dc * 512 + (t & 31) * 16);
+      uint16_t *o = ea.k + (int64_t)h * ea.khs + (int64_t)(vw.dst + b * kBlock + t) * D + dc * 16;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const i32x2 lo = decode4<E4M3>((uint32_t)w[2 * m], s, nan), hi = decode4<E4M3>((uint32_t)w[2 * m + 1], s, nan);
+        *(i32x4 *)(o + 8 * m) = i32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    }
+  }
+}
+
+// One 64-token block of K or V of one head as token-major rows: the pack's
+// thread layout run backwards.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(2 * D) kv8_token_major_kernel(const View vw, uint16_t *__restrict__ ko,
+                                                                uint16_t *__restrict__ vo, int32_t heads) {
+  constexpr int L = D / 8;
+  const int tid = threadIdx.x, dl = tid % L, tg = tid / L, h = blockIdx.y >> 1, b = blockIdx.x;
+  const bool is_v = blockIdx.y & 1;
+  const uint8_t *in = (is_v ? vw.v : vw.k) + ((int64_t)h * vw.cap + b * kBlock) * D;
+  const uint32_t byte = (is_v ? vw.vs : vw.ks)[(int64_t)h * (vw.cap / kBlock) + b];
+  const float s = scale_of(byte);
+  uint32_t c[4][2];
+  if (is_v) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 8 * dl + 4 * half + e;
+        w[e] = *(const uint32_t *)(in + (tg >> 3) * (32 * D) + (d >> 5) * 1024 + (tg & 1) * 512 + (d & 31) * 16 + ((tg >> 1) & 3) * 4);
+      }
+      transpose4(w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i][half] = w[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * tg + i;
+      const i32x2 w = *(const i32x2 *)(in + (t >> 5) * (32 * D) + (dl >> 1) * 512 + (t & 31) * 16 + (dl & 1) * 8);
+      c[i][0] = (uint32_t)w[0], c[i][1] = (uint32_t)w[1];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = b * kBlock + 4 * tg + i;
+    if (t >= vw.tokens) break;
+    const i32x2 lo = decode4<E4M3>(c[i][0], s, byte == 255u), hi = decode4<E4M3>(c[i][1], s, byte == 255u);
+    *(i32x4 *)((is_v ? vo : ko) + ((int64_t)t * heads + h) * D + dl * 8) = i32x4{lo[0], lo[1], hi[0], hi[1]};
+  }
+}
+
+// ---- attention of few query rows
+
+struct Seg8 {
+  const uint8_t *k, *v, *ks, *vs;
+  int32_t cap, tokens;
+};
+struct Call8 {
+  const uint16_t *q;
+  uint16_t *o;
+  int64_t qts, qhs, ots, ohs;
+  const int32_t *q_rows, *o_rows;
+  int32_t q_row0, o_row0, lq;
+  int32_t seg0, nseg, blocks;        // its segments, and their 64-token blocks in all
+  int32_t row_tiles, splits, first;  // first: of the launch's workgroups
+  int32_t part0;                     // first partial result (splits > 1)
+};
+struct Args8 {
+  Call8 call[kMaxCalls];
+  Seg8 seg[kMaxSegs];
+  int32_t n_calls, heads;
+  float scale2;  // softmax scale times log2 e
+  float *ws;
+};
+
+constexpr int kWaves8 = 4;
+
+// Rows of a partial result: QB * 32 of D sums, then the maxima and the weights' sums.
+template <int D, int QB>
+constexpr int part_floats() { return QB * 32 * (D + 2); }
+
+// A workgroup takes 32 QB query rows of one head over a range of 64-token blocks;
+// its four waves take the blocks in turn and merge through LDS.  Per 32 keys a
+// lane loads the 16-byte chunks that are its MFMA operands (no LDS on the way:
+// each code is used once, by all query rows) and turns them into bf16, exactly;
+// S^T = K Q^T leaves 16 keys of one query in a lane, in the order in which the
+// V chunks hold them, so P feeds the second product from registers.  A block's K
+// scale joins the softmax scale, its V scale multiplies P (both powers of two).
+// Bound by HBM: 64 rows need 1024 MFMA cycles per 8 KiB and wave, 32 bytes a
+// clock for a CU, against about 11 that HBM delivers to it.
+template <int D, int QB, bool E4M3>
+__global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_eu(QB == 1 ? 2 : 1, QB == 1 ? 2 : 1)))
+kv8_attn_kernel(const Args8 aa) {
+  constexpr int KC = D / 32;   // 16-byte K chunks of a lane per 32 keys, and V chunks (32-channel blocks)
+  constexpr int RS = D + 4;    // floats of a staged row
+  __shared__ __attribute__((aligned(16))) float stage[kWaves8 * 32 * RS];
+  __shared__ float stat[2][kWaves8][32];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, g = lane >> 5;
+  int ci = 0;
+  while (ci + 1 < aa.n_calls && (int)blockIdx.x >= aa.call[ci + 1].first) ++ci;
+  const Call8 &cl = aa.call[ci];
+  int at = (int)blockIdx.x - cl.first;
+  const int split = at % cl.splits;
+  at /= cl.splits;
+  const int tile = at % cl.row_tiles, h = at / cl.row_tiles;
+  const int r0 = tile * 32 * QB;
+  const int b_begin = (int)((int64_t)cl.blocks * split / cl.splits), b_end = (int)((int64_t)cl.blocks * (split + 1) / cl.splits);
+
+  // Q operands: channel 32 j + 16 g + 8 half + e
+  bf16x8 qf[QB][2 * KC];
+#pragma unroll
+  for (int c = 0; c < QB; ++c) {
+    const int r = min(r0 + 32 * c + lr, cl.lq - 1);
+    const int64_t row = cl.q_rows ? cl.q_rows[r] : cl.q_row0 + r;
+    const uint16_t *qp = cl.q + row * cl.qts + (int64_t)h * cl.qhs + 16 * g;
+#pragma unroll
+    for (int t = 0; t < 2 * KC; ++t) qf[c][t] = *(const bf16x8 *)(qp + 32 * (t >> 1) + 8 * (t & 1));
+  }
+  f32x16 acc[QB][KC];
+  float mx[QB], sum[QB];
+#pragma unroll
+  for (int c = 0; c < QB; ++c) {
+    mx[c] = -__builtin_inff();
+    sum[c] = 0.f;
+#pragma unroll
+    for (int d = 0; d < KC; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][d][i] = 0.f;
+  }
+
+  // the segment of the wave's next block, and that segment's first block
+  int si = cl.seg0, s_first = 0;
+  for (int b = b_begin + w; b < b_end; b += kWaves8) {
+    while (b - s_first >= (aa.seg[si].tokens + kBlock - 1) / kBlock) {
+      s_first += (aa.seg[si].tokens + kBlock - 1) / kBlock;
+      ++si;
+    }
+    const Seg8 &sg = aa.seg[si];
+    const int sb = b - s_first;
+    const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D;
+    const int left = sg.tokens - sb * kBlock;  // valid tokens of the block, 1 or more
+    const int64_t s_at = (int64_t)h * (sg.cap / kBlock) + sb;
+    const float kc = scale_of(sg.ks[s_at]) * aa.scale2, vc = scale_of(sg.vs[s_at]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t == 1 && left <= 32) break;
+      i32x4 kr[KC], vr[KC];
+#pragma unroll
+      for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(sg.k + off + t * 32 * D + j * 1024 + lane * 16);
+#pragma unroll
+      for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(sg.v + off + t * 32 * D + j * 1024 + lane * 16);
+      f32x16 s[QB];
+#pragma unroll
+      for (int c = 0; c < QB; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[c][i] = 0.f;
+      auto operand = [](const i32x4 &raw, int half) {
+        const i32x2 lo = decode4<E4M3>((uint32_t)raw[2 * half], 1.0f, false);
+        const i32x2 hi = decode4<E4M3>((uint32_t)raw[2 * half + 1], 1.0f, false);
+        return __builtin_bit_cast(bf16x8, i32x4{lo[0], lo[1], hi[0], hi[1]});
+      };
+#pragma unroll
+      for (int j = 0; j < 2 * KC; ++j) {
+        const bf16x8 kf = operand(kr[j >> 1], j & 1);
+#pragma unroll
+        for (int c = 0; c < QB; ++c) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c][j], s[c], 0, 0, 0);
+      }
+      bf16x8 pf[QB][2];
+#pragma unroll
+      for (int c = 0; c < QB; ++c) {
+        float x[16], top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[i] = s[c][i] * kc;
+          if (t * 32 + 8 * (i >> 2) + 4 * g + (i & 3) >= left) x[i] = -__builtin_inff();
+          top = fmaxf(top, x[i]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > mx[c])) {
+          // (a first tile of NaN scores leaves the maximum at -inf: sums are 0, NaN follows from the scores)
+          const float m = fmaxf(mx[c], top);
+          const float f = m == mx[c] ? 1.0f : __builtin_amdgcn_exp2f(mx[c] - m);
+          mx[c] = m;
+          sum[c] *= f;
+#pragma unroll
+          for (int d = 0; d < KC; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c][d][i] *= f;
+        }
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(x[i] - mx[c]);
+          sum[c] += p[i];
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          i32x4 pk;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pk[e] = (int)pack_bf16_rne(p[8 * m + 2 * e] * vc, p[8 * m + 2 * e + 1] * vc);
+          pf[c][m] = __builtin_bit_cast(bf16x8, pk);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < KC; ++d)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const bf16x8 vf = operand(vr[d], m);
+#pragma unroll
+          for (int c = 0; c < QB; ++c) acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[c][m], acc[c][d], 0, 0, 0);
+        }
+    }
+  }
+
+  // merge of the four waves, 32 rows at a time, in wave order
+#pragma unroll
+  for (int c = 0; c < QB; ++c) {
+    const float l = sum[c] + __shfl_xor(sum[c], 32);
+    if (c) __syncthreads();
+    if (g == 0) stat[0][w][lr] = mx[c], stat[1][w][lr] = l;
+#pragma unroll
+    for (int d = 0; d < KC; ++d)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *(f32x4 *)&stage[(w * 32 + lr) * RS + d * 32 + 8 * u + 4 * g] =
+            f32x4{acc[c][d][4 * u], acc[c][d][4 * u + 1], acc[c][d][4 * u + 2], acc[c][d][4 * u + 3]};
+    __syncthreads();
+    // thread: row tid / 8, channels 4 (tid % 8) + 32 j ..
+    const int r = threadIdx.x >> 3, dq = threadIdx.x & 7, row = r0 + 32 * c + r;
+    if (row < cl.lq) {
+      float m = stat[0][0][r], f[kWaves8], ls = 0.f;
+#pragma unroll
+      for (int i = 1; i < kWaves8; ++i) m = fmaxf(m, stat[0][i][r]);
+#pragma unroll
+      for (int i = 0; i < kWaves8; ++i) {
+        // a wave without blocks has the maximum -inf and sums 0
+        f[i] = stat[0][i][r] == m ? 1.0f : __builtin_amdgcn_exp2f(stat[0][i][r] - m);
+        ls += f[i] * stat[1][i][r];
+      }
+      float *ws = aa.ws + (int64_t)(cl.part0 + (h * cl.row_tiles + tile) * cl.splits + split) * part_floats<D, QB>();
+      const float inv = 1.0f / ls;
+      uint16_t *op = nullptr;
+      if (cl.splits == 1) {
+        const int64_t orow = cl.o_rows ? cl.o_rows[row] : cl.o_row0 + row;
+        op = cl.o + orow * cl.ots + (int64_t)h * cl.ohs;
+      } else if (dq == 0) {
+        ws[QB * 32 * D + 32 * c + r] = m;
+        ws[QB * 32 * (D + 1) + 32 * c + r] = ls;
+      }
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        const int d = 32 * j + 4 * dq;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kWaves8; ++i) v += f[i] * *(const f32x4 *)&stage[(i * 32 + r) * RS + d];
+        if (op)
+          *(i32x2 *)(op + d) = i32x2{(int)pack_bf16_rne(v[0] * inv, v[1] * inv), (int)pack_bf16_rne(v[2] * inv, v[3] * inv)};
+        else
+          *(f32x4 *)&ws[(32 * c + r) * D + d] = v;
+      }
+    }
+  }
+}
+
+// Merge of a call's key ranges: one workgroup per 32 QB rows of a head, in range order.
+template <int D, int QB>
+__global__ void __launch_bounds__(256) kv8_merge_kernel(const Args8 aa) {
+  constexpr int PF = part_floats<D, QB>(), Q4 = D / 4;
+  int at = (int)blockIdx.x, ci = 0;
+  for (;; ++ci) {  // the grid counts the items of the split calls
+    const int items = aa.call[ci].splits > 1 ? aa.heads * aa.call[ci].row_tiles : 0;
+    if (at < items) break;
+    at -= items;
+  }
+  const Call8 &cl = aa.call[ci];
+  const int tile = at % cl.row_tiles, h = at / cl.row_tiles, r0 = tile * 32 * QB;
+  const float *ws = aa.ws + (int64_t)(cl.part0 + at * cl.splits) * PF;
+  for (int i = threadIdx.x; i < min(32 * QB, cl.lq - r0) * Q4; i += 256) {
+    const int r = i / Q4, d = i % Q4 * 4;
+    float m = -__builtin_inff(), l = 0.f;
+    for (int s = 0; s < cl.splits; ++s) m = fmaxf(m, ws[(int64_t)s * PF + QB * 32 * D + r]);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < cl.splits; ++s) {
+      const float *p = ws + (int64_t)s * PF;
+      const float ms = p[QB * 32 * D + r], f = ms == m ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
+      l += f * p[QB * 32 * (D + 1) + r];
+      v += f * *(const f32x4 *)&p[r * D + d];
+    }
+    const int64_t orow = cl.o_rows ? cl.o_rows[r0 + r] : cl.o_row0 + r0 + r;
+    const float inv = 1.0f / l;
+    *(i32x2 *)(cl.o + orow * cl.ots + (int64_t)h * cl.ohs + d) =
+        i32x2{(int)pack_bf16_rne(v[0] * inv, v[1] * inv), (int)pack_bf16_rne(v[2] * inv, v[3] * inv)};
+  }
+}
+
+// ---- host side
+
+int check_heads(const char *what, int32_t heads, int32_t head_dim) {
+  if (heads <= 0 || heads > 32767) return set_error(TMHD_ERR_INVALID, "%s: heads %d", what, heads);
+  if (head_dim != 64 && head_dim != 128) return set_error(TMHD_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
+  return TMHD_OK;
+}
+
+int check_slot(const char *what, const tmhd_kv8_segment &s) {
+  if (!s.k || !s.v || !s.ks || !s.vs || (uintptr_t)s.k % 16 || (uintptr_t)s.v % 16)
+    return set_error(TMHD_ERR_INVALID, "%s: null or misaligned slot", what);
+  if (s.cap <= 0 || s.cap % kBlock || s.cap >= 1 << 23) return set_error(TMHD_ERR_INVALID, "%s: slot capacity %d", what, s.cap);
+  if (s.format != TMHD_KV8_E4M3 && s.format != TMHD_KV8_INT8)
+    return set_error(TMHD_ERR_UNSUPPORTED, "%s: format %d", what, s.format);
+  return TMHD_OK;
+}
+
+int check_view(const char *what, const tmhd_kv8_segment &s) {
+  if (int st = check_slot(what, s)) return st;
+  if (s.row0 < 0 || s.row0 % kBlock || s.tokens <= 0 || (int64_t)s.row0 + s.tokens > s.cap)
+    return set_error(TMHD_ERR_INVALID, "%s: rows [%d, %d + %d) of a slot of %d", what, s.row0, s.row0, s.tokens, s.cap);
+  return TMHD_OK;
+}
+
+View view_of(const tmhd_kv8_segment &s, int D) {
+  return View{(const uint8_t *)s.k + (int64_t)s.row0 * D, (const uint8_t *)s.v + (int64_t)s.row0 * D,
+              s.ks + s.row0 / kBlock, s.vs + s.row0 / kBlock, s.cap, s.tokens, 0, 0};
+}
+
+template <typename F>
+void dispatch(int D, int format, F &&f) {
+  using std::integral_constant;
+  if (D == 128)
+    format == TMHD_KV8_E4M3 ? f(integral_constant<int, 128>{}, std::true_type{}) : f(integral_constant<int, 128>{}, std::false_type{});
+  else
+    format == TMHD_KV8_E4M3 ? f(integral_constant<int, 64>{}, std::true_type{}) : f(integral_constant<int, 64>{}, std::false_type{});
+}
+
+// How many query rows a workgroup takes (32 QB), and the key ranges of each call.
+struct Plan8 {
+  int qb;
+  int64_t wgs, parts, merge_items;
+};
+
+int blocks_of(const tmhd_kv8_call &c) {
+  int64_t b = 0;
+  for (int i = 0; i < c.n_segments; ++i) b += (c.seg[i].tokens + kBlock - 1) / kBlock;
+  return (int)std::min<int64_t>(b, INT32_MAX);
+}
+
+// The calls [0, n) of one launch.  The blocks of all items are dealt to about
+// two workgroups per CU (one with 64 rows), at least two blocks a wave.
+Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
+  Plan8 p{1, 0, 0, 0};
+  int32_t most = 0;
+  for (int i = 0; i < n; ++i) most = std::max(most, calls[i].lq);
+  p.qb = most > 32 ? 2 : 1;
+  int64_t total = 0;
+  for (int i = 0; i < n; ++i)
+    total += (int64_t)heads * ((calls[i].lq + 32 * p.qb - 1) / (32 * p.qb)) * blocks_of(calls[i]);
+  const int64_t room = (int64_t)std::max(device_cus(), 1) * (p.qb == 1 ? 2 : 1);
+  const int64_t each = std::max<int64_t>(2 * kWaves8, (total + room - 1) / room);
+  for (int i = 0; i < n; ++i) {
+    Call8 c{};
+    c.lq = calls[i].lq;
+    c.blocks = blocks_of(calls[i]);
+    c.row_tiles = (int32_t)(((int64_t)c.lq + 32 * p.qb - 1) / (32 * p.qb));
+    c.splits = c.lq > 0 ? (int32_t)((c.blocks + each - 1) / each) : 1;
+    c.first = (int32_t)std::min<int64_t>(p.wgs, INT32_MAX);
+    c.part0 = (int32_t)std::min<int64_t>(p.parts, INT32_MAX);
+    const int64_t items = (int64_t)heads * c.row_tiles;
+    p.wgs += items * c.splits;
+    if (c.splits > 1) {
+      p.parts += items * c.splits;
+      p.merge_items += items;
+    }
+    if (out) out[i] = c;
+  }
+  return p;
+}
+
+// Calls of the launch that starts at calls[i]
+int group_end(const tmhd_kv8_call *calls, int n, int i) {
+  int segs = 0, e = i;
+  while (e < n && e - i < kMaxCalls && segs + calls[e].n_segments <= kMaxSegs) segs += calls[e++].n_segments;
+  return e;
+}
+
+int check_calls(const char *what, const tmhd_kv8_call *calls, int n) {
+  for (int i = 0; i < n; ++i) {
+    const tmhd_kv8_call &c = calls[i];
+    if (c.lq < 0) return set_error(TMHD_ERR_INVALID, "%s: %d query rows", what, c.lq);
+    if (c.n_segments <= 0 || c.n_segments > TMHD_MAX_SEGMENTS)
+      return set_error(TMHD_ERR_INVALID, "%s: %d segments (1 .. %d)", what, c.n_segments, TMHD_MAX_SEGMENTS);
+    for (int j = 0; j < c.n_segments; ++j) {
+      if (int st = check_view(what, c.seg[j])) return st;
+      if (c.seg[j].format != calls[0].seg[0].format)
+        return set_error(TMHD_ERR_UNSUPPORTED, "%s: segments of both formats in one call", what);
+    }
+    if (c.lq == 0) continue;
+    if (!c.q || !c.o || (uintptr_t)c.q % 16 || (uintptr_t)c.o % 8 || c.q_token_stride % 8 || c.q_head_stride % 8 ||
+        c.o_token_stride % 4 || c.o_head_stride % 4)
+      return set_error(TMHD_ERR_INVALID, "%s: queries need 16-byte and outputs 8-byte aligned rows", what);
+    if ((!c.q_rows && c.q_row0 < 0) || (!c.o_rows && c.o_row0 < 0))
+      return set_error(TMHD_ERR_INVALID, "%s: first row %d, %d", what, c.q_row0, c.o_row0);
+  }
+  return TMHD_OK;
+}
+
+template <int D, bool E4M3>
+void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
+  if (p.qb == 1)
+    hipLaunchKernelGGL((kv8_attn_kernel<D, 1, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
+  else
+    hipLaunchKernelGGL((kv8_attn_kernel<D, 2, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
+  if (p.merge_items == 0) return;
+  if (p.qb == 1)
+    hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((unsigned)p.merge_items), dim3(256), 0, s, aa);
+  else
+    hipLaunchKernelGGL((kv8_merge_kernel<D, 2>), dim3((unsigned)p.merge_items), dim3(256), 0, s, aa);
+}
+
+int64_t parts_bytes(const Plan8 &p, int D) { return p.parts * (32 * p.qb) * (D + 2) * 4; }
+
+}  // namespace
+}  // namespace tmhd
+
+extern "C" int tmhd_kv8_pack_ranges(const void *k, const void *v, int64_t token_stride, int64_t head_stride,
+                                    const tmhd_pack_range *ranges, int32_t n_ranges, const tmhd_kv8_segment *slot,
+                                    int32_t heads, int32_t head_dim, void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_kv8_pack";
+  if (int st = check_heads(what, heads, head_dim)) return st;
+  if (n_ranges < 0 || (n_ranges > 0 && !ranges) || !slot) return set_error(TMHD_ERR_INVALID, "%s: %d ranges", what, n_ranges);
+  if (int st = check_slot(what, *slot)) return st;
+  bool any = false;
+  for (int i = 0; i < n_ranges; ++i) {
+    const tmhd_pack_range &r = ranges[i];
+    if (r.n < 0 || r.dst < 0 || r.dst % kBlock || (int64_t)r.dst + r.n > slot->cap || (!r.rows && r.row0 < 0))
+      return set_error(TMHD_ERR_INVALID, "%s: %d rows to slot row %d of %d", what, r.n, r.dst, slot->cap);
+    for (int j = 0; j < i; ++j)
+      if (r.n > 0 && ranges[j].n > 0 && r.dst < (ranges[j].dst + ranges[j].n + kBlock - 1) / kBlock * kBlock &&
+          ranges[j].dst < (r.dst + r.n + kBlock - 1) / kBlock * kBlock)
+        return set_error(TMHD_ERR_INVALID, "%s: ranges %d and %d share a 64-row block of the slot", what, j, i);
+    any = any || r.n > 0;
+  }
+  if (!any) return TMHD_OK;
+  if (!k || !v || (uintptr_t)k % 16 || (uintptr_t)v % 16 || token_stride % 8 || head_stride % 8)
+    return set_error(TMHD_ERR_INVALID, "%s: K/V rows must be 16-byte aligned", what);
+  PackArgs pa{(const uint16_t *)k, (const uint16_t *)v, token_stride, head_stride, (uint8_t *)slot->k, (uint8_t *)slot->v,
+              (uint8_t *)slot->ks, (uint8_t *)slot->vs, slot->cap, 0, {}};
+  for (int i = 0; i < n_ranges;) {
+    int32_t blocks = 0;
+    pa.n_ranges = 0;
+    for (; i < n_ranges && pa.n_ranges < kMaxRanges; ++i) {
+      if (ranges[i].n == 0) continue;
+      auto &r = pa.r[pa.n_ranges++];
+      r.rows = ranges[i].rows, r.row0 = ranges[i].row0, r.n = ranges[i].n, r.dst = ranges[i].dst, r.first = blocks;
+      blocks += (ranges[i].n + kBlock - 1) / kBlock;
+    }
+    if (blocks == 0) break;
+    dispatch(head_dim, slot->format, [&](auto d, auto e4m3) {
+      hipLaunchKernelGGL((kv8_pack_kernel<d.value, e4m3.value>), dim3((unsigned)blocks, (unsigned)heads * 2),
+                         dim3(2 * d.value), 0, (hipStream_t)stream, pa);
+    });
+    if (int st = check_launch(what)) return st;
+  }
+  return TMHD_OK;
+}
+
+extern "C" int tmhd_kv8_expand(const tmhd_kv8_segment *views, const int32_t *dst, int32_t n, void *k_slot,
+                               void *vt_slot, int64_t k_head_stride, int64_t vt_head_stride, int32_t vt_row_stride,
+                               int32_t heads, int32_t head_dim, void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_kv8_expand";
+  if (int st = check_heads(what, heads, head_dim)) return st;
+  if (n < 0 || (n > 0 && (!views || !dst))) return set_error(TMHD_ERR_INVALID, "%s: %d views", what, n);
+  if (n == 0) return TMHD_OK;
+  if (!k_slot || !vt_slot || (uintptr_t)k_slot % 16 || (uintptr_t)vt_slot % 16 || k_head_stride % 8 || vt_head_stride % 8 ||
+      vt_row_stride % 8 || vt_head_stride < (int64_t)head_dim * vt_row_stride)
+    return set_error(TMHD_ERR_INVALID, "%s: null or misaligned slot", what);
+  for (int i = 0; i < n; ++i) {
+    if (int st = check_view(what, views[i])) return st;
+    const int64_t end = (int64_t)dst[i] + (views[i].tokens + kBlock - 1) / kBlock * kBlock;
+    if (dst[i] < 0 || dst[i] % kBlock || end > vt_row_stride || end * head_dim > k_head_stride)
+      return set_error(TMHD_ERR_INVALID, "%s: view %d of %d rows at slot row %d", what, i, views[i].tokens, dst[i]);
+  }
+  for (int i = 0; i < n;) {
+    ExpandArgs ea{(uint16_t *)k_slot, (uint16_t *)vt_slot, k_head_stride, vt_head_stride, vt_row_stride, 0, {}};
+    const int format = views[i].format;  // a launch expands views of one format
+    int32_t blocks = 0;
+    for (; i < n && ea.n_views < kMaxSegs && views[i].format == format; ++i) {
+      View &vw = ea.view[ea.n_views++];
+      vw = view_of(views[i], head_dim);
+      vw.dst = dst[i], vw.first = blocks;
+      blocks += (views[i].tokens + kBlock - 1) / kBlock;
+    }
+    dispatch(head_dim, format, [&](auto d, auto e4m3) {
+      hipLaunchKernelGGL((kv8_expand_kernel<d.value, e4m3.value>), dim3((unsigned)blocks, (unsigned)heads * 2),
+                         dim3(2 * d.value), 0, (hipStream_t)stream, ea);
+    });
+    if (int st = check_launch(what)) return st;
+  }
+  return TMHD_OK;
+}
+
+extern "C" int tmhd_kv8_token_major(const tmhd_kv8_segment *view, void *k, void *v, int32_t heads, int32_t head_dim,
+                                    void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_kv8_token_major";
+  if (int st = check_heads(what, heads, head_dim)) return st;
+  if (!view) return set_error(TMHD_ERR_INVALID, "%s: null view", what);
+  if (int st = check_view(what, *view)) return st;
+  if (!k || !v || (uintptr_t)k % 16 || (uintptr_t)v % 16) return set_error(TMHD_ERR_INVALID, "%s: null or misaligned output", what);
+  const View vw = view_of(*view, head_dim);
+  dispatch(head_dim, view->format, [&](auto d, auto e4m3) {
+    hipLaunchKernelGGL((kv8_token_major_kernel<d.value, e4m3.value>),
+                       dim3((unsigned)((view->tokens + kBlock - 1) / kBlock), (unsigned)heads * 2), dim3(2 * d.value), 0,
+                       (hipStream_t)stream, vw, (uint16_t *)k, (uint16_t *)v, heads);
+  });
+  return check_launch(what);
+}
+
+extern "C" int64_t tmhd_attn_kv8_workspace_bytes(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim) {
+  using namespace tmhd;
+  if (n <= 0 || !calls || check_heads("tmhd_attn_kv8_workspace_bytes", heads, head_dim) ||
+      check_calls("tmhd_attn_kv8_workspace_bytes", calls, n))
+    return 0;
+  int64_t most = 0;
+  for (int i = 0; i < n;) {
+    const int e = group_end(calls, n, i);
+    most = std::max(most, parts_bytes(plan(calls + i, e - i, heads, nullptr), head_dim));
+    i = e;
+  }
+  return most;
+}
+
+extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim, float scale,
+                                 void *workspace, int64_t workspace_bytes, void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_attn_fwd_kv8";
+  if (int st = check_heads(what, heads, head_dim)) return st;
+  if (n < 0 || (n > 0 && !calls)) return set_error(TMHD_ERR_INVALID, "%s: %d calls", what, n);
+  if (int st = check_calls(what, calls, n)) return st;
+  if (workspace && (uintptr_t)workspace % 16) return set_error(TMHD_ERR_INVALID, "%s: misaligned workspace", what);
+  for (int i = 0; i < n;) {
+    const int e = group_end(calls, n, i);
+    Args8 aa{};
+    const Plan8 p = plan(calls + i, e - i, heads, aa.call);
+    if (p.wgs > INT32_MAX || p.parts > INT32_MAX) return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows", what);
+    if (parts_bytes(p, head_dim) > (workspace ? workspace_bytes : 0))
+      return set_error(TMHD_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,
+                       (long long)parts_bytes(p, head_dim));
+    aa.n_calls = e - i;
+    aa.heads = heads;
+    aa.scale2 = scale * 1.4426950408889634f;
+    aa.ws = (float *)workspace;
+    int segs = 0;
+    for (int c = 0; c < aa.n_calls; ++c) {
+      const tmhd_kv8_call &in = calls[i + c];
+      Call8 &o = aa.call[c];
+      o.q = (const uint16_t *)in.q, o.o = (uint16_t *)in.o;
+      o.qts = in.q_token_stride, o.qhs = in.q_head_stride, o.ots = in.o_token_stride, o.ohs = in.o_head_stride;
+      o.q_rows = in.q_rows, o.o_rows = in.o_rows, o.q_row0 = in.q_row0, o.o_row0 = in.o_row0;
+      o.seg0 = segs, o.nseg = in.n_segments;
+      for (int j = 0; j < in.n_segments; ++j) {
+        const View vw = view_of(in.seg[j], head_dim);
+        aa.seg[segs++] = Seg8{vw.k, vw.v, vw.ks, vw.vs, vw.cap, vw.tokens};
+      }
+    }
+    if (p.wgs > 0) {
+      const int format = calls[i].seg[0].format;
+      dispatch(head_dim, format, [&](auto d, auto e4m3) { launch_attn<d.value, e4m3.value>(aa, p, (hipStream_t)stream); });
+      if (int st = check_launch(what)) return st;
+    }
+    i = e;
+  }
+  return TMHD_OK;
+}

@@ -62,7 +62,7 @@ from .quant import (
     scaled_int8_quant,
 )
 from .session import H3StreamingSession, StreamingInferencePolicy, StreamingSession, apply_cross_chunk_cache_policy
-from .slots import KVSlot, SlotPool, SlotView, vt_position
+from .slots import KVSlot, KVSlot8, SlotPool, SlotView, vt_position
 from .w8a8 import (
     CutlassW8A8Workspace,
     W8A8Workspace,
@@ -105,6 +105,7 @@ __all__ = [
     "HookMode",
     "KVContract",
     "KVSlot",
+    "KVSlot8",
     "MAIN_LAYER_NAMES",
     "QKQuantWorkspace",
     "STREAM_HOOK_ABI",

@@ -90,6 +90,37 @@ class PackRange(ctypes.Structure):
     ]
 
 
+class KV8Segment(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("ks", c_void_p),
+        ("vs", c_void_p),
+        ("cap", c_int32),
+        ("row0", c_int32),
+        ("tokens", c_int32),
+        ("format", c_int32),
+    ]
+
+
+class KV8Call(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("q_token_stride", c_int64),
+        ("q_head_stride", c_int64),
+        ("q_rows", c_void_p),
+        ("q_row0", c_int32),
+        ("lq", c_int32),
+        ("o", c_void_p),
+        ("o_token_stride", c_int64),
+        ("o_head_stride", c_int64),
+        ("o_rows", c_void_p),
+        ("o_row0", c_int32),
+        ("n_segments", c_int32),
+        ("seg", KV8Segment * MAX_SEGMENTS),
+    ]
+
+
 _SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "tmhd_version": (c_char_p, []),
     "tmhd_last_error": (c_char_p, []),
@@ -231,6 +262,21 @@ _LOWBIT_SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_int64,
          c_int64, c_void_p],
     ),
+    "tmhd_kv8_pack_ranges": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_int64, POINTER(PackRange), c_int32, POINTER(KV8Segment), c_int32, c_int32,
+         c_void_p],
+    ),
+    "tmhd_kv8_expand": (
+        c_int,
+        [POINTER(KV8Segment), POINTER(c_int32), c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32,
+         c_int32, c_void_p],
+    ),
+    "tmhd_kv8_token_major": (c_int, [POINTER(KV8Segment), c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    "tmhd_attn_fwd_kv8": (
+        c_int, [POINTER(KV8Call), c_int32, c_int32, c_int32, c_float, c_void_p, c_int64, c_void_p],
+    ),
+    "tmhd_attn_kv8_workspace_bytes": (c_int64, [POINTER(KV8Call), c_int32, c_int32, c_int32]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)  # of include/tmhd.h

@@ -7,19 +7,25 @@ does over the concatenated K/V in the reference
 (src/taomate_hd/streaming/attention_hook.py:100-115).  ``backend="i8qk"`` runs
 the SageAttention-style variant (smooth-K, per-128-block INT8 Q/K, bf16 P.V;
 ref attention_hook.py:335-371, inference/sage_value_padding.py:79-97).
+
+Segments may lie in slots held in 8 bits (``KVSlot8``).  A ``"bf16"`` call of
+up to ``KV8_ROWS`` query rows whose segments all do, in one format, reads their
+codes in place (``tmhd_attn_fwd_kv8``); for any other call they are expanded
+to bf16 first, which is exact, and the call runs as over bf16 slots.
 """
 
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Any, Sequence
 
 from . import _native
 from .profiling import ComponentTimer, maybe_region
-from .slots import KV_TILE, KVSlot, SlotView, round_up, vt_columns
+from .slots import KV_TILE, KVSlot, KVSlot8, SlotView, expand_views, round_up, vt_columns
 
 BACKENDS = ("bf16", "i8qk")
+KV8_ROWS = 64  # query rows up to which 8-bit segments are read in place
 
 
 class QKQuantWorkspace:
@@ -220,7 +226,8 @@ def segment_attention(
     timer: ComponentTimer | None = None,
     rows_checked: bool = False,
 ) -> Any:
-    """Attention of the selected query rows over ``segments`` (in place, no mask).
+    """Attention of the selected query rows over ``segments`` (no mask; bf16 slots are
+    read in place, 8-bit ones too by a ``"bf16"`` call of few query rows).
 
     Query row ``i`` is ``query[q_rows[i]]`` (or ``query[q_row0 + i]``); its
     output goes to ``out[o_rows[i]]`` (or ``out[o_row0 + i]``).  Without
@@ -306,13 +313,82 @@ def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: l
     args.o_head_stride = out.stride(1)
     args.o_rows = _native.ptr(o_rows) if o_rows is not None and lq else None
     args.o_row0 = o_row0
+    args.n_segments = len(segments)
+    if isinstance(args, _native.KV8Call):
+        for i, s in enumerate(segments):
+            s.slot.fill_segment8(args.seg[i], s.row0, s.tokens)
+        return out, segments
     args.heads = heads
     args.head_dim = head_dim
     args.scale = scale
-    args.n_segments = len(segments)
     for i, s in enumerate(segments):
         s.fill_segment(args.seg[i])
     return out, segments
+
+
+def _rows_of(call: AttentionCall) -> int:
+    """Query rows of a call (its arguments not checked yet)."""
+    if call.q_rows is not None:
+        return int(call.q_rows.numel()) if hasattr(call.q_rows, "numel") else KV8_ROWS + 1
+    return int(call.query.shape[0]) - int(call.q_row0) if call.lq is None else int(call.lq)
+
+
+def _in_place_format(call: AttentionCall) -> str | None:
+    """The format of the 8-bit segments that a call reads in place, if it does."""
+    segments = [s for s in call.segments if s.tokens > 0]
+    formats = {s.slot.format if isinstance(s.slot, KVSlot8) else None for s in segments}
+    if len(formats) != 1 or len(segments) > _native.MAX_SEGMENTS or _rows_of(call) > KV8_ROWS:
+        return None
+    return formats.pop()
+
+
+def _attend_in_place(torch: Any, calls: Sequence[AttentionCall], scale: float, timer: ComponentTimer | None) -> list[Any]:
+    """Calls of few query rows over 8-bit segments of one format, in one launch (per 16 calls and 24 segments)."""
+    keep: list[Any] = []
+    args = (_native.KV8Call * len(calls))()
+    outs = [_call_args(torch, call, args[i], scale, keep)[0] for i, call in enumerate(calls)]
+    query = calls[0].query
+    heads, head_dim = int(query.shape[1]), int(query.shape[2])
+    if any(call.query.device != query.device or out.device != query.device or tuple(call.query.shape[1:]) != (heads, head_dim)
+           for call, out in zip(calls, outs)):
+        raise ValueError("the queries and outputs of a batch must share heads, head_dim and one GPU")
+    lib = _native.load()
+    with _native.device_of(torch, query), maybe_region(timer, "attention"):
+        need = int(lib.tmhd_attn_kv8_workspace_bytes(args, len(calls), heads, head_dim))
+        # from the caching allocator each time: ordered with its stream, and a captured graph's own
+        ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+        status = lib.tmhd_attn_fwd_kv8(args, len(calls), heads, head_dim, scale, _native.ptr(ws) if need else None, need,
+                                       _native.stream_ptr(torch, query.device))
+    _native.check(status, "tmhd_attn_fwd_kv8")
+    return outs
+
+
+def _attend_8bit(torch: Any, calls: Sequence[AttentionCall], **options: Any) -> tuple[list[Any], list[dict[str, Any]]]:
+    """``segment_attention_batch`` of calls some of whose segments are held in 8 bits."""
+    scale, timer = float(options["scale"]), options["timer"]
+    for call in calls:
+        _validate_tokens_major(torch, call.query, "query")
+        for s in call.segments:
+            if s.tokens > 0 and (s.slot.heads, s.slot.head_dim, s.slot.device) != (*call.query.shape[1:], call.query.device):
+                raise ValueError("segment heads/dim/device differ from the query")
+    formats = [_in_place_format(call) if options["backend"] == "bf16" else None for call in calls]
+    outs: list[Any] = [None] * len(calls)
+    for fmt in dict.fromkeys(f for f in formats if f is not None):
+        at = [i for i, f in enumerate(formats) if f == fmt]
+        for i, out in zip(at, _attend_in_place(torch, [calls[i] for i in at], scale, timer)):
+            outs[i] = out
+    rest = [i for i, f in enumerate(formats) if f is None]
+    views: list[dict[str, Any]] = []
+    if rest:
+        segments = [[s for s in calls[i].segments if s.tokens > 0] for i in rest]
+        with maybe_region(timer, "expand"):
+            expanded = iter(expand_views(torch, [s for segs in segments for s in segs]))
+        for i, segs in zip(rest, segments):
+            calls[i] = replace(calls[i], segments=[next(expanded) for _ in segs])
+        got, views = segment_attention_batch(torch, [calls[i] for i in rest], **options)
+        for i, out in zip(rest, got):
+            outs[i] = out
+    return outs, views
 
 
 def segment_attention_batch(
@@ -336,6 +412,9 @@ def segment_attention_batch(
         raise ValueError(f"unknown attention backend {backend!r}")
     if not calls:
         return [], []
+    if any(isinstance(s.slot, KVSlot8) for call in calls for s in call.segments if s.tokens > 0):
+        return _attend_8bit(torch, list(calls), scale=scale, backend=backend, workspace=workspace, split=split,
+                            return_quant=return_quant, timer=timer)
     keep: list[Any] = []  # row lists and merged slots, alive until the launches are queued
     args = (_native.AttnArgs * len(calls))()
     outs, segments = [], []

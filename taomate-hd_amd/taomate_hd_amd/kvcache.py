@@ -26,7 +26,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Any, Sequence
 
-from .slots import KVSlot, SlotPool, SlotView
+from .slots import STORAGES, KVSlot, SlotPool, SlotView
 
 MAIN_LAYER_NAMES = tuple(f"blocks.{index}.attn" for index in range(50))
 VIDEO_TOKEN_TAG = 0
@@ -94,10 +94,19 @@ class _Block:
 
 
 class HeadMajorRingKVCache:
-    """Persistent post-RoPE media history committed only from clean AV states."""
+    """Persistent post-RoPE media history committed only from clean AV states.
 
-    def __init__(self, contract: KVContract | None = None) -> None:
+    ``storage`` is how the blocks are held: ``"bf16"`` as staged, or ``"e4m3"``
+    / ``"int8"`` in 8 bits (``KVSlot8``; no counterpart in the reference), half
+    the memory.  The rows a clean commit stages are then attended as they will
+    be read later, from their 8-bit form, in that step already.
+    """
+
+    def __init__(self, contract: KVContract | None = None, *, storage: str = "bf16") -> None:
+        if storage not in STORAGES:
+            raise ValueError(f"unknown K/V storage {storage!r} (one of {STORAGES})")
         self.contract = contract or KVContract()
+        self.storage = storage
         self._blocks: list[_Block] = []
         self._staged: _Block | None = None
         self._staged_commit_indices: Any | None = None
@@ -308,7 +317,7 @@ class HeadMajorRingKVCache:
             # back: keep up to two blocks' worth free
             self._pool = SlotPool(
                 torch, heads=self.contract.local_heads, head_dim=self.contract.head_dim, device=device,
-                max_free=2 * len(self.contract.layer_names),
+                max_free=2 * len(self.contract.layer_names), storage=self.storage,
             )
             self._device = torch.device(device)
         elif torch.device(device) != self._device:

@@ -78,8 +78,10 @@ def fused_qkv_qk_norm_rope_stage_(qkv: Any, q_weight: Any, k_weight: Any, cos_si
     K.  Returns ``qkv``."""
     import torch
 
-    from .slots import KV_TILE, round_up
+    from .slots import KV_TILE, KVSlot8, round_up
 
+    if isinstance(slot, KVSlot8):
+        raise ValueError(f"the staged norm + RoPE writes bf16 slots, not one held in {slot.storage}")
     tokens, heads, head_dim, positions, cache, rotary_dim, q_weight, k_weight = _merged_qkv_args(
         torch, qkv, q_weight, k_weight, cos_sin_cache, positions)
     if (slot.heads, slot.head_dim) != (heads, head_dim) or slot.device != qkv.device:

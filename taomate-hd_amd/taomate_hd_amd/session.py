@@ -81,15 +81,18 @@ class StreamingSession:
         fused_history_recent_blocks: int | None = None,
         condition_attention_cached: Callable[[str, int], bool] | None = None,
         compact_condition_attention_output: Callable[[str, Any], Any] | None = None,
+        kv_storage: str | None = None,
     ) -> None:
         if not hasattr(plan, "phases"):
             raise TypeError("plan must be a StreamPlan")
         if cache is not None and contract is not None and cache.contract != contract:
             raise ValueError("injected clean cache and KV contract differ")
+        if cache is not None and kv_storage is not None and cache.storage != kv_storage:
+            raise ValueError("injected clean cache and K/V storage differ")
         if cache is None:
             if contract is None and model is not None:
                 contract = kv_contract_from_model(model)
-            cache = HeadMajorRingKVCache(contract)
+            cache = HeadMajorRingKVCache(contract, storage=kv_storage or "bf16")
         self.plan = plan
         self.cache = cache
         # local block i of the plan is global block base + i of the cache

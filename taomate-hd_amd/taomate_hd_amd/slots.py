@@ -12,6 +12,12 @@ round_up(tokens, 64))`` are kept zero, so a tile never reads stale data.
 Slots are filled only by ``tmhd_kv_pack`` (``KVSlot.pack``) and the staged
 norm + RoPE, which also drop the slot's memo of key sums (``key_sums``, kept
 for the INT8-QK smooth-K mean); attention reads them in place.
+
+``KVSlot8`` is the same unit held in 8 bits (e4m3 or int8 codes with a
+power-of-two scale for each 64 tokens of a head; layout in
+include/tmhd_lowbit.h): half the memory, written by its quantizing ``pack``.
+Attention of few query rows reads its codes in place; other readers expand it
+to bf16 first, which is exact.
 """
 
 from __future__ import annotations
@@ -61,6 +67,8 @@ class SlotView:
 
     def fill_segment(self, segment: _native.KVSegment) -> _native.KVSegment:
         s = self.slot
+        if isinstance(s, KVSlot8):
+            raise ValueError(f"a slot held in {s.storage} has no bf16 segment (expand_views)")
         row0, tokens = int(self.row0), int(self.tokens)
         if row0 % KV_TILE or row0 + round_up(tokens, KV_TILE) > s.capacity:
             raise ValueError(f"slot view rows [{row0}, {row0 + tokens}) are not a tile-aligned part of the slot")
@@ -95,8 +103,7 @@ class KVSlot:
         if self.capacity > MAX_SLOT_CAPACITY:
             raise ValueError(f"slot capacity {self.capacity} above the {MAX_SLOT_CAPACITY} tokens a slot can hold")
         self.device = torch.device(device)
-        self.k = torch.empty((self.heads, self.capacity, self.head_dim), dtype=torch.bfloat16, device=self.device)
-        self.vt = torch.empty((self.heads, self.head_dim, self.capacity), dtype=torch.bfloat16, device=self.device)
+        self._allocate(torch)
         self.tokens = 0
         # handle of the stream whose allocation pool the memory came from
         self.allocated_on = _native.stream_ptr(torch, self.device) if self.k.is_cuda else 0
@@ -106,9 +113,21 @@ class KVSlot:
         # int64 [H, D]; dropped whenever the slot is written (pack, staged norm + RoPE)
         self.key_sums: dict[tuple[int, int, int], Any] = {}
 
+    def _allocate(self, torch: Any) -> None:
+        self.k = torch.empty((self.heads, self.capacity, self.head_dim), dtype=torch.bfloat16, device=self.device)
+        self.vt = torch.empty((self.heads, self.head_dim, self.capacity), dtype=torch.bfloat16, device=self.device)
+
+    @property
+    def storage(self) -> str:
+        return "bf16"
+
+    def buffers(self) -> tuple[Any, ...]:
+        """The slot's device memory."""
+        return self.k, self.vt
+
     @property
     def nbytes(self) -> int:
-        return 2 * self.k.numel() * self.k.element_size()
+        return sum(t.numel() * t.element_size() for t in self.buffers())
 
     def view(self, tokens: int | None = None) -> SlotView:
         count = self.tokens if tokens is None else int(tokens)
@@ -170,14 +189,17 @@ class KVSlot:
             r.n, r.dst, r.zero_to = n, dst, dst + round_up(n, KV_TILE)
             end = dst + n
         self.key_sums.clear()
+        self._launch_pack(key, value, table, len(ranges))
+        self.tokens = end
+
+    def _launch_pack(self, key: Any, value: Any, table: Any, count: int) -> None:
         stride = self.capacity * self.head_dim
         status = _native.load().tmhd_kv_pack_ranges(
-            _native.ptr(key), _native.ptr(value), key.stride(0), key.stride(1), table, len(ranges),
+            _native.ptr(key), _native.ptr(value), key.stride(0), key.stride(1), table, count,
             _native.ptr(self.k), _native.ptr(self.vt), stride, stride, self.capacity, self.heads, self.head_dim,
-            _native.stream_ptr(torch, key.device),
+            _native.stream_ptr(self._torch, key.device),
         )
         _native.check(status, "tmhd_kv_pack")
-        self.tokens = end
 
     def token_major(self, tokens: int | None = None, order: Any | None = None) -> tuple[Any, Any]:
         """Materialise ``[tokens, H, D]`` key/value copies (compatibility path)."""
@@ -190,6 +212,118 @@ class KVSlot:
             key = key.index_select(0, order)
             value = value.index_select(0, order)
         return key, value
+
+
+KV8_FORMATS = ("e4m3", "int8")  # by their number in the C ABI
+STORAGES = ("bf16", *KV8_FORMATS)
+
+
+class KVSlot8(KVSlot):
+    """One key/value block held in 8 bits (see module docstring).
+
+    Per 64 slot rows of a head, keys and values apart, the scale is the least
+    power of two (not below 2^-117) that brings the largest magnitude to the
+    format's range (448 for ``"e4m3"``, 127 for ``"int8"``); codes are rounded
+    to nearest even.  A block that holds an infinity or NaN reads back as NaN.
+    """
+
+    def __init__(self, torch: Any, *, heads: int, head_dim: int, capacity: int, device: Any, fmt: str = "e4m3") -> None:
+        if fmt not in KV8_FORMATS:
+            raise ValueError(f"unknown 8-bit K/V format {fmt!r} (one of {KV8_FORMATS})")
+        if int(head_dim) not in (64, 128):
+            raise ValueError(f"8-bit K/V slots take a head_dim of 64 or 128, got {head_dim}")
+        self.format = fmt
+        super().__init__(torch, heads=heads, head_dim=head_dim, capacity=capacity, device=device)
+
+    def _allocate(self, torch: Any) -> None:
+        blocks = self.capacity // KV_TILE
+        shape = (self.heads, self.capacity * self.head_dim)
+        self.k = torch.empty(shape, dtype=torch.uint8, device=self.device)
+        self.vt = torch.empty(shape, dtype=torch.uint8, device=self.device)
+        self.k_scale = torch.empty((self.heads, blocks), dtype=torch.uint8, device=self.device)
+        self.v_scale = torch.empty((self.heads, blocks), dtype=torch.uint8, device=self.device)
+
+    @property
+    def storage(self) -> str:
+        return self.format
+
+    def buffers(self) -> tuple[Any, ...]:
+        return self.k, self.vt, self.k_scale, self.v_scale
+
+    def fill_segment8(self, segment: _native.KV8Segment, row0: int = 0, tokens: int | None = None) -> _native.KV8Segment:
+        row0, tokens = int(row0), self.tokens if tokens is None else int(tokens)
+        if row0 < 0 or row0 % KV_TILE or tokens < 0 or row0 + round_up(tokens, KV_TILE) > self.capacity:
+            raise ValueError(f"slot view rows [{row0}, {row0 + tokens}) are not a tile-aligned part of the slot")
+        segment.k, segment.v = _native.ptr(self.k), _native.ptr(self.vt)
+        segment.ks, segment.vs = _native.ptr(self.k_scale), _native.ptr(self.v_scale)
+        segment.cap, segment.row0, segment.tokens = self.capacity, row0, tokens
+        segment.format = KV8_FORMATS.index(self.format)
+        return segment
+
+    def _launch_pack(self, key: Any, value: Any, table: Any, count: int) -> None:
+        torch = self._torch
+        _native.require_same_gpu(torch, self.k.device, key=key, value=value)
+        with _native.device_of(torch, key):
+            status = _native.load().tmhd_kv8_pack_ranges(
+                _native.ptr(key), _native.ptr(value), key.stride(0), key.stride(1), table, count,
+                self.fill_segment8(_native.KV8Segment()), self.heads, self.head_dim, _native.stream_ptr(torch, key.device),
+            )
+        _native.check(status, "tmhd_kv8_pack")
+
+    def token_major(self, tokens: int | None = None, order: Any | None = None) -> tuple[Any, Any]:
+        """The values as ``[tokens, H, D]`` bf16 key/value copies (exact)."""
+        torch = self._torch
+        n = self.tokens if tokens is None else int(tokens)
+        key = torch.empty((n, self.heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
+        value = torch.empty_like(key)
+        if n:
+            with _native.device_of(torch, key):
+                status = _native.load().tmhd_kv8_token_major(
+                    self.fill_segment8(_native.KV8Segment(), 0, n), _native.ptr(key), _native.ptr(value), self.heads,
+                    self.head_dim, _native.stream_ptr(torch, self.device),
+                )
+            _native.check(status, "tmhd_kv8_token_major")
+        if order is not None:
+            key, value = key.index_select(0, order), value.index_select(0, order)
+        return key, value
+
+
+def expand_views(torch: Any, views: Sequence[SlotView]) -> list[SlotView]:
+    """The 8-bit views among ``views`` (one head count, head_dim and device)
+    as views of one new bf16 slot, each distinct one expanded once, in one
+    launch per 24; bf16 views are returned as they are."""
+    places: dict[tuple[int, int, int], tuple[SlotView, int]] = {}
+    total = 0
+    for view in views:
+        if isinstance(view.slot, KVSlot8):
+            key = (id(view.slot), int(view.row0), int(view.tokens))
+            if key not in places:
+                places[key] = (view, total)
+                total += round_up(view.tokens, KV_TILE)
+    if not places:
+        return list(views)
+    first = next(iter(places.values()))[0].slot
+    out = KVSlot(torch, heads=first.heads, head_dim=first.head_dim, capacity=total, device=first.device)
+    table = (_native.KV8Segment * len(places))()
+    dst = (_native.c_int32 * len(places))()
+    for i, (view, at) in enumerate(places.values()):
+        view.slot.fill_segment8(table[i], view.row0, view.tokens)
+        dst[i] = at
+    stride = out.capacity * out.head_dim
+    with _native.device_of(torch, out.k):
+        status = _native.load().tmhd_kv8_expand(
+            table, dst, len(places), _native.ptr(out.k), _native.ptr(out.vt), stride, stride, out.capacity, out.heads,
+            out.head_dim, _native.stream_ptr(torch, out.device),
+        )
+    _native.check(status, "tmhd_kv8_expand")
+    out.tokens = total
+    return [SlotView(out, view.tokens, places[id(view.slot), int(view.row0), int(view.tokens)][1])
+            if isinstance(view.slot, KVSlot8) else view for view in views]
+
+
+def make_slot(torch: Any, storage: str, **shape: Any) -> KVSlot:
+    """A slot of ``storage`` (``"bf16"``, ``"e4m3"`` or ``"int8"``)."""
+    return KVSlot(torch, **shape) if storage == "bf16" else KVSlot8(torch, fmt=storage, **shape)
 
 
 class SlotPool:
@@ -209,9 +343,13 @@ class SlotPool:
     ``release``) is the caller's to order across streams.
     """
 
-    def __init__(self, torch: Any, *, heads: int, head_dim: int, device: Any, max_free: int = 8) -> None:
+    def __init__(self, torch: Any, *, heads: int, head_dim: int, device: Any, max_free: int = 8,
+                 storage: str = "bf16") -> None:
         if int(max_free) < 0:
             raise ValueError("max_free must be non-negative")
+        if storage not in STORAGES:
+            raise ValueError(f"unknown K/V storage {storage!r} (one of {STORAGES})")
+        self.storage = storage
         self._torch = torch
         self.heads = heads
         self.head_dim = head_dim
@@ -236,7 +374,8 @@ class SlotPool:
             self._free.remove(best)
             best.tokens = 0
             return best
-        return KVSlot(self._torch, heads=self.heads, head_dim=self.head_dim, capacity=need, device=self.device)
+        return make_slot(self._torch, self.storage, heads=self.heads, head_dim=self.head_dim, capacity=need,
+                         device=self.device)
 
     def _stream_key(self) -> int:
         """Handle of the current stream on the pool's device (0 off the GPU)."""
@@ -251,8 +390,8 @@ class SlotPool:
         # (the stream of its allocation needs no record)
         if slot.k.is_cuda and _native.stream_ptr(torch, slot.k.device) != slot.allocated_on:
             stream = torch.cuda.current_stream(device=slot.k.device)
-            slot.k.record_stream(stream)
-            slot.vt.record_stream(stream)
+            for buffer in slot.buffers():
+                buffer.record_stream(stream)
         slot.released_on = self._stream_key()
         self._free.append(slot)
         if len(self._free) > self.max_free:

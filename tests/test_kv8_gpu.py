@@ -1,0 +1,381 @@
+"""The K/V slots held in 8 bits: quantizing pack, exact readers, attention over them."""
+
+import numpy as np
+import pytest
+
+from oracle import bf16, lowbit
+
+pytestmark = pytest.mark.gpu
+
+HALF_BF16 = 2.0 ** -8  # half a bf16 step, relative to the value
+FORMATS = ("e4m3", "int8")
+
+
+def _kv(torch, tokens, heads, dim, seed, dev, spread=0):
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randn(tokens, heads, dim, generator=g) + 0.5 * torch.randn(heads, dim, generator=g)
+    v = torch.randn(tokens, heads, dim, generator=g)
+    if spread:
+        f = torch.exp2(torch.randint(-spread, spread + 1, (tokens, heads, dim), generator=g).float())
+        k, v = k * f, v * f.flip(0)
+    return k.to(torch.bfloat16).to(dev), v.to(torch.bfloat16).to(dev)
+
+
+def _f64(t):
+    return bf16.from_torch(t.cpu()).astype(np.float64)
+
+
+def _slot(torch, k, v, fmt, dev, capacity=None, **pack):
+    from taomate_hd_amd import KVSlot8
+
+    slot = KVSlot8(torch, heads=int(k.shape[1]), head_dim=int(k.shape[2]), capacity=capacity or int(k.shape[0]), device=dev,
+                   fmt=fmt)
+    for b in slot.buffers():
+        b.fill_(0xA5)  # stale contents
+    slot.pack(k, v, **pack)
+    return slot
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens,heads,dim", [(1, 1, 64), (63, 3, 128), (64, 2, 64), (65, 5, 128), (331, 14, 128), (1000, 8, 64)])
+def test_pack_is_exact(torch_mod, dev, tokens, heads, dim, fmt):
+    torch = torch_mod
+    k, v = _kv(torch, tokens, heads, dim, tokens + dim, dev, spread=5)
+    slot = _slot(torch, k, v, fmt, dev)
+    got_k, got_v = slot.token_major()
+    for src, got, scale in ((k, got_k, slot.k_scale), (v, got_v, slot.v_scale)):
+        want, byte = lowbit.kv8_values(_f64(src), fmt)
+        np.testing.assert_array_equal(scale.cpu().numpy().T[: len(byte)], byte)
+        np.testing.assert_array_equal(_f64(got), want)
+    assert slot.nbytes == slot.capacity * heads * (2 * dim) + 2 * heads * slot.capacity // 64
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_pack_of_every_bf16_value(torch_mod, dev, fmt):
+    """Every finite bf16 as the largest of its 64-token block, among random smaller ones."""
+    torch, d = torch_mod, 64
+    g = torch.Generator().manual_seed(6)
+    bits = torch.arange(65536, dtype=torch.int32)
+    bits = bits[(bits & 0x7FF0) != 0x7F80][::16]  # a block for every 16th, all of them as other values below
+    bits = bits[(bits & 0x7F80) != 0x7F80]
+    n = int(bits.numel())
+    mag = (bits & 0x7FFF).unsqueeze(1)
+    other = (mag - torch.randint(0, 1600, (n, 64 * d - 1), generator=g)).clamp_min(0)
+    other = other | (torch.randint(0, 2, other.shape, generator=g) << 15)
+    block = torch.cat([bits.unsqueeze(1), other], 1)
+    x = torch.where(block >= 32768, block - 65536, block).to(torch.int16).view(torch.bfloat16)
+    x = x.view(n * 64, 1, d).to(dev)
+    slot = _slot(torch, x, x, fmt, dev)
+    want, byte = lowbit.kv8_values(_f64(x), fmt)
+    for got, scale in zip(slot.token_major(), (slot.k_scale, slot.v_scale)):
+        np.testing.assert_array_equal(scale.cpu().numpy().T, byte)
+        np.testing.assert_array_equal(_f64(got), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_pack_ranges_rows_and_stale_blocks(torch_mod, dev, fmt):
+    """Ranges and a row list of strided K/V land where they are sent; other blocks stay; a block's tail is zero."""
+    from taomate_hd_amd.slots import PackRows
+
+    torch = torch_mod
+    qkv = torch.cat(_kv(torch, 500, 4, 128, 1, dev) + _kv(torch, 500, 4, 128, 2, dev), 2)
+    k, v = qkv[:, :, 128:256], qkv[:, :, 256:384]
+    rows = torch.randperm(500, generator=torch.Generator().manual_seed(3))[:100].to(dev)
+    slot = _slot(torch, k, v, fmt, dev, capacity=640, row0=7, count=70)
+    slot.pack_ranges(k, v, [PackRows(rows=rows, dst=256), PackRows(row0=490, count=10, dst=448)])
+    assert slot.tokens == 458
+    slot.tokens = 640
+    got = slot.token_major()
+    for src, out, codes in zip((k, v), got, (slot.k, slot.vt)):
+        for at, part in ((0, src[7:77]), (256, src[rows]), (448, src[490:])):
+            want, _ = lowbit.kv8_values(_f64(part), fmt)
+            np.testing.assert_array_equal(_f64(out[at : at + len(want)]), want)
+            tail = out[at + len(want) : (at + len(want) + 63) // 64 * 64]
+            assert bool((tail == 0).all())
+        blocks = codes.view(4, 10, 64 * 128)
+        assert bool((blocks[:, [2, 3, 6, 8, 9]] == 0xA5).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_expand_equals_a_bf16_pack_of_the_values(torch_mod, dev, fmt, dim):
+    from taomate_hd_amd.slots import KVSlot, SlotView, expand_views
+
+    torch = torch_mod
+    slots, views = [], []
+    for i, n in enumerate((1, 64, 130, 333)):
+        k, v = _kv(torch, n + 64, 3, dim, i, dev, spread=3)
+        slots.append(_slot(torch, k, v, fmt, dev))
+        views.append(SlotView(slots[-1], n, 64 if n > 1 else 0))
+    views.append(views[2])  # the same rows again
+    out = expand_views(torch, views)
+    assert out[4].row0 == out[2].row0 and out[4].slot is out[2].slot
+    for view, got in zip(views, out):
+        k, v = (t[view.row0 : view.row0 + view.tokens] for t in view.slot.token_major())
+        want = KVSlot(torch, heads=3, head_dim=dim, capacity=view.tokens, device=dev)
+        want.pack(k.contiguous(), v.contiguous())
+        at, cap = got.row0, want.capacity
+        if view.row0 + cap <= view.slot.tokens:  # rows behind the view are the block's own here
+            cap = view.tokens // 64 * 64
+        assert torch.equal(got.slot.k[:, at : at + cap], want.k[:, :cap])
+        assert torch.equal(got.slot.vt[:, :, at : at + cap], want.vt[:, :, :cap])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_blocks_without_finite_values(torch_mod, dev, fmt):
+    """An infinity or NaN makes its block and head NaN, in every reader, and nothing else."""
+    from taomate_hd_amd import segment_attention
+    from taomate_hd_amd.slots import expand_views
+
+    torch = torch_mod
+    k, v = _kv(torch, 200, 4, 64, 1, dev)
+    k[70, 1, 3], v[130, 2, 60] = float("inf"), float("nan")
+    slot = _slot(torch, k, v, fmt, dev)
+    nan = [torch.isnan(t) for t in slot.token_major()]
+    assert int(nan[0].sum()) == 64 * 64 == int(nan[0][64:128, 1].sum())
+    assert int(nan[1].sum()) == 64 * 64 == int(nan[1][128:192, 2].sum())
+    big = expand_views(torch, [slot.view()])[0].slot
+    assert int(torch.isnan(big.k).sum()) == 64 * 64 == int(torch.isnan(big.vt).sum())
+    for rows in (1, 40, 200):
+        q = _kv(torch, rows, 4, 64, 2, dev)[0]
+        bad = torch.isnan(segment_attention(torch, q, [slot.view()], scale=0.125))
+        assert bool(bad[:, 1:3].all()) and not bool(bad[:, [0, 3]].any())
+
+
+def _want(q, segments, scale):
+    """fp64 attention over the slots' own values, and the bound of a bf16-weight kernel's error."""
+    k = np.concatenate([_f64(s.slot.token_major()[0])[s.row0 : s.row0 + s.tokens] for s in segments])
+    v = np.concatenate([_f64(s.slot.token_major()[1])[s.row0 : s.row0 + s.tokens] for s in segments])
+    q = _f64(q)
+    want = lowbit.attention(q, k, v, scale)
+    size = lowbit.attention(q, k, np.abs(v), scale)  # sum of weight * |v|
+    # scores: fp32 sums of D products, each add off by at most 2^-23 of the size; then a few roundings of
+    # a number of the score's size and the hardware exponential (2^-22)
+    reach = max(float((np.abs(q[:, i]) @ np.abs(k[:, i]).T).max()) for i in range(q.shape[1])) * scale
+    weight = HALF_BF16 + 2 * (q.shape[2] + 8) * 2.0 ** -23 * reach + len(k) * 2.0 ** -23 + 2.0 ** -20
+    return want, HALF_BF16 * np.abs(want) + 1.02 * weight * size
+
+
+CASES = [(1, 1, 64, [1]), (1, 3, 128, [33]), (5, 2, 64, [64, 1, 130]), (32, 4, 128, [500]), (33, 2, 128, [65]),
+         (64, 3, 64, [1000, 70]), (1, 14, 128, [9000, 777, 64]), (17, 1, 128, [20000])]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,heads,dim,sizes", CASES)
+def test_attention_of_few_rows(torch_mod, dev, rows, heads, dim, sizes, fmt):
+    from taomate_hd_amd import segment_attention
+
+    torch = torch_mod
+    views = []
+    for i, n in enumerate(sizes):
+        k, v = _kv(torch, n, heads, dim, 10 * i + n, dev)
+        views.append(_slot(torch, k, v * (4.0 ** i), fmt, dev).view())
+    q = _kv(torch, rows, heads, dim, rows, dev)[0]
+    got = segment_attention(torch, q, views, scale=dim ** -0.5)
+    want, bound = _want(q, views, dim ** -0.5)
+    err = np.abs(_f64(got) - want)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_many_rows_equal_attention_over_the_expanded_slot(torch_mod, dev, fmt):
+    """Beyond the rows read in place, and with the INT8-QK backend, a call gives the bits of the same call over a
+    bf16 slot packed with the 8-bit slot's values."""
+    from taomate_hd_amd import segment_attention
+    from taomate_hd_amd.slots import KVSlot
+
+    torch = torch_mod
+    k, v = _kv(torch, 700, 4, 128, 1, dev)
+    slot = _slot(torch, k, v, fmt, dev)
+    plain = KVSlot(torch, heads=4, head_dim=128, capacity=700, device=dev)
+    plain.pack(*slot.token_major())
+    q = _kv(torch, 300, 4, 128, 2, dev)[0]
+    for backend, rows in (("bf16", 300), ("i8qk", 300), ("i8qk", 3)):
+        a = segment_attention(torch, q[:rows], [slot.view()], scale=0.1, backend=backend)
+        b = segment_attention(torch, q[:rows], [plain.view()], scale=0.1, backend=backend)
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_batch_of_unlike_calls(torch_mod, dev, fmt):
+    """Calls of few and many rows, over 8-bit, bf16 and mixed segments, views inside a slot, row lists, strided
+    queries and outputs: each as alone, and rows that belong to no call stay."""
+    from taomate_hd_amd import AttentionCall, KVSlot, segment_attention_batch
+    from taomate_hd_amd.slots import SlotView
+
+    torch, heads, dim = torch_mod, 3, 64
+    other = "int8" if fmt == "e4m3" else "e4m3"
+    a = _slot(torch, *_kv(torch, 400, heads, dim, 1, dev), fmt, dev)
+    b = _slot(torch, *_kv(torch, 90, heads, dim, 2, dev), other, dev)
+    c = KVSlot(torch, heads=heads, head_dim=dim, capacity=100, device=dev)
+    ck, cv = _kv(torch, 100, heads, dim, 3, dev)
+    c.pack(ck, cv)
+    q = _kv(torch, 400, 3 * heads, dim, 4, dev)[0][:, heads : 2 * heads]
+    out = torch.full((400, 2 * heads, dim), 7.0, dtype=torch.bfloat16, device=dev)
+    o = out[:, heads:]
+    rows = torch.tensor([390, 5, 17, 399], device=dev)
+    plan = [
+        (AttentionCall(q, [SlotView(a, 130, 64), SlotView(a, 8, 320)], q_row0=20, lq=9, out=o, o_row0=20), range(20, 29)),
+        (AttentionCall(q, [b.view()], q_rows=rows, out=o, o_rows=rows), rows.tolist()),
+        (AttentionCall(q, [a.view(), c.view()], q_row0=100, lq=2, out=o, o_row0=100), range(100, 102)),
+        (AttentionCall(q, [a.view(), b.view()], q_row0=110, lq=70, out=o, o_row0=110), range(110, 180)),
+        (AttentionCall(q, [a.view()], q_row0=200, lq=0, out=o, o_row0=200), ()),
+        (AttentionCall(q, [c.view()], q_row0=300, lq=5, out=o, o_row0=300), range(300, 305)),
+    ]
+    segment_attention_batch(torch, [call for call, _ in plan], scale=0.125)
+    torch.cuda.synchronize()
+    values = {}
+    for slot in (a, b):
+        values[id(slot)] = slot.token_major()
+    values[id(c)] = (ck, cv)
+
+    class _Held:
+        def __init__(self, slot):
+            self.token_major = lambda: values[id(slot)]
+
+    touched = torch.zeros(400, dtype=torch.bool)
+    for call, where in plan:
+        where = list(where)
+        touched[where] = True
+        if where:
+            want, bound = _want(q[where], [SlotView(_Held(s.slot), s.tokens, s.row0) for s in call.segments], 0.125)
+            assert (np.abs(_f64(o[where]) - want) <= bound).all()
+    assert bool((out[:, :heads] == 7.0).all()) and bool((o[~touched.to(dev)] == 7.0).all())
+
+
+def test_more_calls_than_one_launch(torch_mod, dev):
+    from taomate_hd_amd import AttentionCall, segment_attention, segment_attention_batch
+
+    torch = torch_mod
+    calls = []
+    for i in range(19):
+        views = [_slot(torch, *_kv(torch, 40 + 70 * i + j, 2, 64, i + j, dev), "e4m3", dev).view() for j in range(1 + i % 3)]
+        calls.append(AttentionCall(_kv(torch, 1 + i, 2, 64, 100 + i, dev)[0], views))
+    outs, _ = segment_attention_batch(torch, calls, scale=0.125)
+    for call, out in zip(calls, outs):
+        want, bound = _want(call.query, call.segments, 0.125)
+        assert (np.abs(_f64(out) - want) <= bound).all()
+        again = segment_attention(torch, call.query, call.segments, scale=0.125)
+        assert (np.abs(_f64(again) - want) <= bound).all()
+
+
+def test_large_scores_move_the_running_maximum(torch_mod, dev):
+    from taomate_hd_amd import segment_attention
+
+    torch = torch_mod
+    k, v = _kv(torch, 1500, 2, 128, 1, dev)
+    k = k * torch.linspace(0.1, 6.0, 1500, device=dev).view(-1, 1, 1).to(torch.bfloat16)
+    slot = _slot(torch, k, v, "int8", dev)
+    q = 8 * _kv(torch, 20, 2, 128, 2, dev)[0]
+    got = segment_attention(torch, q, [slot.view()], scale=128 ** -0.5)
+    want, bound = _want(q, [slot.view()], 128 ** -0.5)
+    assert (np.abs(_f64(got) - want) <= bound).all()
+
+
+def test_refusals(torch_mod, dev):
+    from taomate_hd_amd import KVSlot8, fused_qkv_qk_norm_rope_stage_, segment_attention
+
+    torch = torch_mod
+    slot = _slot(torch, *_kv(torch, 100, 2, 64, 1, dev), "e4m3", dev)
+    q = _kv(torch, 3, 2, 64, 2, dev)[0]
+    with pytest.raises(ValueError, match="at least one key"):
+        segment_attention(torch, q, [], scale=1.0)
+    with pytest.raises(ValueError, match="differ from the query"):
+        segment_attention(torch, q[:, :1], [slot.view()], scale=1.0)
+    with pytest.raises(ValueError, match="outside query"):
+        segment_attention(torch, q, [slot.view()], scale=1.0, q_row0=1, lq=3)
+    with pytest.raises(ValueError, match="entries must lie"):
+        segment_attention(torch, q, [slot.view()], scale=1.0, q_rows=torch.tensor([3], device=dev))
+    with pytest.raises(ValueError, match="differ from slot"):
+        slot.pack(*_kv(torch, 10, 3, 64, 1, dev))
+    with pytest.raises(ValueError, match="fit the slot"):
+        slot.pack(*_kv(torch, 10, 2, 64, 1, dev), dst=32)
+    with pytest.raises(ValueError, match="bfloat16|bf16"):
+        slot.pack(*(t.float() for t in _kv(torch, 10, 2, 64, 1, dev)))
+    with pytest.raises(ValueError, match="8-bit K/V format"):
+        KVSlot8(torch, heads=1, head_dim=64, capacity=64, device=dev, fmt="e5m2")
+    with pytest.raises(ValueError, match="bf16 slots"):
+        fused_qkv_qk_norm_rope_stage_(q, None, None, None, None, 1e-6, slot)
+    with pytest.raises(ValueError, match="no bf16 segment"):
+        slot.view().to_segment()
+
+
+def test_streams_and_graph(torch_mod, dev):
+    """A pack and a decode call on another stream, and captured and replayed with new K/V between eager calls."""
+    from taomate_hd_amd import KVSlot8, segment_attention
+
+    torch = torch_mod
+    slot = KVSlot8(torch, heads=4, head_dim=128, capacity=5000, device=dev)
+    k, v = _kv(torch, 5000, 4, 128, 1, dev)
+    q = _kv(torch, 2, 4, 128, 2, dev)[0]
+
+    def step():
+        slot.pack(k, v)
+        return segment_attention(torch, q, [slot.view()], scale=0.1)
+
+    want = step().clone()
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        other = step()
+    stream.synchronize()
+    assert torch.equal(other, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (5, 6, 7):
+        nk, nv = _kv(torch, 5000, 4, 128, seed, dev)
+        k.copy_(nk), v.copy_(nv)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step())
+
+
+@pytest.mark.parametrize("backend", ["sdpa", "sage_attn"])
+@pytest.mark.parametrize("storage", FORMATS)
+def test_hook_over_an_8bit_cache(torch_mod, dev, storage, backend):
+    """Commits and noisy steps through the hook: outputs near those over a bf16 cache, equal to attention over the
+    values the cache gives back, history read back as packed, and half the memory."""
+    from taomate_hd_amd import HeadMajorRingKVCache, HookMode, KVContract, KVSlot, StreamingAttentionHook, segment_attention
+
+    torch, heads, dim, layer = torch_mod, 4, 64, "blocks.0.attn"
+    contract = KVContract(layer_names=(layer,), local_heads=heads, head_dim=dim)
+
+    class Attn:
+        softmax_scale = dim ** -0.5
+
+    def call(hook, n, seed, mode, block):
+        q, k = _kv(torch, n, heads, dim, seed, dev)
+        v = _kv(torch, n, heads, dim, seed + 1, dev)[1]
+        tags = torch.zeros(n, dtype=torch.int64, device=dev)
+        tags[::7] = 2
+        hook.activate(mode=mode, block_index=block)
+        out = hook(attention=Attn(), layer_name=layer, query=q, key=k, value=v, token_tags=tags,
+                   commit_mask=torch.ones(n, dtype=torch.bool, device=dev), cu_seqlens=None, cu_seqlens_host=(0, n),
+                   max_seqlen=n)
+        hook.deactivate()
+        return out, q, k, v
+
+    caches = {s: HeadMajorRingKVCache(contract, storage=s) for s in ("bf16", storage)}
+    last = {}
+    for s, cache in caches.items():
+        hook = StreamingAttentionHook(cache, attention_backend=backend)
+        for block, n in enumerate((210, 130)):
+            cache.begin_clean_commit(block)
+            call(hook, n, 10 * block, HookMode.CLEAN_COMMIT, block)
+            cache.commit()
+        last[s] = call(hook, 300, 50, HookMode.NOISY, 2)
+    cache = caches[storage]
+    assert 0.5 <= cache.slot_bytes / caches["bf16"].slot_bytes < 0.52
+    hist = cache.history(layer)
+    views = []
+    for k, v in ((hist.key, hist.value), last[storage][2:]):
+        views.append(KVSlot(torch, heads=heads, head_dim=dim, capacity=len(k), device=dev))
+        views[-1].pack(k.contiguous(), v.contiguous())
+    want = segment_attention(torch, last[storage][1], [s.view() for s in views], scale=dim ** -0.5)
+    got, plain = _f64(last[storage][0]), _f64(last["bf16"][0])
+    # against attention over the cache's own values: both backends within their rounding of it
+    tol = 2e-2 if backend == "sdpa" else 6e-2
+    assert np.abs(got - _f64(want)).max() <= tol
+    cos = (got * plain).sum() / np.sqrt((got ** 2).sum() * (plain ** 2).sum())
+    assert cos >= 0.99, cos

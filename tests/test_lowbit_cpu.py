@@ -86,3 +86,78 @@ def test_mxfp4_c_entries_refuse():
         assert g(*{**args, **change}.values(), None) == _native.TMHD_ERR_INVALID, change
     assert g(*{**args, "k": 48}.values(), None) == _native.TMHD_ERR_UNSUPPORTED
     assert g(*{**args, "m": 0}.values(), None) == _native.TMHD_OK
+
+
+def _view(**change):
+    from taomate_hd_amd import _native
+
+    base = dict(k=4096, v=4096, ks=4096, vs=4096, cap=128, row0=0, tokens=100, format=0)
+    return _native.KV8Segment(**{**base, **change})
+
+
+def test_kv8_c_entries_refuse():
+    from taomate_hd_amd import _native
+
+    lib, ok, inv, uns = _native.load(), 4096, _native.TMHD_ERR_INVALID, _native.TMHD_ERR_UNSUPPORTED
+    ranges = (_native.PackRange * 2)(_native.PackRange(None, 0, 70, 0, 0), _native.PackRange(None, 0, 10, 64, 0))
+
+    def pack(n=1, slot=None, k=ok, ts=64, hs=64, heads=2, dim=64):
+        return lib.tmhd_kv8_pack_ranges(k, ok, ts, hs, ranges, n, slot or _view(), heads, dim, None)
+
+    assert pack(n=2) == inv and "share a 64-row block" in lib.tmhd_last_error().decode()
+    assert pack(heads=0) == inv and pack(dim=96) == uns and pack(n=-1) == inv
+    assert pack(ts=60) == inv and pack(k=ok + 2) == inv and pack(slot=_view(cap=100)) == inv
+    assert pack(slot=_view(cap=64)) == inv and pack(slot=_view(format=2)) == uns and pack(slot=_view(ks=None)) == inv
+    assert pack(n=0) == _native.TMHD_OK
+
+    def expand(view, dst=0, row=128, head=128 * 64, n=1):
+        return lib.tmhd_kv8_expand(view, (_native.c_int32 * 1)(dst), n, ok, ok, head, head, row, 2, 64, None)
+
+    assert expand(_view(tokens=0)) == inv and expand(_view(row0=32)) == inv and expand(_view(row0=64, tokens=65)) == inv
+    assert expand(_view(), dst=64) == inv and expand(_view(), dst=1) == inv and expand(_view(), head=64 * 64) == inv
+    assert expand(_view(), n=0) == _native.TMHD_OK
+    assert lib.tmhd_kv8_token_major(_view(tokens=129), ok, ok, 2, 64, None) == inv
+    assert lib.tmhd_kv8_token_major(_view(), ok + 8, ok, 2, 64, None) == inv
+
+
+def test_kv8_attention_c_entry_refuses():
+    from taomate_hd_amd import _native
+
+    lib, ok, inv = _native.load(), 4096, _native.TMHD_ERR_INVALID
+
+    def attend(view=None, n_segments=1, heads=2, dim=64, ws=None, ws_bytes=0, second=None, **change):
+        base = dict(q=ok, q_token_stride=128, q_head_stride=64, lq=1, o=ok, o_token_stride=128, o_head_stride=64)
+        c = _native.KV8Call(**{**base, **change}, n_segments=n_segments)
+        for i, s in enumerate([view or _view(), second or _view()]):
+            c.seg[i] = s
+        calls = (_native.KV8Call * 1)(c)
+        return lib.tmhd_attn_fwd_kv8(calls, 1, heads, dim, 1.0, ws, ws_bytes, None)
+
+    assert attend(n_segments=0) == inv and attend(n_segments=17) == inv and attend(lq=-1) == inv
+    assert attend(view=_view(tokens=0)) == inv and attend(q=ok + 8) == inv and attend(q_head_stride=60) == inv
+    assert attend(o_token_stride=126) == inv and attend(o=ok + 2) == inv and attend(q_row0=-1) == inv
+    assert attend(n_segments=2, second=_view(format=1)) == _native.TMHD_ERR_UNSUPPORTED
+    assert attend(dim=256) == _native.TMHD_ERR_UNSUPPORTED and attend(ws=ok + 4, ws_bytes=64) == inv
+    # a long cache is dealt to key ranges: no workspace, no call
+    assert attend(view=_view(cap=1 << 20, tokens=1 << 20), heads=1) == inv and "workspace" in lib.tmhd_last_error().decode()
+    assert attend(lq=0) == _native.TMHD_OK
+
+
+def test_slots_refuse_on_the_host():
+    import torch
+
+    import taomate_hd_amd as tm
+
+    with pytest.raises(ValueError, match="K/V storage"):
+        tm.HeadMajorRingKVCache(storage="fp8")
+    with pytest.raises(ValueError, match="K/V storage"):
+        tm.SlotPool(torch, heads=1, head_dim=64, device="cpu", storage="e5m2")
+    with pytest.raises(ValueError, match="head_dim"):
+        tm.KVSlot8(torch, heads=1, head_dim=96, capacity=64, device="cpu")
+    with pytest.raises(ValueError, match="storage differ"):
+        tm.StreamingSession(type("P", (), {"phases": ()})(), cache=tm.HeadMajorRingKVCache(storage="int8"), kv_storage="e4m3")
+    slot = tm.KVSlot8(torch, heads=1, head_dim=64, capacity=65, device="cpu", fmt="int8")
+    assert slot.capacity == 128 and slot.nbytes == 2 * 128 * 64 + 4
+    k = torch.zeros(10, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        slot.pack(k, k)
