@@ -5,6 +5,7 @@
 
 #include <algorithm>
 
+#include "tmhd_gemm.h"
 #include "tmhd_internal.h"
 #include "tmhd_lowbit.h"
 
@@ -135,12 +136,53 @@ struct XArgs {
   int32_t am4, bn4;  // rows of the scale arrays
   int64_t lda, ldb, ldo;
   int32_t st_ok;     // 8-byte stores of 4 columns
+  int32_t st16_ok;   // 16-byte stores of 8
 };
 
 template <int B>
 __device__ __forceinline__ f32x4 mfma_fp4(const i32x4 &b, const i32x4 &a, const f32x4 &c, int sb, int sa) {
   const i32x8 bb = {b[0], b[1], b[2], b[3]}, aa = {a[0], a[1], a[2], a[3]};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bb, aa, c, 4, 4, B, sb, B, sa);
+}
+
+// The same with the accumulators pinned to AGPRs (IN_AGPR) or VGPRs: left to the
+// builtin, the compiler moves the tiles' accumulators between the two around
+// their MFMAs.  mfma_settle() goes before other code reads them.
+template <int B, bool IN_AGPR>
+__device__ __forceinline__ void mfma_fp4_into(f32x4 &c, const i32x4 &b, const i32x4 &a, int sb, int sa) {
+#define TMHD_MFMA(reg, sel)                                                                                    \
+  asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " sel " cbsz:4 blgp:4" : "+" reg(c) : "v"(b), "v"(a), "v"(sb), "v"(sa))
+#define TMHD_MFMA_BYTE(reg)                                       \
+  if constexpr (B == 0)                                           \
+    TMHD_MFMA(reg, "op_sel:[0,0,0] op_sel_hi:[0,0,0]");           \
+  else if constexpr (B == 1)                                      \
+    TMHD_MFMA(reg, "op_sel:[1,1,0] op_sel_hi:[0,0,0]");           \
+  else if constexpr (B == 2)                                      \
+    TMHD_MFMA(reg, "op_sel:[0,0,0] op_sel_hi:[1,1,0]");           \
+  else                                                            \
+    TMHD_MFMA(reg, "op_sel:[1,1,0] op_sel_hi:[1,1,0]")
+  if constexpr (IN_AGPR) {
+    TMHD_MFMA_BYTE("a");
+  } else {
+    TMHD_MFMA_BYTE("v");
+  }
+#undef TMHD_MFMA_BYTE
+#undef TMHD_MFMA
+}
+
+// The wait states between the last MFMAs and code that reads their results.
+template <bool IN_AGPR, int NB, int MB>
+__device__ __forceinline__ void mfma_settle(f32x4 (&acc)[NB][MB]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      if constexpr (IN_AGPR)
+        asm volatile("" : "+a"(acc[i][j]));
+      else
+        asm volatile("" : "+v"(acc[i][j]));
+    }
 }
 
 // Four columns n .. n + 3 of row m, bias added, rounded once.
@@ -213,6 +255,208 @@ __global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Tiles of 2 MH rows x 2 NH columns, 4 waves as 2 x 2 of MH x NH (blocks of
+// 16 x 16).  k moves in blocks of 128 bytes (256 columns, two MFMA steps), NBUF
+// blocks deep in LDS: rows of 128 bytes (whole cache lines) with chunk c of row
+// r at c ^ ((r >> 1) & 7), which keeps the 16-byte operand reads free of bank
+// conflicts, and each row's scale words for the block's 512 columns, entry g of
+// row r at (r + 16 g) mod rows.  Block d: step 0 multiplies operands that are
+// in registers and reads step 1's; behind the wait for block d + 1 and the
+// barrier nobody reads block d any more, so step 1 loads block d + NBUF in its
+// place and reads block d + 1's first operands and scale words.
+// Columns past k: the loads repeat the row's last chunk, and its scale bytes
+// there are zero, 2^-127 on both sides: the products underflow to 0.
+constexpr int KB = 128;  // bytes of a row in a block
+
+template <int MH, int NH, int NBUF, int WPE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) mxfp4_tile_kernel(const XArgs xa) {
+  constexpr int BM = 2 * MH, BN = 2 * NH, MB = MH / 16, NB = NH / 16, NR = MB + NB, NM = MB * NB;
+  constexpr int DATA = (BM + BN) * KB, SCALE = (BM + BN) * 16, BUF = DATA + SCALE;
+  constexpr int AL = BM / 32, DL = (BM + BN) / 32;  // 1 KiB data loads of a wave: of A, in all
+  constexpr int SN = (BM + BN) / 64;                // 1 KiB scale loads of the workgroup
+  constexpr int SL = SN > 4 ? SN / 4 : 1;           // of a wave (with fewer than 4, waves repeat them)
+  constexpr int LPB = DL + SL;
+  constexpr bool STAGED = MH == 128 && NH == 128, AG = NM > 32;
+  static_assert(NBUF >= 2 && NBUF * BUF <= 160 * 1024 && (NBUF - 1) * LPB < 64, "buffers fit the LDS and vmcnt");
+  __shared__ __attribute__((aligned(1024))) char smem[NBUF * BUF];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
+  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w >> 1, wn = w & 1;
+  const int tmc = (xa.m + BM - 1) / BM, tnc = (xa.n + BN - 1) / BN;
+  int tm, tn;
+  grouped_tile(xcd_logical_id(blockIdx.x, gridDim.x), tmc, tnc, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int chunks = xa.k >> 5, nd = (xa.k + 255) >> 8;
+
+  // data loads: 8 rows of 128 bytes each; lane: row lane / 8, physical chunk lane % 8
+  const int lch = (lane & 7) ^ ((4 * (w & 1) + (lane >> 4)) & 7);
+  uint32_t doff[DL];
+#pragma unroll
+  for (int i = 0; i < DL; ++i) {
+    const int r = (w + 4 * (i < AL ? i : i - AL)) * 8 + (lane >> 3);
+    doff[i] = i < AL ? (uint32_t)((int64_t)min(m0 + r, xa.m - 1) * xa.lda) : (uint32_t)((int64_t)min(n0 + r, xa.n - 1) * xa.ldb);
+  }
+  // scale loads: 64 lanes of 4 words; word q of the area is entry g = q / rows of row (q - 16 g) mod rows
+  uint32_t soff[SL], sdst[SL];
+  bool s_is_a[SL];
+#pragma unroll
+  for (int i = 0; i < SL; ++i) {
+    const int at = SN >= 4 ? w + 4 * i : w % SN;  // of the workgroup's scale loads, A's first
+    const bool is_a = at < BM / 64;
+    const int rows = is_a ? BM : BN, q = (is_a ? at : at - BM / 64) * 256 + lane * 4;
+    const int g = q / rows, r = (q % rows - 16 * g + 4 * rows) % rows;
+    const int r4 = is_a ? xa.am4 : xa.bn4;
+    soff[i] = (uint32_t)(((int64_t)g * r4 + min((is_a ? m0 : n0) + r, r4 - 4)) * 4);
+    sdst[i] = (uint32_t)(DATA + at * 1024);
+    s_is_a[i] = is_a;
+  }
+  // load n of block d (blocks past the last repeat it, into a buffer nobody reads)
+  auto load_one = [&](int d, uint32_t koff, int buf, int n) {
+    const uint32_t at = lds0 + (uint32_t)(buf * BUF);
+    if (n < DL) {
+      const uint32_t dst = at + (n < AL ? (w + 4 * n) * 1024 : BM * KB + (w + 4 * (n - AL)) * 1024);
+      hload_lds16(n < AL ? xa.a : xa.b, doff[n] + koff, dst);
+    } else {
+      const int i = n - DL;
+      const uint32_t *base = s_is_a[i] ? xa.as + (int64_t)(d >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(d >> 1) * 4 * xa.bn4;
+      hload_lds16(base, soff[i], at + sdst[i]);
+    }
+  };
+  auto koff_of = [&](int d) { return (uint32_t)(min(8 * d + lch, chunks - 1) * 16); };
+
+  // operand reads: row i of a 16-row block, logical chunk 4 q + lg
+  uint32_t rdq[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) rdq[q] = (uint32_t)(li * KB + (((4 * q + lg) ^ ((li >> 1) & 7)) * 16));
+  auto read_op = [&](int buf, int q, int r) -> i32x4 {
+    const uint32_t at = (uint32_t)(buf * BUF) + rdq[q];
+    return *(const i32x4 *)(smem + at + (r < MB ? (wm * MH + r * 16) * KB : (BM + wn * NH + (r - MB) * 16) * KB));
+  };
+  uint32_t rds[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int rows = r < MB ? BM : BN, row = (r < MB ? wm * MH + r * 16 : wn * NH + (r - MB) * 16) + li;
+    rds[r] = (uint32_t)(DATA + (r < MB ? 0 : BM * 16) + (lg * rows + (row + 16 * lg) % rows) * 4);
+  }
+  auto read_scale = [&](int buf, int r) -> int { return *(const int *)(smem + (uint32_t)(buf * BUF) + rds[r]); };
+
+  f32x4 acc[NB][MB];  // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+  for (int u = 0; u < NBUF; ++u) {
+    const int d = min(u, nd - 1);
+    const uint32_t ko = koff_of(d);
+#pragma unroll
+    for (int n = 0; n < LPB; ++n) load_one(d, ko, u, n);
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm((NBUF - 1) * LPB));
+  __syncthreads();
+  i32x4 cur[NR], nxt[NR];
+  int sc[NR], nsc[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    cur[r] = read_op(0, 0, r);
+    sc[r] = read_scale(0, r);
+  }
+  // block d in buffer `buf`; ODD: the second of its 512 columns' blocks
+  auto block = [&](auto odd_c, int d, int buf) {
+    constexpr int ODD = decltype(odd_c)::value;
+    const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
+#pragma unroll
+    for (int idx = 0; idx < NM; ++idx) {
+#pragma unroll
+      for (int r = idx * NR / NM; r < (idx + 1) * NR / NM; ++r) nxt[r] = read_op(buf, 1, r);
+      mfma_fp4_into<2 * ODD, AG>(acc[idx / MB][idx % MB], cur[MB + idx / MB], cur[idx % MB], sc[MB + idx / MB], sc[idx % MB]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NBUF - 2) * LPB));
+    __syncthreads();
+    const int dl = min(d + NBUF, nd - 1);
+    const uint32_t ko = koff_of(dl);
+#pragma unroll
+    for (int idx = 0; idx < NM; ++idx) {
+#pragma unroll
+      for (int r = idx * NR / NM; r < (idx + 1) * NR / NM; ++r) {
+        cur[r] = read_op(nbuf, 0, r);
+        nsc[r] = read_scale(nbuf, r);
+      }
+      // loads in the step's first half: they have until the next block's barrier
+#pragma unroll
+      for (int n = 2 * idx * LPB / NM; n < 2 * (idx + 1) * LPB / NM; ++n)
+        if (n < LPB) load_one(dl, ko, buf, n);
+      mfma_fp4_into<2 * ODD + 1, AG>(acc[idx / MB][idx % MB], nxt[MB + idx / MB], nxt[idx % MB], sc[MB + idx / MB], sc[idx % MB]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) sc[r] = nsc[r];
+    // a register that vector code wrote (a copy above) may be an MFMA's operand two wait states later
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 1");
+    __builtin_amdgcn_sched_barrier(0);
+    return nbuf;
+  };
+  int buf = 0, d = 0;
+  for (; d + 1 < nd; d += 2) {
+    buf = block(std::integral_constant<int, 0>{}, d, buf);
+    buf = block(std::integral_constant<int, 1>{}, d + 1, buf);
+  }
+  if (d < nd) block(std::integral_constant<int, 0>{}, d, buf);
+  // every wave drains its loads before the LDS is used again or the workgroup ends
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  mfma_settle<AG>(acc);
+
+  if constexpr (STAGED) {
+    if (xa.st16_ok) {
+      // bf16 tile through LDS: each wave stages its 128 x 128 outputs in rows of
+      // 256 bytes whose 16-byte chunk c sits at c ^ 2((row >> 1) & 7), then writes
+      // 16 bytes per lane, 256-byte row segments
+      constexpr int ROWB = 128 * 2;
+      static_assert(4 * 128 * ROWB <= NBUF * BUF, "staging fits the buffers");
+      auto sw = [](int row) { return 2 * ((row >> 1) & 7); };
+      __syncthreads();
+      const uint32_t wt = (uint32_t)(w * 128 * ROWB);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int n = n0 + wn * 128 + i * 16 + 4 * lg;
+        float bf[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bf[e] = xa.bias ? bf16_bits_to_f32(xa.bias[min(n + e, xa.n - 1)]) : 0.0f;
+        const int ch = 2 * i + (lg >> 1);
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+          const int row = j * 16 + li;
+          *(i32x2 *)(smem + wt + row * ROWB + (ch ^ sw(row)) * 16 + (lg & 1) * 8) =
+              i32x2{(int)pack_bf16_rne(acc[i][j][0] + bf[0], acc[i][j][1] + bf[1]),
+                    (int)pack_bf16_rne(acc[i][j][2] + bf[2], acc[i][j][3] + bf[3])};
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < 32; ++it) {
+        const int r = it * 4 + (lane >> 4), c = lane & 15;
+        const i32x4 v = *(const i32x4 *)(smem + wt + r * ROWB + (c ^ sw(r)) * 16);
+        const int m = m0 + wm * 128 + r, n = n0 + wn * 128 + c * 8;
+        if (m < xa.m && n < xa.n) {
+          uint16_t *op = xa.out + (int64_t)m * xa.ldo + n;
+          if (n + 7 < xa.n)
+            *(i32x4 *)op = v;
+          else
+            for (int e = 0; e < 8 && n + e < xa.n; ++e) op[e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j) store_quad(xa, acc[i][j], m0 + wm * MH + j * 16 + li, n0 + wn * NH + i * 16 + 4 * lg);
+}
+
 int round4(int32_t rows) { return (int)(((int64_t)rows + 3) / 4 * 4); }
 
 int check_matrix(const char *what, int32_t rows, int32_t cols) {
@@ -276,11 +520,20 @@ extern "C" int tmhd_gemm_mxfp4(void *out, const uint8_t *a, const uint8_t *b, co
     return set_error(TMHD_ERR_INVALID, "%s: row strides %lld, %lld, %lld", what, (long long)lda, (long long)ldb, (long long)ldo);
   const XArgs xa{a, b, (const uint32_t *)a_scale, (const uint32_t *)b_scale, (uint16_t *)out, (const uint16_t *)bias,
                  m, n, k, round4(m), round4(n), lda, ldb, ldo,
-                 (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0)};
+                 (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0), (int32_t)((uintptr_t)out % 16 == 0 && ldo % 8 == 0)};
   hipStream_t s = (hipStream_t)stream;
   const unsigned nt = (unsigned)((n + 15) / 16);
   if ((m + 63) / 64 > 65535) return set_error(TMHD_ERR_UNSUPPORTED, "%s: m %d is too large", what, m);
-  if (m <= 16)
+  // the tiles take 32-bit row and scale offsets
+  const bool wide = (int64_t)(m - 1) * lda + k < (int64_t)1 << 32 && (int64_t)(n - 1) * ldb + k < (int64_t)1 << 32;
+  if (wide && m > 64) {
+    const int64_t big = ((int64_t)(m + 255) / 256) * ((n + 255) / 256);
+    if (big >= 128)
+      hipLaunchKernelGGL((mxfp4_tile_kernel<128, 128, 2, 1>), dim3((unsigned)big), dim3(256), 0, s, xa);
+    else
+      hipLaunchKernelGGL((mxfp4_tile_kernel<64, 64, 4, 1>), dim3((unsigned)(((int64_t)(m + 127) / 128) * ((n + 127) / 128))),
+                         dim3(256), 0, s, xa);
+  } else if (m <= 16)
     hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4>), dim3(nt, 1), dim3(256), 0, s, xa);
   else
     hipLaunchKernelGGL((mxfp4_rows_kernel<4, 4>), dim3(nt, (unsigned)((m + 63) / 64)), dim3(256), 0, s, xa);

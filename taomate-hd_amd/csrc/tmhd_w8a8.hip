@@ -8,6 +8,7 @@
 
 #include <algorithm>
 
+#include "tmhd_gemm.h"
 #include "tmhd_internal.h"
 
 namespace tmhd {
@@ -189,18 +190,6 @@ struct GArgs {
   int32_t *ws;
 };
 
-// Tile (tm, tn) of logical tile L: 4 row tiles share each column sweep (L2
-// reuse).  Measured on the 12,252-row projections: 4 beats 2, 6, 8, 16 and 48
-// (about 3% against 8 on 5,120 x 13,824, 1.4% on the 5,376 x 28,672 FC1).
-__device__ __forceinline__ void grouped_tile(int L, int tm_count, int tn_count, int &tm, int &tn) {
-  constexpr int GROUP = 4;
-  const int per_group = GROUP * tn_count;
-  const int first_tm = (L / per_group) * GROUP;
-  const int gsize = min(tm_count - first_tm, GROUP);
-  tm = first_tm + (L % per_group) % gsize;
-  tn = (L % per_group) / gsize;
-}
-
 // The dequantisation epilogue of one accumulator, the same operations in the
 // same order as the GEMM's own epilogue: (float)acc * b_scale * a_scale (+ bias);
 // rounded to bf16 by bf16_quad.
@@ -218,11 +207,6 @@ __device__ __forceinline__ float dequant_f32(int32_t acc, float bs, float as, bo
 __device__ __forceinline__ void bf16_quad(const float (&t)[4], uint16_t (&v)[4]) {
   const uint32_t p01 = pack_bf16_rne(t[0], t[1]), p23 = pack_bf16_rne(t[2], t[3]);
   v[0] = (uint16_t)p01, v[1] = (uint16_t)(p01 >> 16), v[2] = (uint16_t)p23, v[3] = (uint16_t)(p23 >> 16);
-}
-
-__device__ __forceinline__ int xcd_logical_id(int b, int G) {
-  const int xcd = b & 7, pos = b >> 3, per = G >> 3, rem = G & 7;
-  return xcd < rem ? xcd * (per + 1) + pos : rem * (per + 1) + (xcd - rem) * per + pos;
 }
 
 __device__ __forceinline__ void load_lds16(const void *gptr, void *lds) {
@@ -396,13 +380,6 @@ gemm_i8_kernel(const GArgs ga) {
 // nothing.
 constexpr int HBM_ = 256, HBN = 256, HKD = 128, HWAVES = 4, HRING = 5;
 constexpr int HUNIT = 2 * 128 * HKD;  // bytes of one ring unit: 128 rows of A, then of B
-
-// s_waitcnt immediate that leaves n vector-memory operations in flight (and waits for nothing else)
-constexpr int vmcnt_imm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
-
-__device__ __forceinline__ void hload_lds16(const void *base, uint32_t off, uint32_t lds_addr) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
-}
 
 // GLU: the weight rows come in blocks of 256 (128 gate rows, then the 128
 // matching up rows), so tile column c < 128 and c + 128 are the gate and up of

@@ -185,3 +185,26 @@ def test_on_another_stream_and_in_a_graph(torch_mod, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, mxfp4_linear(new, w, ws))
+
+
+# tiles of 256 and of 128, one and more blocks of k, odd numbers of them, k ending inside a block, ragged edges
+TILED = [(257, 128, 32), (256, 256, 256), (256, 256, 512), (65, 128, 768), (129, 131, 800), (300, 4112, 1312),
+         (3000, 3000, 544), (2100, 5000, 1280), (4500, 2000, 64)]
+
+
+@pytest.mark.parametrize("m,n,k", TILED)
+def test_tiled_product(torch_mod, dev, m, n, k):
+    """Whole products of the tiled kernels, against an fp64 product on the GPU."""
+    from taomate_hd_amd import mxfp4_dequant, mxfp4_quant, mxfp4_scaled_mm_out
+
+    torch = torch_mod
+    x, w, b = _rows(torch, m, k, 1, dev, spread=1), _rows(torch, n, k, 2, dev, spread=1), _rows(torch, 1, n, 3, dev)[0]
+    (a, sa), (wq, sw) = mxfp4_quant(x), mxfp4_quant(w)
+    av, wv = mxfp4_dequant(a, sa).double(), mxfp4_dequant(wq, sw).double()
+    want = av @ wv.t() + b.double()
+    slack = (k + 1) * 2.0 ** -23 * (av.abs() @ wv.abs().t() + b.double().abs())
+    out = torch.full((m + 1, n), 7.0, dtype=torch.bfloat16, device=dev)
+    mxfp4_scaled_mm_out(out[:m], a, wq.t(), sa, sw, b)
+    err = (out[:m].double() - want).abs()
+    assert bool((err <= HALF_BF16 * (want.abs() + slack) + slack).all())
+    assert bool((out[m] == 7.0).all())
