@@ -1,6 +1,8 @@
 // K/V slots held in 8 bits (e4m3 or int8 codes, a power-of-two scale for each 64
 // tokens of a head; formats: include/tmhd_lowbit.h): the quantizing pack, the
 // exact expansion to bf16 and attention of few query rows that reads the codes.
+#include <math.h>
+
 #include <type_traits>
 
 #include <algorithm>
@@ -288,7 +290,8 @@ struct Args8 {
   Call8 call[kMaxCalls];
   Seg8 seg[kMaxSegs];
   int32_t n_calls, heads;
-  float scale2;  // softmax scale times log2 e
+  float scale2;  // |softmax scale| times log2 e
+  int32_t flip;  // sign bits to change in Q: a negative scale's
   float *ws;
 };
 
@@ -333,7 +336,12 @@ kv8_attn_kernel(const Args8 aa) {
     const int64_t row = cl.q_rows ? cl.q_rows[r] : cl.q_row0 + r;
     const uint16_t *qp = cl.q + row * cl.qts + (int64_t)h * cl.qhs + 16 * g;
 #pragma unroll
-    for (int t = 0; t < 2 * KC; ++t) qf[c][t] = *(const bf16x8 *)(qp + 32 * (t >> 1) + 8 * (t & 1));
+    for (int t = 0; t < 2 * KC; ++t) {
+      i32x4 v = *(const i32x4 *)(qp + 32 * (t >> 1) + 8 * (t & 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] ^= aa.flip;
+      qf[c][t] = __builtin_bit_cast(bf16x8, v);
+    }
   }
   f32x16 acc[QB][KC];
   float mx[QB], sum[QB];
@@ -347,88 +355,119 @@ kv8_attn_kernel(const Args8 aa) {
       for (int i = 0; i < 16; ++i) acc[c][d][i] = 0.f;
   }
 
-  // the segment of the wave's next block, and that segment's first block
-  int si = cl.seg0, s_first = 0;
-  for (int b = b_begin + w; b < b_end; b += kWaves8) {
+  // The wave's tiles of 32 keys, in order: where the next one's chunks lie, the
+  // softmax factor and the V scale of its block, its valid keys.  The next
+  // tile's K and V chunks are loaded as soon as the current ones are operands.
+  int si = cl.seg0, s_first = 0, b = b_begin + w, t = 0;
+  const uint8_t *kp = nullptr, *vp = nullptr;
+  float kc = 0.f, vc = 0.f;
+  int left = 0;
+  auto locate = [&]() {  // block b of the call, tile 0
     while (b - s_first >= (aa.seg[si].tokens + kBlock - 1) / kBlock) {
       s_first += (aa.seg[si].tokens + kBlock - 1) / kBlock;
       ++si;
     }
     const Seg8 &sg = aa.seg[si];
     const int sb = b - s_first;
-    const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D;
-    const int left = sg.tokens - sb * kBlock;  // valid tokens of the block, 1 or more
-    const int64_t s_at = (int64_t)h * (sg.cap / kBlock) + sb;
-    const float kc = scale_of(sg.ks[s_at]) * aa.scale2, vc = scale_of(sg.vs[s_at]);
+    const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D, s_at = (int64_t)h * (sg.cap / kBlock) + sb;
+    kp = sg.k + off + lane * 16, vp = sg.v + off + lane * 16;
+    left = sg.tokens - sb * kBlock;  // 1 or more
+    kc = scale_of(sg.ks[s_at]) * aa.scale2, vc = scale_of(sg.vs[s_at]);
+    t = 0;
+  };
+  i32x4 kr[KC], vr[KC];
+  if (b < b_end) {
+    locate();
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t == 1 && left <= 32) break;
-      i32x4 kr[KC], vr[KC];
+    for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
 #pragma unroll
-      for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(sg.k + off + t * 32 * D + j * 1024 + lane * 16);
-#pragma unroll
-      for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(sg.v + off + t * 32 * D + j * 1024 + lane * 16);
-      f32x16 s[QB];
-#pragma unroll
-      for (int c = 0; c < QB; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[c][i] = 0.f;
-      auto operand = [](const i32x4 &raw, int half) {
-        const i32x2 lo = decode4<E4M3>((uint32_t)raw[2 * half], 1.0f, false);
-        const i32x2 hi = decode4<E4M3>((uint32_t)raw[2 * half + 1], 1.0f, false);
-        return __builtin_bit_cast(bf16x8, i32x4{lo[0], lo[1], hi[0], hi[1]});
-      };
-#pragma unroll
-      for (int j = 0; j < 2 * KC; ++j) {
-        const bf16x8 kf = operand(kr[j >> 1], j & 1);
-#pragma unroll
-        for (int c = 0; c < QB; ++c) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c][j], s[c], 0, 0, 0);
-      }
-      bf16x8 pf[QB][2];
-#pragma unroll
-      for (int c = 0; c < QB; ++c) {
-        float x[16], top = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] = s[c][i] * kc;
-          if (t * 32 + 8 * (i >> 2) + 4 * g + (i & 3) >= left) x[i] = -__builtin_inff();
-          top = fmaxf(top, x[i]);
-        }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > mx[c])) {
-          // (a first tile of NaN scores leaves the maximum at -inf: sums are 0, NaN follows from the scores)
-          const float m = fmaxf(mx[c], top);
-          const float f = m == mx[c] ? 1.0f : __builtin_amdgcn_exp2f(mx[c] - m);
-          mx[c] = m;
-          sum[c] *= f;
-#pragma unroll
-          for (int d = 0; d < KC; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c][d][i] *= f;
-        }
-        float p[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(x[i] - mx[c]);
-          sum[c] += p[i];
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          i32x4 pk;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pk[e] = (int)pack_bf16_rne(p[8 * m + 2 * e] * vc, p[8 * m + 2 * e + 1] * vc);
-          pf[c][m] = __builtin_bit_cast(bf16x8, pk);
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < KC; ++d)
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const bf16x8 vf = operand(vr[d], m);
-#pragma unroll
-          for (int c = 0; c < QB; ++c) acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[c][m], acc[c][d], 0, 0, 0);
-        }
+    for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
+  }
+  while (b < b_end) {
+    const int here = left;  // valid keys from the tile's first
+    const float kc_now = kc, vc_now = vc;
+    // the next tile: the block's second, or the first of the wave's next block
+    if (t == 0 && left > 32) {
+      t = 1, left -= 32, kp += 32 * D, vp += 32 * D;
+    } else {
+      b += kWaves8;
+      if (b < b_end) locate();
     }
+    f32x16 s[QB];
+#pragma unroll
+    for (int c = 0; c < QB; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[c][i] = 0.f;
+    auto operand = [](const i32x4 &raw, int half, float scale) {
+      const i32x2 lo = decode4<E4M3>((uint32_t)raw[2 * half], scale, false);
+      const i32x2 hi = decode4<E4M3>((uint32_t)raw[2 * half + 1], scale, false);
+      return __builtin_bit_cast(bf16x8, i32x4{lo[0], lo[1], hi[0], hi[1]});
+    };
+#pragma unroll
+    for (int j = 0; j < 2 * KC; ++j) {
+      const bf16x8 kf = operand(kr[j >> 1], j & 1, 1.0f);
+#pragma unroll
+      for (int c = 0; c < QB; ++c) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c][j], s[c], 0, 0, 0);
+    }
+    // (after the last tile: its own chunks again)
+#pragma unroll
+    for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
+    bf16x8 pf[QB][2];
+#pragma unroll
+    for (int c = 0; c < QB; ++c) {
+      if (here < 32) {  // keys past the last: out of the maximum, weight 0 below
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + 4 * g + (i & 3) >= here) s[c][i] = -3.4e38f;
+      }
+      float top = fmaxf(s[c][0], s[c][1]);
+#pragma unroll
+      for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[c][i]), s[c][i + 1]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * kc_now;
+      // the reference moves only where a score passes it by 8 (weights up to 2^8)
+      if (__any(top > mx[c] + 8.0f)) {
+        const float m = fmaxf(mx[c], top);
+        const float f = m == mx[c] ? 1.0f : __builtin_amdgcn_exp2f(mx[c] - m);
+        mx[c] = m;
+        sum[c] *= f;
+#pragma unroll
+        for (int d = 0; d < KC; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[c][d][i] *= f;
+      }
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i], kc_now, -mx[c]));
+      if (here < 32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + 4 * g + (i & 3) >= here) p[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[c] += p[i];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        i32x4 pk;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          pk[e] = E4M3 ? (int)pack_bf16_rne(p[8 * m + 2 * e], p[8 * m + 2 * e + 1])
+                       : (int)pack_bf16_rne(p[8 * m + 2 * e] * vc_now, p[8 * m + 2 * e + 1] * vc_now);
+        pf[c][m] = __builtin_bit_cast(bf16x8, pk);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < KC; ++d)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const bf16x8 vf = operand(vr[d], m, E4M3 ? vc_now : 1.0f);
+#pragma unroll
+        for (int c = 0; c < QB; ++c) acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[c][m], acc[c][d], 0, 0, 0);
+      }
+    if (E4M3 && vc_now != vc_now)  // (the conversion's scale operand has no NaN)
+#pragma unroll
+      for (int c = 0; c < QB; ++c) sum[c] = vc_now;
+#pragma unroll
+    for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
   }
 
   // merge of the four waves, 32 rows at a time, in wave order
@@ -481,35 +520,54 @@ kv8_attn_kernel(const Args8 aa) {
   }
 }
 
-// Merge of a call's key ranges: one workgroup per 32 QB rows of a head, in range order.
+// Merge of a call's key ranges: a workgroup per query row of a head, its 256
+// threads as 1024 / D groups of D / 4 (four channels each); a group takes every
+// (1024 / D)-th range, and the groups' sums are added through LDS in order.  The
+// ranges' maxima and sums are read once, by all threads at a time.
+constexpr int kMaxSplits = 1024;
 template <int D, int QB>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Args8 aa) {
-  constexpr int PF = part_floats<D, QB>(), Q4 = D / 4;
+  constexpr int PF = part_floats<D, QB>(), Q4 = D / 4, G = 256 / Q4;
+  __shared__ f32x4 part[G][Q4];
+  __shared__ float lsum[G], top[kMaxSplits], wmax[4];
   int at = (int)blockIdx.x, ci = 0;
-  for (;; ++ci) {  // the grid counts the items of the split calls
-    const int items = aa.call[ci].splits > 1 ? aa.heads * aa.call[ci].row_tiles : 0;
+  for (;; ++ci) {  // the grid counts the rows of the split calls
+    const int items = aa.call[ci].splits > 1 ? aa.heads * aa.call[ci].lq : 0;
     if (at < items) break;
     at -= items;
   }
   const Call8 &cl = aa.call[ci];
-  const int tile = at % cl.row_tiles, h = at / cl.row_tiles, r0 = tile * 32 * QB;
-  const float *ws = aa.ws + (int64_t)(cl.part0 + at * cl.splits) * PF;
-  for (int i = threadIdx.x; i < min(32 * QB, cl.lq - r0) * Q4; i += 256) {
-    const int r = i / Q4, d = i % Q4 * 4;
-    float m = -__builtin_inff(), l = 0.f;
-    for (int s = 0; s < cl.splits; ++s) m = fmaxf(m, ws[(int64_t)s * PF + QB * 32 * D + r]);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < cl.splits; ++s) {
-      const float *p = ws + (int64_t)s * PF;
-      const float ms = p[QB * 32 * D + r], f = ms == m ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
-      l += f * p[QB * 32 * (D + 1) + r];
-      v += f * *(const f32x4 *)&p[r * D + d];
-    }
-    const int64_t orow = cl.o_rows ? cl.o_rows[r0 + r] : cl.o_row0 + r0 + r;
-    const float inv = 1.0f / l;
-    *(i32x2 *)(cl.o + orow * cl.ots + (int64_t)h * cl.ohs + d) =
-        i32x2{(int)pack_bf16_rne(v[0] * inv, v[1] * inv), (int)pack_bf16_rne(v[2] * inv, v[3] * inv)};
+  const int h = at / cl.lq, row = at - h * cl.lq, tile = row / (32 * QB), r = row % (32 * QB);
+  const float *ws = aa.ws + (int64_t)(cl.part0 + (h * cl.row_tiles + tile) * cl.splits) * PF;
+  const int d4 = threadIdx.x % Q4, grp = threadIdx.x / Q4;
+  float m = -__builtin_inff();
+  for (int s = threadIdx.x; s < cl.splits; s += 256) m = fmaxf(m, top[s] = ws[(int64_t)s * PF + QB * 32 * D + r]);
+  m = wave_max(m);
+  if (threadIdx.x % 64 == 0) wmax[threadIdx.x / 64] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  float l = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = grp; s < cl.splits; s += G) {
+    const float *p = ws + (int64_t)s * PF;
+    const float f = top[s] == m ? 1.0f : __builtin_amdgcn_exp2f(top[s] - m);
+    l += f * p[QB * 32 * (D + 1) + r];
+    v += f * *(const f32x4 *)&p[r * D + 4 * d4];
   }
+  part[grp][d4] = v;
+  if (d4 == 0) lsum[grp] = l;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) {
+    v += part[i][d4];
+    l += lsum[i];
+  }
+  const int64_t orow = cl.o_rows ? cl.o_rows[row] : cl.o_row0 + row;
+  const float inv = 1.0f / l;
+  *(i32x2 *)(cl.o + orow * cl.ots + (int64_t)h * cl.ohs + 4 * d4) =
+      i32x2{(int)pack_bf16_rne(v[0] * inv, v[1] * inv), (int)pack_bf16_rne(v[2] * inv, v[3] * inv)};
 }
 
 // ---- host side
@@ -573,7 +631,8 @@ Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
   for (int i = 0; i < n; ++i)
     total += (int64_t)heads * ((calls[i].lq + 32 * p.qb - 1) / (32 * p.qb)) * blocks_of(calls[i]);
   const int64_t room = (int64_t)std::max(device_cus(), 1) * (p.qb == 1 ? 2 : 1);
-  const int64_t each = std::max<int64_t>(2 * kWaves8, (total + room - 1) / room);
+  int64_t each = std::max<int64_t>(2 * kWaves8, (total + room - 1) / room);
+  for (int i = 0; i < n; ++i) each = std::max<int64_t>(each, (blocks_of(calls[i]) + kMaxSplits - 1) / kMaxSplits);
   for (int i = 0; i < n; ++i) {
     Call8 c{};
     c.lq = calls[i].lq;
@@ -586,7 +645,7 @@ Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
     p.wgs += items * c.splits;
     if (c.splits > 1) {
       p.parts += items * c.splits;
-      p.merge_items += items;
+      p.merge_items += (int64_t)heads * c.lq;
     }
     if (out) out[i] = c;
   }
@@ -761,13 +820,14 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
     const int e = group_end(calls, n, i);
     Args8 aa{};
     const Plan8 p = plan(calls + i, e - i, heads, aa.call);
-    if (p.wgs > INT32_MAX || p.parts > INT32_MAX) return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows", what);
+    if (p.wgs > INT32_MAX || p.parts > INT32_MAX || p.merge_items > INT32_MAX) return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows", what);
     if (parts_bytes(p, head_dim) > (workspace ? workspace_bytes : 0))
       return set_error(TMHD_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,
                        (long long)parts_bytes(p, head_dim));
     aa.n_calls = e - i;
     aa.heads = heads;
-    aa.scale2 = scale * 1.4426950408889634f;
+    aa.scale2 = fabsf(scale) * 1.4426950408889634f;
+    aa.flip = scale < 0.f ? (int32_t)0x80008000u : 0;
     aa.ws = (float *)workspace;
     int segs = 0;
     for (int c = 0; c < aa.n_calls; ++c) {

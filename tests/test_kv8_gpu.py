@@ -151,9 +151,12 @@ def _want(q, segments, scale):
     size = lowbit.attention(q, k, np.abs(v), scale)  # sum of weight * |v|
     # scores: fp32 sums of D products, each add off by at most 2^-23 of the size; then a few roundings of
     # a number of the score's size and the hardware exponential (2^-22)
-    reach = max(float((np.abs(q[:, i]) @ np.abs(k[:, i]).T).max()) for i in range(q.shape[1])) * scale
+    reach = max(float((np.abs(q[:, i]) @ np.abs(k[:, i]).T).max()) for i in range(q.shape[1])) * abs(scale)
     weight = HALF_BF16 + 2 * (q.shape[2] + 8) * 2.0 ** -23 * reach + len(k) * 2.0 ** -23 + 2.0 ** -20
-    return want, HALF_BF16 * np.abs(want) + 1.02 * weight * size
+    # a weight below 2^-126 of the largest is not a normal fp32 number and may count as zero: at most 2^-126 of
+    # each value's size (scores 969.0 and 801.9, the larger's value 0, give an output of 1.6e-74 in fp64, 0 in fp32)
+    lost = 2.0 ** -126 * np.abs(v).sum(0)
+    return want, HALF_BF16 * np.abs(want) + 1.02 * weight * size + lost
 
 
 CASES = [(1, 1, 64, [1]), (1, 3, 128, [33]), (5, 2, 64, [64, 1, 130]), (32, 4, 128, [500]), (33, 2, 128, [65]),
@@ -269,6 +272,19 @@ def test_large_scores_move_the_running_maximum(torch_mod, dev):
     q = 8 * _kv(torch, 20, 2, 128, 2, dev)[0]
     got = segment_attention(torch, q, [slot.view()], scale=128 ** -0.5)
     want, bound = _want(q, [slot.view()], 128 ** -0.5)
+    assert (np.abs(_f64(got) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 40.0])
+def test_any_softmax_scale(torch_mod, dev, scale):
+    """No scale (the mean of the values), a negative, a vanishing and a large one, with a ragged last tile."""
+    from taomate_hd_amd import segment_attention
+
+    torch = torch_mod
+    slot = _slot(torch, *_kv(torch, 71, 2, 64, 1, dev), "int8", dev)
+    q = _kv(torch, 33, 2, 64, 2, dev)[0]
+    got = segment_attention(torch, q, [slot.view()], scale=scale)
+    want, bound = _want(q, [slot.view()], scale)
     assert (np.abs(_f64(got) - want) <= bound).all()
 
 
