@@ -56,6 +56,18 @@ int tmhd_gemm_mxfp4(void *out, const uint8_t *a, const uint8_t *b, const uint8_t
                     const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb, int64_t ldo,
                     void *stream);
 
+/*
+ * tmhd_mxfp4_quant of x [m][k] (bf16, ldx elements between rows) and the product
+ * with b, with the same results: in one launch for few rows, whose blocks the
+ * product quantizes as it reads them, else in two with the rows' codes and
+ * scales in workspace (tmhd_linear_mxfp4_workspace_bytes; 16-byte aligned, may
+ * be NULL if that is 0; calls that share it must be ordered).
+ */
+int tmhd_linear_mxfp4(void *out, const void *x, const uint8_t *b, const uint8_t *b_scale, const void *bias, int32_t m,
+                      int32_t n, int32_t k, int64_t ldx, int64_t ldb, int64_t ldo, void *workspace,
+                      int64_t workspace_bytes, void *stream);
+int64_t tmhd_linear_mxfp4_workspace_bytes(int32_t m, int32_t n, int32_t k);
+
 enum { TMHD_KV8_E4M3 = 0, TMHD_KV8_INT8 = 1 };
 
 /* Rows row0 .. of an 8-bit slot as one attention segment (pointers to the slot's

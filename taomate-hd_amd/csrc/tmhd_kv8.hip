@@ -360,7 +360,8 @@ kv8_attn_kernel(const Args8 aa) {
   // tile's K and V chunks are loaded as soon as the current ones are operands.
   int si = cl.seg0, s_first = 0, b = b_begin + w, t = 0;
   const uint8_t *kp = nullptr, *vp = nullptr;
-  float kc = 0.f, vc = 0.f;
+  // (scale bytes as loaded: turning them into factors here would wait for every load in flight)
+  uint32_t kb = 0, vb = 0;
   int left = 0;
   auto locate = [&]() {  // block b of the call, tile 0
     while (b - s_first >= (aa.seg[si].tokens + kBlock - 1) / kBlock) {
@@ -372,7 +373,7 @@ kv8_attn_kernel(const Args8 aa) {
     const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D, s_at = (int64_t)h * (sg.cap / kBlock) + sb;
     kp = sg.k + off + lane * 16, vp = sg.v + off + lane * 16;
     left = sg.tokens - sb * kBlock;  // 1 or more
-    kc = scale_of(sg.ks[s_at]) * aa.scale2, vc = scale_of(sg.vs[s_at]);
+    kb = sg.ks[s_at], vb = sg.vs[s_at];
     t = 0;
   };
   i32x4 kr[KC], vr[KC];
@@ -385,7 +386,7 @@ kv8_attn_kernel(const Args8 aa) {
   }
   while (b < b_end) {
     const int here = left;  // valid keys from the tile's first
-    const float kc_now = kc, vc_now = vc;
+    const uint32_t kb_now = kb, vb_now = vb;
     // the next tile: the block's second, or the first of the wave's next block
     if (t == 0 && left > 32) {
       t = 1, left -= 32, kp += 32 * D, vp += 32 * D;
@@ -409,6 +410,7 @@ kv8_attn_kernel(const Args8 aa) {
 #pragma unroll
       for (int c = 0; c < QB; ++c) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c][j], s[c], 0, 0, 0);
     }
+    const float kc_now = scale_of(kb_now) * aa.scale2, vc_now = scale_of(vb_now);
     // (after the last tile: its own chunks again)
 #pragma unroll
     for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);

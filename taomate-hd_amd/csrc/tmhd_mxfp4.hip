@@ -199,11 +199,21 @@ __device__ __forceinline__ void store_quad(const XArgs &xa, const f32x4 &v, int 
     for (int e = 0; e < 4 && n + e < xa.n; ++e) op[e] = (uint16_t)((uint32_t)o[e >> 1] >> (16 * (e & 1)));
 }
 
+// 32 bf16 (a lane's block) -> 16 bytes of codes; returns the scale byte
+__device__ __forceinline__ uint32_t quant32(const i32x4 (&x)[4], i32x4 &codes) {
+  const uint32_t byte = scale_byte(max(max(amax8(x[0]), amax8(x[1])), max(amax8(x[2]), amax8(x[3]))));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) codes[i] = (int)codes8(x[i], byte);
+  return byte;
+}
+
 // Few rows: 16 columns of n and 16 MB rows of m a workgroup, its W waves take
 // the 512-column blocks of k in turn, straight from global memory to the MFMA
 // (each code is used once or by MB MFMAs), and add their sums through LDS in
-// wave order.
-template <int MB, int W>
+// wave order.  QUANT: the rows are bf16 (xa.a, lda in elements); a lane's
+// operand is a whole 32-column block, so it finds the block's scale and codes
+// by itself.
+template <int MB, int W, bool QUANT>
 __global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
   __shared__ f32x4 part[W][MB][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
@@ -216,7 +226,7 @@ __global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
     arow[j] = min(m0 + j * 16 + li, xa.m - 1);
-    ap[j] = xa.a + (int64_t)arow[j] * xa.lda + lg * 16;
+    ap[j] = xa.a + (int64_t)arow[j] * xa.lda * (QUANT ? 2 : 1) + lg * (QUANT ? 64 : 16);
   }
   f32x4 acc[MB];
 #pragma unroll
@@ -226,16 +236,34 @@ __global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
     const int64_t at = (int64_t)s * (kSuper / 2);
     i32x4 bv[4], av[MB][4];
     int sa[MB];
+    const int sb = (int)xa.bs[scale_word(s, lg, brow, xa.bn4)];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const bool in = 16 * s + 4 * t + lg < chunks;
       bv[t] = in ? *(const i32x4 *)(bp + at + 64 * t) : i32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < MB; ++j) av[j][t] = in ? *(const i32x4 *)(ap[j] + at + 64 * t) : i32x4{0, 0, 0, 0};
     }
-    const int sb = (int)xa.bs[scale_word(s, lg, brow, xa.bn4)];
+    if constexpr (QUANT) {
 #pragma unroll
-    for (int j = 0; j < MB; ++j) sa[j] = (int)xa.as[scale_word(s, lg, arow[j], xa.am4)];
+      for (int j = 0; j < MB; ++j) {
+        sa[j] = 0;
+        i32x4 x[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[t][e] = 16 * s + 4 * t + lg < chunks ? *(const i32x4 *)(ap[j] + 4 * (at + 64 * t) + 16 * e) : i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sa[j] |= (int)(quant32(x[t], av[j][t]) << (8 * t));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < MB; ++j) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          av[j][t] = 16 * s + 4 * t + lg < chunks ? *(const i32x4 *)(ap[j] + at + 64 * t) : i32x4{0, 0, 0, 0};
+        sa[j] = (int)xa.as[scale_word(s, lg, arow[j], xa.am4)];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < MB; ++j) {
       acc[j] = mfma_fp4<0>(bv[0], av[j][0], acc[j], sb, sa[j]);
@@ -471,6 +499,54 @@ unsigned quant_grid(int32_t rows, int32_t cols) {
   return g <= INT32_MAX ? (unsigned)g : 0u;
 }
 
+// rows that mxfp4_rows_kernel quantizes itself
+constexpr int kFusedRows = 16;
+
+int64_t codes_bytes(int32_t rows, int32_t k) { return ((int64_t)rows * (k / 2) + 255) / 256 * 256; }
+int64_t scale_bytes(int32_t rows, int32_t k) { return ((int64_t)k + kSuper - 1) / kSuper * 16 * round4(rows); }
+
+int check_product(const char *what, const void *out, const uint8_t *b, const uint8_t *b_scale, const void *bias, int32_t m,
+                  int32_t n, int32_t k, int64_t ldb, int64_t ldo) {
+  if (int st = check_matrix(what, m, k)) return st;
+  if (n <= 0 || n > INT32_MAX - 64) return set_error(TMHD_ERR_INVALID, "%s: n %d", what, n);
+  if (m == 0) return TMHD_OK;
+  if (!out || !b || !b_scale || (uintptr_t)b % 16 || (uintptr_t)b_scale % 16 || (uintptr_t)out % 2 || (uintptr_t)bias % 2)
+    return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
+  if (ldb % 16 || ldb < k / 2 || ldo < n)
+    return set_error(TMHD_ERR_INVALID, "%s: row strides %lld, %lld", what, (long long)ldb, (long long)ldo);
+  if ((m + 63) / 64 > 65535) return set_error(TMHD_ERR_UNSUPPORTED, "%s: m %d is too large", what, m);
+  return TMHD_OK;
+}
+
+XArgs product_args(void *out, const uint8_t *a, const uint8_t *a_scale, const uint8_t *b, const uint8_t *b_scale,
+                   const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb, int64_t ldo) {
+  return XArgs{a, b, (const uint32_t *)a_scale, (const uint32_t *)b_scale, (uint16_t *)out, (const uint16_t *)bias,
+               m, n, k, round4(m), round4(n), lda, ldb, ldo,
+               (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0), (int32_t)((uintptr_t)out % 16 == 0 && ldo % 8 == 0)};
+}
+
+// The product of checked arguments.
+int launch_product(const char *what, void *out, const uint8_t *a, const uint8_t *a_scale, const uint8_t *b,
+                   const uint8_t *b_scale, const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb,
+                   int64_t ldo, hipStream_t s) {
+  const XArgs xa = product_args(out, a, a_scale, b, b_scale, bias, m, n, k, lda, ldb, ldo);
+  const unsigned nt = (unsigned)((n + 15) / 16);
+  // the tiles take 32-bit row and scale offsets
+  const bool wide = (int64_t)(m - 1) * lda + k < (int64_t)1 << 32 && (int64_t)(n - 1) * ldb + k < (int64_t)1 << 32;
+  if (wide && m > 64) {
+    const int64_t big = ((int64_t)(m + 255) / 256) * ((n + 255) / 256);
+    if (big >= 128)
+      hipLaunchKernelGGL((mxfp4_tile_kernel<128, 128, 2, 1>), dim3((unsigned)big), dim3(256), 0, s, xa);
+    else
+      hipLaunchKernelGGL((mxfp4_tile_kernel<64, 64, 4, 1>), dim3((unsigned)(((int64_t)(m + 127) / 128) * ((n + 127) / 128))),
+                         dim3(256), 0, s, xa);
+  } else if (m <= 16)
+    hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4, false>), dim3(nt, 1), dim3(256), 0, s, xa);
+  else
+    hipLaunchKernelGGL((mxfp4_rows_kernel<4, 4, false>), dim3(nt, (unsigned)((m + 63) / 64)), dim3(256), 0, s, xa);
+  return check_launch(what);
+}
+
 }  // namespace
 }  // namespace tmhd
 
@@ -510,32 +586,38 @@ extern "C" int tmhd_gemm_mxfp4(void *out, const uint8_t *a, const uint8_t *b, co
                                int64_t ldb, int64_t ldo, void *stream) {
   using namespace tmhd;
   const char *what = "tmhd_gemm_mxfp4";
-  if (int st = check_matrix(what, m, k)) return st;
-  if (n <= 0 || n > INT32_MAX - 64) return set_error(TMHD_ERR_INVALID, "%s: n %d", what, n);
+  if (int st = check_product(what, out, b, b_scale, bias, m, n, k, ldb, ldo)) return st;
   if (m == 0) return TMHD_OK;
-  if (!out || !a || !b || !a_scale || !b_scale || (uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)a_scale % 16 ||
-      (uintptr_t)b_scale % 16 || (uintptr_t)out % 2 || (uintptr_t)bias % 2)
+  if (!a || !a_scale || (uintptr_t)a % 16 || (uintptr_t)a_scale % 16)
     return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
-  if (lda % 16 || ldb % 16 || lda < k / 2 || ldb < k / 2 || ldo < n)
-    return set_error(TMHD_ERR_INVALID, "%s: row strides %lld, %lld, %lld", what, (long long)lda, (long long)ldb, (long long)ldo);
-  const XArgs xa{a, b, (const uint32_t *)a_scale, (const uint32_t *)b_scale, (uint16_t *)out, (const uint16_t *)bias,
-                 m, n, k, round4(m), round4(n), lda, ldb, ldo,
-                 (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0), (int32_t)((uintptr_t)out % 16 == 0 && ldo % 8 == 0)};
+  if (lda % 16 || lda < k / 2) return set_error(TMHD_ERR_INVALID, "%s: row stride %lld", what, (long long)lda);
+  return launch_product(what, out, a, a_scale, b, b_scale, bias, m, n, k, lda, ldb, ldo, (hipStream_t)stream);
+}
+
+extern "C" int64_t tmhd_linear_mxfp4_workspace_bytes(int32_t m, int32_t n, int32_t k) {
+  (void)n;
+  if (m <= tmhd::kFusedRows || k <= 0 || k % 32) return 0;
+  return tmhd::codes_bytes(m, k) + tmhd::scale_bytes(m, k);
+}
+
+extern "C" int tmhd_linear_mxfp4(void *out, const void *x, const uint8_t *b, const uint8_t *b_scale, const void *bias,
+                                 int32_t m, int32_t n, int32_t k, int64_t ldx, int64_t ldb, int64_t ldo,
+                                 void *workspace, int64_t workspace_bytes, void *stream) {
+  using namespace tmhd;
+  const char *what = "tmhd_linear_mxfp4";
+  if (int st = check_product(what, out, b, b_scale, bias, m, n, k, ldb, ldo)) return st;
+  if (m == 0) return TMHD_OK;
+  if (!x || (uintptr_t)x % 16) return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
+  if (ldx % 8 || ldx < k) return set_error(TMHD_ERR_INVALID, "%s: row stride %lld", what, (long long)ldx);
   hipStream_t s = (hipStream_t)stream;
-  const unsigned nt = (unsigned)((n + 15) / 16);
-  if ((m + 63) / 64 > 65535) return set_error(TMHD_ERR_UNSUPPORTED, "%s: m %d is too large", what, m);
-  // the tiles take 32-bit row and scale offsets
-  const bool wide = (int64_t)(m - 1) * lda + k < (int64_t)1 << 32 && (int64_t)(n - 1) * ldb + k < (int64_t)1 << 32;
-  if (wide && m > 64) {
-    const int64_t big = ((int64_t)(m + 255) / 256) * ((n + 255) / 256);
-    if (big >= 128)
-      hipLaunchKernelGGL((mxfp4_tile_kernel<128, 128, 2, 1>), dim3((unsigned)big), dim3(256), 0, s, xa);
-    else
-      hipLaunchKernelGGL((mxfp4_tile_kernel<64, 64, 4, 1>), dim3((unsigned)(((int64_t)(m + 127) / 128) * ((n + 127) / 128))),
-                         dim3(256), 0, s, xa);
-  } else if (m <= 16)
-    hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4>), dim3(nt, 1), dim3(256), 0, s, xa);
-  else
-    hipLaunchKernelGGL((mxfp4_rows_kernel<4, 4>), dim3(nt, (unsigned)((m + 63) / 64)), dim3(256), 0, s, xa);
-  return check_launch(what);
+  if (m <= kFusedRows) {
+    const XArgs xa = product_args(out, (const uint8_t *)x, nullptr, b, b_scale, bias, m, n, k, ldx, ldb, ldo);
+    hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4, true>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, xa);
+    return check_launch(what);
+  }
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < codes_bytes(m, k) + scale_bytes(m, k))
+    return set_error(TMHD_ERR_INVALID, "%s: workspace of %lld bytes", what, (long long)workspace_bytes);
+  uint8_t *q = (uint8_t *)workspace, *scale = q + codes_bytes(m, k);
+  if (int st = tmhd_mxfp4_quant(q, scale, x, m, k, ldx, stream)) return st;
+  return launch_product(what, out, q, scale, b, b_scale, bias, m, n, k, k / 2, ldb, ldo, s);
 }

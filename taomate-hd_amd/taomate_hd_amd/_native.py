@@ -262,6 +262,12 @@ _LOWBIT_SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_int64,
          c_int64, c_void_p],
     ),
+    "tmhd_linear_mxfp4": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64,
+         c_void_p, c_int64, c_void_p],
+    ),
+    "tmhd_linear_mxfp4_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
     "tmhd_kv8_pack_ranges": (
         c_int,
         [c_void_p, c_void_p, c_int64, c_int64, POINTER(PackRange), c_int32, POINTER(KV8Segment), c_int32, c_int32,
@@ -366,7 +372,7 @@ def device_of(torch: Any, tensor: Any) -> Any:
     """A context in which the GPU of ``tensor`` is the current one (a launch goes
     to the current device; the guard costs host time only where it changes)."""
     index = tensor.device.index
-    return _ON_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _ON_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def ptr(tensor: Any) -> int:

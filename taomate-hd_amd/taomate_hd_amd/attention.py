@@ -263,13 +263,15 @@ class AttentionCall:
 
 
 def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: list[Any]) -> tuple[Any, list[SlotView]]:
-    """Check one call and fill its C arguments; returns its output and segments."""
+    """Check one call and fill its C arguments (``AttnArgs``, or ``KV8Call`` for
+    8-bit segments read in place); returns its output and segments."""
     query, out, q_rows, o_rows, lq = call.query, call.out, call.q_rows, call.o_rows, call.lq
     q_row0, o_row0 = int(call.q_row0), int(call.o_row0)
     _validate_tokens_major(torch, query, "query")
     rows_in, heads, head_dim = query.shape
+    device = query.device
     if q_rows is not None:
-        q_rows = _row_list(torch, q_rows, query.device, rows_in, "q_rows", call.rows_checked)
+        q_rows = _row_list(torch, q_rows, device, rows_in, "q_rows", call.rows_checked)
         keep.append(q_rows)
         n = int(q_rows.numel())
         if lq is not None and int(lq) != n:
@@ -279,115 +281,117 @@ def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: l
         lq = rows_in - q_row0
     lq = int(lq)
     if out is None:
-        out = torch.empty((lq, heads, head_dim), dtype=torch.bfloat16, device=query.device)
+        out = torch.empty((lq, heads, head_dim), dtype=torch.bfloat16, device=device)
         o_rows, o_row0 = None, 0
-    _validate_tokens_major(torch, out, "out")
-    if tuple(out.shape[1:]) != (heads, head_dim):
-        raise ValueError("out heads/dim differ from query")
-    if o_rows is not None:
-        o_rows = _row_list(torch, o_rows, out.device, int(out.shape[0]), "o_rows", call.rows_checked)
-        keep.append(o_rows)
-        if int(o_rows.numel()) != lq:
-            raise ValueError("output row list length differs from the query rows")
-    elif not (0 <= o_row0 and o_row0 + lq <= int(out.shape[0])):
-        raise ValueError(f"output rows [{o_row0}, {o_row0 + lq}) outside out ({int(out.shape[0])} rows)")
+    else:
+        _validate_tokens_major(torch, out, "out")
+        if tuple(out.shape[1:]) != (heads, head_dim):
+            raise ValueError("out heads/dim differ from query")
+        if o_rows is not None:
+            o_rows = _row_list(torch, o_rows, out.device, int(out.shape[0]), "o_rows", call.rows_checked)
+            keep.append(o_rows)
+            if int(o_rows.numel()) != lq:
+                raise ValueError("output row list length differs from the query rows")
+        elif not (0 <= o_row0 and o_row0 + lq <= int(out.shape[0])):
+            raise ValueError(f"output rows [{o_row0}, {o_row0 + lq}) outside out ({int(out.shape[0])} rows)")
     if q_rows is None and not (0 <= q_row0 and q_row0 + lq <= rows_in):
         raise ValueError(f"query rows [{q_row0}, {q_row0 + lq}) outside query ({rows_in} rows)")
     segments = [s for s in call.segments if s.tokens > 0]
     if not segments:
         raise ValueError("attention needs at least one key/value token")
     for s in segments:
-        if s.slot.heads != heads or s.slot.head_dim != head_dim or s.slot.device != query.device:
+        slot = s.slot
+        if slot.heads != heads or slot.head_dim != head_dim or slot.device != device:
             raise ValueError("segment heads/dim/device differ from the query")
     if len(segments) > _native.MAX_SEGMENTS:
         segments = _coalesce_segments(torch, segments, _native.MAX_SEGMENTS)
         keep.append(segments)
-    args.q = _native.ptr(query)
-    args.q_token_stride = query.stride(0)
-    args.q_head_stride = query.stride(1)
+    args.q = query.data_ptr()
+    args.q_token_stride, args.q_head_stride, _ = query.stride()
     args.q_rows = _native.ptr(q_rows) if q_rows is not None and lq else None
     args.q_row0 = q_row0
     args.lq = lq
-    args.o = _native.ptr(out)
-    args.o_token_stride = out.stride(0)
-    args.o_head_stride = out.stride(1)
+    args.o = out.data_ptr()
+    args.o_token_stride, args.o_head_stride, _ = out.stride()
     args.o_rows = _native.ptr(o_rows) if o_rows is not None and lq else None
     args.o_row0 = o_row0
     args.n_segments = len(segments)
+    table = args.seg
     if isinstance(args, _native.KV8Call):
         for i, s in enumerate(segments):
-            s.slot.fill_segment8(args.seg[i], s.row0, s.tokens)
+            s.slot.fill_segment8(table, i, s.row0, s.tokens)
         return out, segments
     args.heads = heads
     args.head_dim = head_dim
     args.scale = scale
     for i, s in enumerate(segments):
-        s.fill_segment(args.seg[i])
+        s.fill_segment(table[i])
     return out, segments
 
 
-def _rows_of(call: AttentionCall) -> int:
-    """Query rows of a call (its arguments not checked yet)."""
-    if call.q_rows is not None:
-        return int(call.q_rows.numel()) if hasattr(call.q_rows, "numel") else KV8_ROWS + 1
-    return int(call.query.shape[0]) - int(call.q_row0) if call.lq is None else int(call.lq)
-
-
 def _in_place_format(call: AttentionCall) -> str | None:
-    """The format of the 8-bit segments that a call reads in place, if it does."""
-    segments = [s for s in call.segments if s.tokens > 0]
-    formats = {s.slot.format if isinstance(s.slot, KVSlot8) else None for s in segments}
-    if len(formats) != 1 or len(segments) > _native.MAX_SEGMENTS or _rows_of(call) > KV8_ROWS:
-        return None
-    return formats.pop()
+    """The format of the 8-bit segments that a ``"bf16"`` call reads in place, if it does."""
+    fmt, count = None, 0
+    for s in call.segments:
+        if s.tokens > 0:
+            if not isinstance(s.slot, KVSlot8) or fmt not in (None, s.slot.format):
+                return None
+            fmt, count = s.slot.format, count + 1
+    if call.q_rows is not None:
+        rows = call.q_rows.numel() if hasattr(call.q_rows, "numel") else KV8_ROWS + 1  # (refused later)
+    else:
+        rows = call.query.shape[0] - call.q_row0 if call.lq is None else call.lq
+    return fmt if rows <= KV8_ROWS and count <= _native.MAX_SEGMENTS else None
 
 
 def _attend_in_place(torch: Any, calls: Sequence[AttentionCall], scale: float, timer: ComponentTimer | None) -> list[Any]:
     """Calls of few query rows over 8-bit segments of one format, in one launch (per 16 calls and 24 segments)."""
     keep: list[Any] = []
-    args = (_native.KV8Call * len(calls))()
+    n = len(calls)
+    args = (_native.KV8Call * n)()
     outs = [_call_args(torch, call, args[i], scale, keep)[0] for i, call in enumerate(calls)]
     query = calls[0].query
-    heads, head_dim = int(query.shape[1]), int(query.shape[2])
-    if any(call.query.device != query.device or out.device != query.device or tuple(call.query.shape[1:]) != (heads, head_dim)
-           for call, out in zip(calls, outs)):
-        raise ValueError("the queries and outputs of a batch must share heads, head_dim and one GPU")
+    device, shape = query.device, query.shape[1:]
+    for call, out in zip(calls, outs):
+        if call.query.shape[1:] != shape or call.query.device != device or out.device != device:
+            raise ValueError("the queries and outputs of a batch must share heads, head_dim and one GPU")
+    heads, head_dim = shape
     lib = _native.load()
     with _native.device_of(torch, query), maybe_region(timer, "attention"):
-        need = int(lib.tmhd_attn_kv8_workspace_bytes(args, len(calls), heads, head_dim))
+        need = lib.tmhd_attn_kv8_workspace_bytes(args, n, heads, head_dim)
         # from the caching allocator each time: ordered with its stream, and a captured graph's own
-        ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-        status = lib.tmhd_attn_fwd_kv8(args, len(calls), heads, head_dim, scale, _native.ptr(ws) if need else None, need,
-                                       _native.stream_ptr(torch, query.device))
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        status = lib.tmhd_attn_fwd_kv8(args, n, heads, head_dim, scale, ws.data_ptr() if need else None, need,
+                                       _native.stream_ptr(torch, device))
     _native.check(status, "tmhd_attn_fwd_kv8")
     return outs
 
 
-def _attend_8bit(torch: Any, calls: Sequence[AttentionCall], **options: Any) -> tuple[list[Any], list[dict[str, Any]]]:
+def _attend_8bit(torch: Any, calls: list[AttentionCall], **options: Any) -> tuple[list[Any], list[dict[str, Any]]]:
     """``segment_attention_batch`` of calls some of whose segments are held in 8 bits."""
     scale, timer = float(options["scale"]), options["timer"]
-    for call in calls:
-        _validate_tokens_major(torch, call.query, "query")
-        for s in call.segments:
-            if s.tokens > 0 and (s.slot.heads, s.slot.head_dim, s.slot.device) != (*call.query.shape[1:], call.query.device):
-                raise ValueError("segment heads/dim/device differ from the query")
     formats = [_in_place_format(call) if options["backend"] == "bf16" else None for call in calls]
+    kinds = set(formats)
+    if len(kinds) == 1 and None not in kinds:
+        return _attend_in_place(torch, calls, scale, timer), []
     outs: list[Any] = [None] * len(calls)
-    for fmt in dict.fromkeys(f for f in formats if f is not None):
+    rest = [i for i, f in enumerate(formats) if f is None]
+    segments = [[s for s in calls[i].segments if s.tokens > 0] for i in rest]
+    for i, segs in zip(rest, segments):
+        _validate_tokens_major(torch, calls[i].query, "query")
+        for s in segs:
+            if (s.slot.heads, s.slot.head_dim, s.slot.device) != (*calls[i].query.shape[1:], calls[i].query.device):
+                raise ValueError("segment heads/dim/device differ from the query")
+    for fmt in sorted(kinds - {None}):
         at = [i for i, f in enumerate(formats) if f == fmt]
         for i, out in zip(at, _attend_in_place(torch, [calls[i] for i in at], scale, timer)):
             outs[i] = out
-    rest = [i for i, f in enumerate(formats) if f is None]
-    views: list[dict[str, Any]] = []
-    if rest:
-        segments = [[s for s in calls[i].segments if s.tokens > 0] for i in rest]
-        with maybe_region(timer, "expand"):
-            expanded = iter(expand_views(torch, [s for segs in segments for s in segs]))
-        for i, segs in zip(rest, segments):
-            calls[i] = replace(calls[i], segments=[next(expanded) for _ in segs])
-        got, views = segment_attention_batch(torch, [calls[i] for i in rest], **options)
-        for i, out in zip(rest, got):
-            outs[i] = out
+    with maybe_region(timer, "expand"):
+        expanded = iter(expand_views(torch, [s for segs in segments for s in segs]))
+    calls = [replace(calls[i], segments=[next(expanded) for _ in segs]) for i, segs in zip(rest, segments)]
+    got, views = segment_attention_batch(torch, calls, **options) if calls else ([], [])
+    for i, out in zip(rest, got):
+        outs[i] = out
     return outs, views
 
 

@@ -60,7 +60,7 @@ def mxfp4_scale_to_rows(scale: Any, rows: int, cols: int) -> Any:
 
 def _check_scale(torch: Any, scale: Any, rows: int, cols: int, name: str) -> None:
     shape = scale_shape(rows, cols)
-    if not torch.is_tensor(scale) or scale.dtype != torch.uint8 or tuple(scale.shape) != shape or not scale.is_contiguous():
+    if not torch.is_tensor(scale) or scale.dtype != torch.uint8 or scale.shape != shape or not scale.is_contiguous():
         raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {list(shape)} (mxfp4_scale_from_rows)")
 
 
@@ -69,45 +69,52 @@ def _check_cols(cols: int, name: str) -> None:
         raise ValueError(f"{name} needs a multiple of {MXFP4_BLOCK} columns, got {cols}")
 
 
-def _bf16_rows(torch: Any, x: Any, name: str) -> Any:
-    """``x`` as 2-D bf16 rows that the kernels read in place (copied if they cannot)."""
+def _bf16_rows(torch: Any, x: Any, name: str) -> tuple[Any, int, int, int]:
+    """``x`` as 2-D bf16 rows that the kernels read in place (copied if they cannot), their count, width and stride."""
     _native.require_device_tensor(torch, x, name)
     if x.dtype != torch.bfloat16 or x.ndim < 1:
         raise ValueError(f"{name} must be a bf16 tensor with at least one dimension")
-    _check_cols(int(x.shape[-1]), name)
-    rows = x.reshape(-1, int(x.shape[-1]))
-    if rows.stride(1) != 1 or rows.stride(0) % 8 or rows.stride(0) < rows.shape[1] or rows.data_ptr() % 16:
-        rows = rows.contiguous() if not rows.is_contiguous() else rows.clone()
-    return rows
+    k = x.shape[-1]
+    _check_cols(k, name)
+    rows = x if x.ndim == 2 else x.reshape(-1, k)
+    m = rows.shape[0]
+    stride, step = rows.stride()
+    if m <= 1:
+        stride = k  # a single row's stride says nothing
+    if step != 1 or stride % 8 or stride < k or rows.data_ptr() % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        stride = k
+    return rows, m, k, stride
+
+
+def _launch_quant(torch: Any, q: Any, scale: Any, rows: Any, m: int, k: int, stride: int) -> None:
+    with _native.device_of(torch, rows):
+        status = _native.load().tmhd_mxfp4_quant(
+            q.data_ptr(), scale.data_ptr(), rows.data_ptr(), m, k, stride, _native.stream_ptr(torch, rows.device),
+        )
+    _native.check(status, "tmhd_mxfp4_quant")
 
 
 def mxfp4_quant_into(q: Any, scale: Any, x: Any) -> None:
     """``mxfp4_quant`` writing into caller storage: ``q`` a contiguous uint8
     ``[rows, K / 2]`` tensor, ``scale`` uint8 of ``scale_shape(rows, K)``."""
     torch = _torch()
-    rows = _bf16_rows(torch, x, "x")
-    m, k = int(rows.shape[0]), int(rows.shape[1])
+    rows, m, k, stride = _bf16_rows(torch, x, "x")
     _native.require_same_gpu(torch, rows.device, q=q, scale=scale)
     if q.dtype != torch.uint8 or tuple(q.shape) != (m, k // 2) or not q.is_contiguous():
         raise ValueError("q must be a contiguous uint8 [rows, K / 2] tensor")
     _check_scale(torch, scale, m, k, "scale")
-    with _native.device_of(torch, rows):
-        status = _native.load().tmhd_mxfp4_quant(
-            _native.ptr(q), _native.ptr(scale), _native.ptr(rows), m, k, rows.stride(0) if m > 1 else k,
-            _native.stream_ptr(torch, rows.device),
-        )
-    _native.check(status, "tmhd_mxfp4_quant")
+    _launch_quant(torch, q, scale, rows, m, k, stride)
 
 
 def mxfp4_quant(x: Any) -> tuple[Any, Any]:
     """Rows of bf16 to MXFP4: ``(codes [..., K / 2], scale)`` (activations and weights alike)."""
     torch = _torch()
-    rows = _bf16_rows(torch, x, "x")
-    m, k = int(rows.shape[0]), int(rows.shape[1])
-    q = torch.empty((m, k // 2), dtype=torch.uint8, device=rows.device)
-    scale = torch.empty(scale_shape(m, k), dtype=torch.uint8, device=rows.device)
-    mxfp4_quant_into(q, scale, rows)
-    return q.view(*x.shape[:-1], k // 2), scale
+    rows, m, k, stride = _bf16_rows(torch, x, "x")
+    q = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty(scale_shape(m, k), dtype=torch.uint8, device=x.device)
+    _launch_quant(torch, q, scale, rows, m, k, stride)
+    return q, scale
 
 
 def mxfp4_dequant(q: Any, scale: Any) -> Any:
@@ -121,16 +128,16 @@ def mxfp4_dequant(q: Any, scale: Any) -> Any:
     codes = q.reshape(-1, k // 2).contiguous()
     if codes.data_ptr() % 16:
         codes = codes.clone()
-    m = int(codes.shape[0])
+    m = codes.shape[0]
     _native.require_same_gpu(torch, codes.device, scale=scale)
     _check_scale(torch, scale, m, k, "scale")
-    out = torch.empty((m, k), dtype=torch.bfloat16, device=codes.device)
+    out = torch.empty((*q.shape[:-1], k), dtype=torch.bfloat16, device=codes.device)
     with _native.device_of(torch, codes):
         status = _native.load().tmhd_mxfp4_dequant(
-            _native.ptr(out), _native.ptr(codes), _native.ptr(scale), m, k, _native.stream_ptr(torch, codes.device),
+            out.data_ptr(), codes.data_ptr(), scale.data_ptr(), m, k, _native.stream_ptr(torch, codes.device),
         )
     _native.check(status, "tmhd_mxfp4_dequant")
-    return out.view(*q.shape[:-1], k)
+    return out
 
 
 def _bias_ptr(torch: Any, bias: Any | None, n: int) -> tuple[int | None, Any]:
@@ -142,40 +149,53 @@ def _bias_ptr(torch: Any, bias: Any | None, n: int) -> tuple[int | None, Any]:
     return _native.ptr(bias), bias
 
 
+def _check_codes(torch: Any, a: Any, b: Any, scale_a: Any, scale_b: Any, bias: Any) -> tuple[int, int, int, int, int]:
+    _native.require_device_tensor(torch, a, "a")
+    _native.require_same_gpu(torch, a.device, b=b, scale_a=scale_a, scale_b=scale_b, bias=bias)
+    if a.dtype != torch.uint8 or b.dtype != torch.uint8:
+        raise ValueError("a and b must hold MXFP4 codes in uint8")
+    if a.ndim != 2 or b.ndim != 2 or a.stride(1) != 1:
+        raise ValueError("a must be a row-major [M, K / 2] matrix of codes")
+    m, kb = a.shape
+    kb_b, n = b.shape
+    step, ldb = b.stride()
+    if step != 1:
+        raise ValueError("b must be the [K / 2, N] column-major view (weight.t()) of row-major [N, K / 2] codes")
+    if kb_b != kb:
+        raise ValueError(f"inner dimensions differ: a {tuple(a.shape)}, b {tuple(b.shape)}")
+    _check_cols(2 * kb, "a")
+    _check_scale(torch, scale_a, m, 2 * kb, "scale_a")
+    _check_scale(torch, scale_b, n, 2 * kb, "scale_b")
+    # a single row's stride says nothing
+    return m, n, 2 * kb, a.stride(0) if m > 1 else kb, ldb if n > 1 else kb
+
+
+def _launch_mm(torch: Any, out: Any, ldo: int, a: Any, b: Any, scale_a: Any, scale_b: Any, bias: Any,
+               sizes: tuple[int, int, int, int, int]) -> None:
+    m, n, k, lda, ldb = sizes
+    bias_at, bias = _bias_ptr(torch, bias, n)
+    with _native.device_of(torch, a):
+        status = _native.load().tmhd_gemm_mxfp4(
+            out.data_ptr(), a.data_ptr(), b.data_ptr(), scale_a.data_ptr(), scale_b.data_ptr(), bias_at, m, n, k, lda, ldb,
+            ldo, _native.stream_ptr(torch, a.device),
+        )
+    _native.check(status, "tmhd_gemm_mxfp4")
+
+
 def mxfp4_scaled_mm_out(out: Any, a: Any, b: Any, scale_a: Any, scale_b: Any, bias: Any | None = None) -> None:
     """out = bf16(sum_k a[m, k] b[k, n] (+ bias[n])) of MXFP4 operands, fp32 sums.
 
     ``a``: codes ``[M, K / 2]``; ``b``: the ``[K / 2, N]`` view (``weight.t()``) of a weight's row-major codes
     ``[N, K / 2]``; the scales as ``mxfp4_quant`` gives them (``scale_b`` for the weight's N rows)."""
     torch = _torch()
-    _native.require_device_tensor(torch, a, "a")
-    _native.require_same_gpu(torch, a.device, b=b, out=out, scale_a=scale_a, scale_b=scale_b, bias=bias)
-    if a.dtype != torch.uint8 or b.dtype != torch.uint8:
-        raise ValueError("a and b must hold MXFP4 codes in uint8")
-    if a.ndim != 2 or b.ndim != 2 or a.stride(1) != 1:
-        raise ValueError("a must be a row-major [M, K / 2] matrix of codes")
-    if b.stride(0) != 1 and int(b.shape[0]) != 1:
-        raise ValueError("b must be the [K / 2, N] column-major view (weight.t()) of row-major [N, K / 2] codes")
-    m, kb, n = int(a.shape[0]), int(a.shape[1]), int(b.shape[1])
-    if int(b.shape[0]) != kb:
-        raise ValueError(f"inner dimensions differ: a {tuple(a.shape)}, b {tuple(b.shape)}")
-    k = 2 * kb
-    _check_cols(k, "a")
+    sizes = _check_codes(torch, a, b, scale_a, scale_b, bias)
+    m, n = sizes[:2]
+    _native.require_same_gpu(torch, a.device, out=out)
     if out.dtype != torch.bfloat16:
         raise NotImplementedError("only bf16 output is implemented")
     if tuple(out.shape) != (m, n) or (n > 1 and out.stride(1) != 1):
         raise ValueError("out must be a row-major [M, N] bf16 tensor")
-    _check_scale(torch, scale_a, m, k, "scale_a")
-    _check_scale(torch, scale_b, n, k, "scale_b")
-    bias_at, bias = _bias_ptr(torch, bias, n)
-    # a single row's stride says nothing
-    lda, ldb, ldo = (a.stride(0) if m > 1 else kb), (b.stride(1) if n > 1 else kb), (out.stride(0) if m > 1 else n)
-    with _native.device_of(torch, a):
-        status = _native.load().tmhd_gemm_mxfp4(
-            _native.ptr(out), _native.ptr(a), _native.ptr(b), _native.ptr(scale_a), _native.ptr(scale_b), bias_at,
-            m, n, k, lda, ldb, ldo, _native.stream_ptr(torch, a.device),
-        )
-    _native.check(status, "tmhd_gemm_mxfp4")
+    _launch_mm(torch, out, out.stride(0) if m > 1 else n, a, b, scale_a, scale_b, bias, sizes)
 
 
 def mxfp4_scaled_mm(a: Any, b: Any, scale_a: Any, scale_b: Any, out_dtype: Any = None, bias: Any | None = None) -> Any:
@@ -183,12 +203,34 @@ def mxfp4_scaled_mm(a: Any, b: Any, scale_a: Any, scale_b: Any, out_dtype: Any =
     torch = _torch()
     if out_dtype is not None and out_dtype != torch.bfloat16:
         raise NotImplementedError("only bf16 output is implemented")
-    out = torch.empty((int(a.shape[0]), int(b.shape[1])), dtype=torch.bfloat16, device=a.device)
-    mxfp4_scaled_mm_out(out, a, b, scale_a, scale_b, bias)
+    sizes = _check_codes(torch, a, b, scale_a, scale_b, bias)
+    out = torch.empty(sizes[:2], dtype=torch.bfloat16, device=a.device)
+    _launch_mm(torch, out, sizes[1], a, b, scale_a, scale_b, bias, sizes)
     return out
 
 
 def mxfp4_linear(inputs: Any, weight: Any, weight_scale: Any, bias: Any | None = None) -> Any:
-    """A projection of bf16 rows ``[..., K]`` on an MXFP4 weight (``mxfp4_quant`` of ``[N, K]``): ``[..., N]`` bf16."""
-    q, scale = mxfp4_quant(inputs.reshape(-1, int(inputs.shape[-1])))
-    return mxfp4_scaled_mm(q, weight.t(), scale, weight_scale, bias=bias).view(*inputs.shape[:-1], int(weight.shape[0]))
+    """A projection of bf16 rows ``[..., K]`` on an MXFP4 weight (``mxfp4_quant`` of ``[N, K]``): ``[..., N]`` bf16,
+    the bits of ``mxfp4_scaled_mm`` of the quantised rows (few rows are quantised inside the product)."""
+    torch = _torch()
+    rows, m, k, stride = _bf16_rows(torch, inputs, "inputs")
+    device = rows.device
+    _native.require_same_gpu(torch, device, weight=weight, weight_scale=weight_scale, bias=bias)
+    if weight.dtype != torch.uint8 or weight.ndim != 2 or weight.stride(1) != 1 or weight.shape[1] * 2 != k:
+        raise ValueError(f"weight must hold row-major MXFP4 codes [N, {k // 2}] in uint8")
+    n = weight.shape[0]
+    _check_scale(torch, weight_scale, n, k, "weight_scale")
+    bias_at, bias = _bias_ptr(torch, bias, n)
+    out = torch.empty((*inputs.shape[:-1], n), dtype=torch.bfloat16, device=device)
+    with _native.device_of(torch, rows):
+        lib = _native.load()
+        need = lib.tmhd_linear_mxfp4_workspace_bytes(m, n, k)
+        # from the caching allocator each time: ordered with its stream, and a captured graph's own
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        status = lib.tmhd_linear_mxfp4(
+            out.data_ptr(), rows.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), bias_at, m, n, k, stride,
+            weight.stride(0) if n > 1 else k // 2, n, ws.data_ptr() if need else None, need,
+            _native.stream_ptr(torch, device),
+        )
+    _native.check(status, "tmhd_linear_mxfp4")
+    return out

@@ -242,6 +242,9 @@ class KVSlot8(KVSlot):
         self.vt = torch.empty(shape, dtype=torch.uint8, device=self.device)
         self.k_scale = torch.empty((self.heads, blocks), dtype=torch.uint8, device=self.device)
         self.v_scale = torch.empty((self.heads, blocks), dtype=torch.uint8, device=self.device)
+        self._segment = _native.KV8Segment(
+            *(_native.ptr(t) for t in self.buffers()), self.capacity, 0, 0, KV8_FORMATS.index(self.format),
+        )
 
     @property
     def storage(self) -> str:
@@ -250,15 +253,19 @@ class KVSlot8(KVSlot):
     def buffers(self) -> tuple[Any, ...]:
         return self.k, self.vt, self.k_scale, self.v_scale
 
-    def fill_segment8(self, segment: _native.KV8Segment, row0: int = 0, tokens: int | None = None) -> _native.KV8Segment:
-        row0, tokens = int(row0), self.tokens if tokens is None else int(tokens)
+    def fill_segment8(self, table: Any, at: int, row0: int = 0, tokens: int = 0) -> None:
+        """Entry ``at`` of an array of C segments: rows ``row0 .. row0 + tokens`` of the slot."""
+        row0, tokens = int(row0), int(tokens)
         if row0 < 0 or row0 % KV_TILE or tokens < 0 or row0 + round_up(tokens, KV_TILE) > self.capacity:
             raise ValueError(f"slot view rows [{row0}, {row0 + tokens}) are not a tile-aligned part of the slot")
-        segment.k, segment.v = _native.ptr(self.k), _native.ptr(self.vt)
-        segment.ks, segment.vs = _native.ptr(self.k_scale), _native.ptr(self.v_scale)
-        segment.cap, segment.row0, segment.tokens = self.capacity, row0, tokens
-        segment.format = KV8_FORMATS.index(self.format)
-        return segment
+        table[at] = self._segment  # (copied)
+        segment = table[at]
+        segment.row0, segment.tokens = row0, tokens
+
+    def _segment8(self, tokens: int = 0) -> Any:
+        table = (_native.KV8Segment * 1)()
+        self.fill_segment8(table, 0, 0, tokens)
+        return table
 
     def _launch_pack(self, key: Any, value: Any, table: Any, count: int) -> None:
         torch = self._torch
@@ -266,7 +273,7 @@ class KVSlot8(KVSlot):
         with _native.device_of(torch, key):
             status = _native.load().tmhd_kv8_pack_ranges(
                 _native.ptr(key), _native.ptr(value), key.stride(0), key.stride(1), table, count,
-                self.fill_segment8(_native.KV8Segment()), self.heads, self.head_dim, _native.stream_ptr(torch, key.device),
+                self._segment8(), self.heads, self.head_dim, _native.stream_ptr(torch, key.device),
             )
         _native.check(status, "tmhd_kv8_pack")
 
@@ -279,7 +286,7 @@ class KVSlot8(KVSlot):
         if n:
             with _native.device_of(torch, key):
                 status = _native.load().tmhd_kv8_token_major(
-                    self.fill_segment8(_native.KV8Segment(), 0, n), _native.ptr(key), _native.ptr(value), self.heads,
+                    self._segment8(n), _native.ptr(key), _native.ptr(value), self.heads,
                     self.head_dim, _native.stream_ptr(torch, self.device),
                 )
             _native.check(status, "tmhd_kv8_token_major")
@@ -307,7 +314,7 @@ def expand_views(torch: Any, views: Sequence[SlotView]) -> list[SlotView]:
     table = (_native.KV8Segment * len(places))()
     dst = (_native.c_int32 * len(places))()
     for i, (view, at) in enumerate(places.values()):
-        view.slot.fill_segment8(table[i], view.row0, view.tokens)
+        view.slot.fill_segment8(table, i, view.row0, view.tokens)
         dst[i] = at
     stride = out.capacity * out.head_dim
     with _native.device_of(torch, out.k):

@@ -161,3 +161,17 @@ def test_slots_refuse_on_the_host():
     k = torch.zeros(10, 1, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="GPU tensor"):
         slot.pack(k, k)
+
+
+def test_mxfp4_linear_c_entry_refuses():
+    from taomate_hd_amd import _native
+
+    lib, ok, inv = _native.load(), 4096, _native.TMHD_ERR_INVALID
+    need = lib.tmhd_linear_mxfp4_workspace_bytes(100, 8, 64)
+    assert need == (100 * 32 + 255) // 256 * 256 + 16 * 100 and lib.tmhd_linear_mxfp4_workspace_bytes(1, 8, 64) == 0
+    args = dict(out=ok, x=ok, b=ok, sb=ok, bias=None, m=100, n=8, k=64, ldx=64, ldb=32, ldo=8, ws=ok, bytes=need)
+    for change in (dict(x=ok + 8), dict(ldx=60), dict(ldx=56), dict(ws=None), dict(bytes=need - 1), dict(ws=ok + 8),
+                   dict(n=0), dict(ldb=16)):
+        assert lib.tmhd_linear_mxfp4(*{**args, **change}.values(), None) == inv, change
+    assert lib.tmhd_linear_mxfp4(*{**args, "k": 48}.values(), None) == _native.TMHD_ERR_UNSUPPORTED
+    assert lib.tmhd_linear_mxfp4(*{**args, "m": 0}.values(), None) == _native.TMHD_OK
