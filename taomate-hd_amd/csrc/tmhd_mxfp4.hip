@@ -137,6 +137,7 @@ struct XArgs {
   int64_t lda, ldb, ldo;
   int32_t st_ok;     // 8-byte stores of 4 columns
   int32_t st16_ok;   // 16-byte stores of 8
+  int32_t full;      // tiles of the big kernel
 };
 
 template <int B>
@@ -147,24 +148,30 @@ __device__ __forceinline__ f32x4 mfma_fp4(const i32x4 &b, const i32x4 &a, const 
 
 // The same with the accumulators pinned to AGPRs (IN_AGPR) or VGPRs: left to the
 // builtin, the compiler moves the tiles' accumulators between the two around
-// their MFMAs.  mfma_settle() goes before other code reads them.
-template <int B, bool IN_AGPR>
+// their MFMAs.  FIRST: c = b a.  mfma_settle() goes before other code reads them.
+template <int B, bool IN_AGPR, bool FIRST = false>
 __device__ __forceinline__ void mfma_fp4_into(f32x4 &c, const i32x4 &b, const i32x4 &a, int sb, int sa) {
-#define TMHD_MFMA(reg, sel)                                                                                    \
-  asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " sel " cbsz:4 blgp:4" : "+" reg(c) : "v"(b), "v"(a), "v"(sb), "v"(sa))
+#define TMHD_MFMA(reg, sel)                                                                                      \
+  if constexpr (FIRST)                                                                                           \
+    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 " sel " cbsz:4 blgp:4"                          \
+        : "=&" reg(c) : "v"(b), "v"(a), "v"(sb), "v"(sa));                                                        \
+  else                                                                                                           \
+    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " sel " cbsz:4 blgp:4"                         \
+        : "+" reg(c) : "v"(b), "v"(a), "v"(sb), "v"(sa))
 #define TMHD_MFMA_BYTE(reg)                                       \
-  if constexpr (B == 0)                                           \
+  if constexpr (B == 0) {                                         \
     TMHD_MFMA(reg, "op_sel:[0,0,0] op_sel_hi:[0,0,0]");           \
-  else if constexpr (B == 1)                                      \
+  } else if constexpr (B == 1) {                                  \
     TMHD_MFMA(reg, "op_sel:[1,1,0] op_sel_hi:[0,0,0]");           \
-  else if constexpr (B == 2)                                      \
+  } else if constexpr (B == 2) {                                  \
     TMHD_MFMA(reg, "op_sel:[0,0,0] op_sel_hi:[1,1,0]");           \
-  else                                                            \
-    TMHD_MFMA(reg, "op_sel:[1,1,0] op_sel_hi:[1,1,0]")
+  } else {                                                        \
+    TMHD_MFMA(reg, "op_sel:[1,1,0] op_sel_hi:[1,1,0]");           \
+  }
   if constexpr (IN_AGPR) {
-    TMHD_MFMA_BYTE("a");
+    TMHD_MFMA_BYTE("a")
   } else {
-    TMHD_MFMA_BYTE("v");
+    TMHD_MFMA_BYTE("v")
   }
 #undef TMHD_MFMA_BYTE
 #undef TMHD_MFMA
@@ -297,103 +304,146 @@ __global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
 // there are zero, 2^-127 on both sides: the products underflow to 0.
 constexpr int KB = 128;  // bytes of a row in a block
 
-template <int MH, int NH, int NBUF, int WPE>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) mxfp4_tile_kernel(const XArgs xa) {
-  constexpr int BM = 2 * MH, BN = 2 * NH, MB = MH / 16, NB = NH / 16, NR = MB + NB, NM = MB * NB;
-  constexpr int DATA = (BM + BN) * KB, SCALE = (BM + BN) * 16, BUF = DATA + SCALE;
-  constexpr int AL = BM / 32, DL = (BM + BN) / 32;  // 1 KiB data loads of a wave: of A, in all
-  constexpr int SN = (BM + BN) / 64;                // 1 KiB scale loads of the workgroup
-  constexpr int SL = SN > 4 ? SN / 4 : 1;           // of a wave (with fewer than 4, waves repeat them)
-  constexpr int LPB = DL + SL;
-  constexpr bool STAGED = MH == 128 && NH == 128, AG = NM > 32;
-  static_assert(NBUF >= 2 && NBUF * BUF <= 160 * 1024 && (NBUF - 1) * LPB < 64, "buffers fit the LDS and vmcnt");
-  __shared__ __attribute__((aligned(1024))) char smem[NBUF * BUF];
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w >> 1, wn = w & 1;
-  const int tmc = (xa.m + BM - 1) / BM, tnc = (xa.n + BN - 1) / BN;
-  int tm, tn;
-  grouped_tile(xcd_logical_id(blockIdx.x, gridDim.x), tmc, tnc, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
-  const int chunks = xa.k >> 5, nd = (xa.k + 255) >> 8;
+// hload_lds16 with the wait states that a vector-memory instruction needs after
+// the vector instruction that wrote its scalar base (five: v_readlane of a
+// spilled register, v_readfirstlane) and after the write of m0 (one).  The
+// compiler keeps those for its own instructions, not for inline asm, and the
+// product kernels hold enough scalars for it to spill some to vector lanes.  The
+// copy of the base is a scalar instruction: it waits for the vector write by
+// itself, and a scalar write needs no wait states before the load.
+__device__ __forceinline__ void load_lds16_any(const void *base, uint32_t off, uint32_t lds_addr) {
+  const void *copy;
+  asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(copy) : "v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
+}
 
-  // data loads: 8 rows of 128 bytes each; lane: row lane / 8, physical chunk lane % 8
-  const int lch = (lane & 7) ^ ((4 * (w & 1) + (lane >> 4)) & 7);
-  uint32_t doff[DL];
+// A wave's sums, rounded to bf16 and stored from registers: rows m0 .., columns n0 ...  A
+// pair of 16-column blocks trades halves between neighbouring lane groups, so that a
+// lane holds 8 consecutive columns of one block (16 bytes).
+template <int NB, int MB>
+__device__ __forceinline__ void store_tile(const XArgs &xa, const f32x4 (&acc)[NB][MB], int m0, int n0, int li, int lg) {
 #pragma unroll
-  for (int i = 0; i < DL; ++i) {
-    const int r = (w + 4 * (i < AL ? i : i - AL)) * 8 + (lane >> 3);
-    doff[i] = i < AL ? (uint32_t)((int64_t)min(m0 + r, xa.m - 1) * xa.lda) : (uint32_t)((int64_t)min(n0 + r, xa.n - 1) * xa.ldb);
-  }
-  // scale loads: 64 lanes of 4 words; word q of the area is entry g = q / rows of row (q - 16 g) mod rows
-  uint32_t soff[SL], sdst[SL];
-  bool s_is_a[SL];
+  for (int i = 0; i < NB; i += 2) {
+    const int n = n0 + i * 16 + 4 * lg;  // of the lane's own columns, in block i
+    float bf[2][4];
 #pragma unroll
-  for (int i = 0; i < SL; ++i) {
-    const int at = SN >= 4 ? w + 4 * i : w % SN;  // of the workgroup's scale loads, A's first
-    const bool is_a = at < BM / 64;
-    const int rows = is_a ? BM : BN, q = (is_a ? at : at - BM / 64) * 256 + lane * 4;
-    const int g = q / rows, r = (q % rows - 16 * g + 4 * rows) % rows;
-    const int r4 = is_a ? xa.am4 : xa.bn4;
-    soff[i] = (uint32_t)(((int64_t)g * r4 + min((is_a ? m0 : n0) + r, r4 - 4)) * 4);
-    sdst[i] = (uint32_t)(DATA + at * 1024);
-    s_is_a[i] = is_a;
-  }
-  // load n of block d (blocks past the last repeat it, into a buffer nobody reads)
-  auto load_one = [&](int d, uint32_t koff, int buf, int n) {
-    const uint32_t at = lds0 + (uint32_t)(buf * BUF);
-    if (n < DL) {
-      const uint32_t dst = at + (n < AL ? (w + 4 * n) * 1024 : BM * KB + (w + 4 * (n - AL)) * 1024);
-      hload_lds16(n < AL ? xa.a : xa.b, doff[n] + koff, dst);
-    } else {
-      const int i = n - DL;
-      const uint32_t *base = s_is_a[i] ? xa.as + (int64_t)(d >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(d >> 1) * 4 * xa.bn4;
-      hload_lds16(base, soff[i], at + sdst[i]);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bf[h][e] = xa.bias ? bf16_bits_to_f32(xa.bias[min(n + 16 * h + e, xa.n - 1)]) : 0.0f;
+    const int nn = n0 + (i + (lg & 1)) * 16 + 8 * (lg >> 1);  // of what it stores
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      uint32_t p[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          p[h][e] = pack_bf16_rne(acc[i + h][j][2 * e] + bf[h][2 * e], acc[i + h][j][2 * e + 1] + bf[h][2 * e + 1]);
+      const auto lo = __builtin_amdgcn_permlane16_swap(p[0][0], p[1][0], false, false);
+      const auto hi = __builtin_amdgcn_permlane16_swap(p[0][1], p[1][1], false, false);
+      const i32x4 v = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+      const int m = m0 + j * 16 + li;
+      if (m < xa.m && nn < xa.n) {
+        uint16_t *op = xa.out + (int64_t)m * xa.ldo + nn;
+        if (xa.st16_ok && nn + 7 < xa.n)
+          *(i32x4 *)op = v;
+        else
+          for (int e = 0; e < 8 && nn + e < xa.n; ++e) op[e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+      }
     }
-  };
-  auto koff_of = [&](int d) { return (uint32_t)(min(8 * d + lch, chunks - 1) * 16); };
-
-  // operand reads: row i of a 16-row block, logical chunk 4 q + lg
-  uint32_t rdq[2];
-#pragma unroll
-  for (int q = 0; q < 2; ++q) rdq[q] = (uint32_t)(li * KB + (((4 * q + lg) ^ ((li >> 1) & 7)) * 16));
-  auto read_op = [&](int buf, int q, int r) -> i32x4 {
-    const uint32_t at = (uint32_t)(buf * BUF) + rdq[q];
-    return *(const i32x4 *)(smem + at + (r < MB ? (wm * MH + r * 16) * KB : (BM + wn * NH + (r - MB) * 16) * KB));
-  };
-  uint32_t rds[NR];
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    const int rows = r < MB ? BM : BN, row = (r < MB ? wm * MH + r * 16 : wn * NH + (r - MB) * 16) + li;
-    rds[r] = (uint32_t)(DATA + (r < MB ? 0 : BM * 16) + (lg * rows + (row + 16 * lg) % rows) * 4);
   }
-  auto read_scale = [&](int buf, int r) -> int { return *(const int *)(smem + (uint32_t)(buf * BUF) + rds[r]); };
+}
 
+// The k loop of one tile: DATA / SCALE bytes of a buffer, a wave's loads and the
+// operands of its MFMAs.
+template <int MH, int NH, int NBUF>
+struct TileLoop {
+  static constexpr int BM = 2 * MH, BN = 2 * NH, MB = MH / 16, NB = NH / 16, NR = MB + NB, NM = MB * NB;
+  static constexpr int DATA = (BM + BN) * KB, SCALE = (BM + BN) * 16, BUF = DATA + SCALE;
+  static constexpr int AL = BM / 32, DL = (BM + BN) / 32;  // 1 KiB data loads of a wave: of A, in all
+  static constexpr int SN = (BM + BN) / 64;                // 1 KiB scale loads of the workgroup
+  static constexpr int SL = (SN + 3) / 4;                  // of a wave (where 4 does not divide them, waves repeat some)
+  static constexpr int LPB = DL + SL;
+  static constexpr bool AG = NM > 32;
+  static_assert(NBUF >= 2 && NBUF * BUF <= 160 * 1024 && (NBUF - 1) * LPB < 64, "buffers fit the LDS and vmcnt");
+
+  const XArgs &xa;
+  char *smem;
+  uint32_t lds0;
+  int w, wm, wn, lane, li, lg, lch, chunks, nd;
+  uint32_t doff[DL], soff[SL], sdst[SL], rdq[2], rds[NR];
   f32x4 acc[NB][MB];  // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-#pragma unroll
-  for (int u = 0; u < NBUF; ++u) {
-    const int d = min(u, nd - 1);
-    const uint32_t ko = koff_of(d);
-#pragma unroll
-    for (int n = 0; n < LPB; ++n) load_one(d, ko, u, n);
-  }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm((NBUF - 1) * LPB));
-  __syncthreads();
   i32x4 cur[NR], nxt[NR];
   int sc[NR], nsc[NR];
+
+  __device__ __forceinline__ TileLoop(const XArgs &args, char *lds) : xa(args), smem(lds) {
+    lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
+    chunks = xa.k >> 5, nd = (xa.k + 255) >> 8;
+    lch = (lane & 7) ^ ((4 * (w & 1) + (lane >> 4)) & 7);
+    // operand reads: row i of a 16-row block, logical chunk 4 q + lg
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    cur[r] = read_op(0, 0, r);
-    sc[r] = read_scale(0, r);
+    for (int q = 0; q < 2; ++q) rdq[q] = (uint32_t)(li * KB + (((4 * q + lg) ^ ((li >> 1) & 7)) * 16));
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int rows = r < MB ? BM : BN, row = (r < MB ? wm * MH + r * 16 : wn * NH + (r - MB) * 16) + li;
+      rds[r] = (uint32_t)(DATA + (r < MB ? 0 : BM * 16) + (lg * rows + (row + 16 * lg) % rows) * 4);
+    }
   }
-  // block d in buffer `buf`; ODD: the second of its 512 columns' blocks
-  auto block = [&](auto odd_c, int d, int buf) {
-    constexpr int ODD = decltype(odd_c)::value;
+  // Where the tile's rows and scale words lie.  Data loads: 8 rows of 128 bytes
+  // each; lane: row lane / 8, physical chunk lane % 8.  Scale loads: 64 lanes of 4
+  // words; word q of the area is entry g = q / rows of row (q - 16 g) mod rows.
+  __device__ __forceinline__ void at(int m0, int n0) {
+#pragma unroll
+    for (int i = 0; i < DL; ++i) {
+      const int r = (w + 4 * (i < AL ? i : i - AL)) * 8 + (lane >> 3);
+      doff[i] = i < AL ? (uint32_t)((int64_t)min(m0 + r, xa.m - 1) * xa.lda) : (uint32_t)((int64_t)min(n0 + r, xa.n - 1) * xa.ldb);
+    }
+#pragma unroll
+    for (int i = 0; i < SL; ++i) {
+      const int load = (w + 4 * i) % SN;  // of the workgroup's scale loads, A's first
+      const bool is_a = scale_of_a(i);
+      const int rows = is_a ? BM : BN, q = (is_a ? load : load - BM / 64) * 256 + lane * 4;
+      const int g = q / rows, r = (q % rows - 16 * g + 4 * rows) % rows;
+      const int r4 = is_a ? xa.am4 : xa.bn4;
+      soff[i] = (uint32_t)(((int64_t)g * r4 + min((is_a ? m0 : n0) + r, r4 - 4)) * 4);
+      sdst[i] = (uint32_t)(DATA + load * 1024);
+    }
+  }
+  // whether scale load i of the wave is one of A's (known at compile time for 256 x 256)
+  __device__ __forceinline__ bool scale_of_a(int i) const { return BM == 256 && BN == 256 ? i == 0 : (w + 4 * i) % SN < BM / 64; }
+  // load n of block d (blocks past the last repeat it, into a buffer nobody reads)
+  __device__ __forceinline__ void load_one(int d, uint32_t koff, int buf, int n) {
+    const uint32_t to = lds0 + (uint32_t)(buf * BUF);
+    if (n < DL) {
+      const uint32_t dst = to + (n < AL ? (w + 4 * n) * 1024 : BM * KB + (w + 4 * (n - AL)) * 1024);
+      load_lds16_any(n < AL ? xa.a : xa.b, doff[n] + koff, dst);
+    } else {
+      const int i = n - DL;
+      const uint32_t *base = scale_of_a(i) ? xa.as + (int64_t)(d >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(d >> 1) * 4 * xa.bn4;
+      load_lds16_any(base, soff[i], to + sdst[i]);
+    }
+  }
+  __device__ __forceinline__ uint32_t koff_of(int d) const { return (uint32_t)(min(8 * d + lch, chunks - 1) * 16); }
+  __device__ __forceinline__ i32x4 read_op(int buf, int q, int r) const {
+    const uint32_t from = (uint32_t)(buf * BUF) + rdq[q];
+    return *(const i32x4 *)(smem + from + (r < MB ? (wm * MH + r * 16) * KB : (BM + wn * NH + (r - MB) * 16) * KB));
+  }
+  __device__ __forceinline__ int read_scale(int buf, int r) const { return *(const int *)(smem + (uint32_t)(buf * BUF) + rds[r]); }
+
+  // the loads of the tile's first NBUF blocks
+  __device__ __forceinline__ void first_loads() {
+#pragma unroll
+    for (int u = 0; u < NBUF; ++u) {
+      const int d = min(u, nd - 1);
+      const uint32_t ko = koff_of(d);
+#pragma unroll
+      for (int n = 0; n < LPB; ++n) load_one(d, ko, u, n);
+    }
+  }
+  // block d in buffer `buf`; ODD: the second of its 512 columns' blocks; returns the next buffer
+  template <int ODD>
+  __device__ __forceinline__ int block(int d, int buf) {
     const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
 #pragma unroll
     for (int idx = 0; idx < NM; ++idx) {
@@ -427,62 +477,235 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
     asm volatile("s_nop 1");
     __builtin_amdgcn_sched_barrier(0);
     return nbuf;
-  };
-  int buf = 0, d = 0;
-  for (; d + 1 < nd; d += 2) {
-    buf = block(std::integral_constant<int, 0>{}, d, buf);
-    buf = block(std::integral_constant<int, 1>{}, d + 1, buf);
   }
-  if (d < nd) block(std::integral_constant<int, 0>{}, d, buf);
-  // every wave drains its loads before the LDS is used again or the workgroup ends
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  mfma_settle<AG>(acc);
+  // The sums of the tile whose first block has landed for every wave.  Leaves the
+  // buffers free for every wave and no load in flight.
+  __device__ __forceinline__ void run() {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      cur[r] = read_op(0, 0, r);
+      sc[r] = read_scale(0, r);
+    }
+    int buf = 0, d = 0;
+    for (; d + 1 < nd; d += 2) {
+      buf = block<0>(d, buf);
+      buf = block<1>(d + 1, buf);
+    }
+    if (d < nd) block<0>(d, buf);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    mfma_settle<AG>(acc);
+    __syncthreads();
+  }
+  __device__ __forceinline__ void store(int m0, int n0) {
+    store_tile<NB, MB>(xa, acc, m0 + wm * MH, n0 + wn * NH, li, lg);
+  }
+};
 
-  if constexpr (STAGED) {
-    if (xa.st16_ok) {
-      // bf16 tile through LDS: each wave stages its 128 x 128 outputs in rows of
-      // 256 bytes whose 16-byte chunk c sits at c ^ 2((row >> 1) & 7), then writes
-      // 16 bytes per lane, 256-byte row segments
-      constexpr int ROWB = 128 * 2;
-      static_assert(4 * 128 * ROWB <= NBUF * BUF, "staging fits the buffers");
-      auto sw = [](int row) { return 2 * ((row >> 1) & 7); };
-      __syncthreads();
-      const uint32_t wt = (uint32_t)(w * 128 * ROWB);
+// Tiles of a launch of its own (few workgroups): one tile each.
+template <int MH, int NH, int NBUF, int WPE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) mxfp4_tile_kernel(const XArgs xa) {
+  using T = TileLoop<MH, NH, NBUF>;
+  __shared__ __attribute__((aligned(1024))) char smem[NBUF * T::BUF];
+  T t(xa, smem);
+  int tm, tn;
+  grouped_tile(xcd_logical_id(blockIdx.x, gridDim.x), (xa.m + T::BM - 1) / T::BM, (xa.n + T::BN - 1) / T::BN, tm, tn);
+  t.at(tm * T::BM, tn * T::BN);
+  t.first_loads();
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm((NBUF - 1) * T::LPB));
+  __syncthreads();
+  t.run();
+  t.store(tm * T::BM, tn * T::BN);
+}
+
+// 256 x 256 tiles [0, xa.full), 4 waves as 2 x 2 of 128 x 128 (256 sums a lane, in
+// AGPRs), by a grid that is resident at once: a workgroup takes one tile after the
+// other and its loads never pause, for the next tile's first blocks are loaded
+// under the last MFMAs of a tile and land while it is stored.
+// k moves in blocks of 128 bytes.  A block's operands are four units of 128 rows
+// (A rows 0 .., B rows 0 .., A rows 128 .., B rows 128 ..; rows and swizzle as in
+// TileLoop) in a ring of nine; its scale words, 8 KiB, in one of two buffers: all
+// of the LDS.  Block d: step 0 multiplies operands that are in registers, reads
+// step 1's and loads the first unit of block d + 2 (the ninth slot); behind the
+// wait for block d + 1 and the barrier, step 1 reads block d + 1's first operands
+// and scale words and loads the other three units and the scale words of block
+// d + 2.  With whole blocks in two buffers instead, all loads in half a step, the
+// loads came in bursts that the L1 took 1,150 cycles and more to deliver, and the
+// matrix units were busy 41% of the time.
+template <int UNITS>
+struct BigLoop {
+  static constexpr int UNIT = 128 * KB, RING = UNITS * UNIT, SBUF = 512 * 16;
+  static_assert(RING + 2 * SBUF <= 160 * 1024, "the ring fits the LDS");
+
+  const XArgs &xa;
+  char *smem;
+  uint32_t lds0;
+  int w, wm, wn, lane, li, lg, lch, chunks, nd, tmc, tnc;
+  int L, end, wgs;           // the tile whose blocks are loaded, and the workgroup's others
+  int lb;                    // its next block
+  int tm, tn;                // its place
+  int slot, sbuf;            // ring slot of the current block's first unit, its scale buffer
+  uint32_t doff[4][4], soff[2], rdq[2], rds[16];
+  f32x4 acc[8][8];           // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
+  i32x4 cur[16], nxt[16];    // operands: A blocks 0 .. 7, B blocks 0 .. 7
+  int sc[16], nsc[16];
+
+  __device__ __forceinline__ BigLoop(const XArgs &args, char *lds) : xa(args), smem(lds) {
+    lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
+    chunks = xa.k >> 5, nd = (xa.k + 255) >> 8;
+    lch = (lane & 7) ^ ((4 * (w & 1) + (lane >> 4)) & 7);
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int n = n0 + wn * 128 + i * 16 + 4 * lg;
-        float bf[4];
+    for (int q = 0; q < 2; ++q) rdq[q] = (uint32_t)(li * KB + (((4 * q + lg) ^ ((li >> 1) & 7)) * 16));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bf[e] = xa.bias ? bf16_bits_to_f32(xa.bias[min(n + e, xa.n - 1)]) : 0.0f;
-        const int ch = 2 * i + (lg >> 1);
+    for (int r = 0; r < 16; ++r) {
+      const int row = (r < 8 ? wm * 128 + r * 16 : wn * 128 + (r - 8) * 16) + li;
+      rds[r] = (uint32_t)(RING + (r < 8 ? 0 : 4096) + (lg * 256 + (row + 16 * lg) % 256) * 4);
+    }
+    tmc = (xa.m + 255) / 256, tnc = (xa.n + 255) / 256;
+  }
+  // Where tile L's rows and scale words lie (see TileLoop::at)
+  __device__ __forceinline__ void at() {
+    grouped_tile(L, tmc, tnc, tm, tn);
 #pragma unroll
-        for (int j = 0; j < MB; ++j) {
-          const int row = j * 16 + li;
-          *(i32x2 *)(smem + wt + row * ROWB + (ch ^ sw(row)) * 16 + (lg & 1) * 8) =
-              i32x2{(int)pack_bf16_rne(acc[i][j][0] + bf[0], acc[i][j][1] + bf[1]),
-                    (int)pack_bf16_rne(acc[i][j][2] + bf[2], acc[i][j][3] + bf[3])};
-        }
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (j >> 1) * 128 + (w + 4 * i) * 8 + (lane >> 3);
+        doff[j][i] = j & 1 ? (uint32_t)((int64_t)min(tn * 256 + r, xa.n - 1) * xa.ldb)
+                           : (uint32_t)((int64_t)min(tm * 256 + r, xa.m - 1) * xa.lda);
       }
-#pragma unroll
-      for (int it = 0; it < 32; ++it) {
-        const int r = it * 4 + (lane >> 4), c = lane & 15;
-        const i32x4 v = *(const i32x4 *)(smem + wt + r * ROWB + (c ^ sw(r)) * 16);
-        const int m = m0 + wm * 128 + r, n = n0 + wn * 128 + c * 8;
-        if (m < xa.m && n < xa.n) {
-          uint16_t *op = xa.out + (int64_t)m * xa.ldo + n;
-          if (n + 7 < xa.n)
-            *(i32x4 *)op = v;
-          else
-            for (int e = 0; e < 8 && n + e < xa.n; ++e) op[e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
-        }
-      }
-      return;
+    const int r = (lane * 4 - 16 * w + 256) % 256;  // entry g = w of A's words, then of B's
+    soff[0] = (uint32_t)(((int64_t)w * xa.am4 + min(tm * 256 + r, xa.am4 - 4)) * 4);
+    soff[1] = (uint32_t)(((int64_t)w * xa.bn4 + min(tn * 256 + r, xa.bn4 - 4)) * 4);
+  }
+  // load i of unit j of the block at the load cursor, into ring slot s
+  __device__ __forceinline__ void load_data(int s, int j, int i, uint32_t koff) {
+    load_lds16_any(j & 1 ? xa.b : xa.a, doff[j][i] + koff, lds0 + (uint32_t)(s * UNIT + (w + 4 * i) * 1024));
+  }
+  __device__ __forceinline__ void load_scale(int buf, int i) {
+    const uint32_t *base = i ? xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4 : xa.as + (int64_t)(lb >> 1) * 4 * xa.am4;
+    load_lds16_any(base, soff[i], lds0 + (uint32_t)(RING + buf * SBUF + i * 4096 + w * 1024));
+  }
+  __device__ __forceinline__ uint32_t koff() const { return (uint32_t)(min(8 * lb + lch, chunks - 1) * 16); }
+  // the load cursor's next block: of this tile, of the workgroup's next one, or
+  // (none left) the same again, into slots that nobody reads
+  __device__ __forceinline__ void advance() {
+    if (lb + 1 < nd) {
+      ++lb;
+    } else if (L + wgs < end) {
+      L += wgs;
+      lb = 0;
+      at();
     }
   }
+  static __device__ __forceinline__ int wrap(int s) { return s >= UNITS ? s - UNITS : s; }
+  __device__ __forceinline__ i32x4 read_op(int s, int q, int r) const {  // s: slot of the block's first unit
+    const int unit = r < 8 ? 2 * wm : 2 * wn + 1;
+    return *(const i32x4 *)(smem + (uint32_t)(wrap(s + unit) * UNIT) + rdq[q] + (r & 7) * 16 * KB);
+  }
+  __device__ __forceinline__ int read_scale(int buf, int r) const { return *(const int *)(smem + (uint32_t)(buf * SBUF) + rds[r]); }
+
+  // the first tile's first two blocks on their way, the first in registers
+  __device__ __forceinline__ void begin() {
+    slot = 0, sbuf = 0, lb = 0;
+    at();
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+    for (int d = 0; d < 2; ++d) {
+      const uint32_t ko = koff();
 #pragma unroll
-    for (int j = 0; j < MB; ++j) store_quad(xa, acc[i][j], m0 + wm * MH + j * 16 + li, n0 + wn * NH + i * 16 + 4 * lg);
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_data(4 * d + j, j, i, ko);
+      load_scale(d, 0);
+      load_scale(d, 1);
+      advance();
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(18));
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      cur[r] = read_op(0, 0, r);
+      sc[r] = read_scale(0, r);
+    }
+  }
+  template <int ODD, bool FIRST>
+  __device__ __forceinline__ void block() {
+    const int next = wrap(slot + 4), over = wrap(next + 4);  // over: block d + 2's first unit
+    uint32_t ko = koff();
+#pragma unroll
+    for (int idx = 0; idx < 64; ++idx) {
+      if (idx % 4 == 0) nxt[idx / 4] = read_op(slot, 1, idx / 4);
+      if (idx % 16 == 2) load_data(over, 0, idx / 16, ko);
+      mfma_fp4_into<2 * ODD, true, FIRST>(acc[idx >> 3][idx & 7], cur[8 + (idx >> 3)], cur[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(4));
+    __syncthreads();
+#pragma unroll
+    for (int idx = 0; idx < 64; ++idx) {
+      if (idx % 4 == 0) {
+        cur[idx / 4] = read_op(next, 0, idx / 4);
+        nsc[idx / 4] = read_scale(sbuf ^ 1, idx / 4);
+      }
+      if (idx % 4 == 2 && idx / 4 < 12) load_data(wrap(over + 1 + idx / 16), 1 + idx / 16, idx / 4 % 4, ko);
+      if (idx % 4 == 2 && idx / 4 >= 12 && idx / 4 < 14) load_scale(sbuf, idx / 4 - 12);
+      mfma_fp4_into<2 * ODD + 1, true>(acc[idx >> 3][idx & 7], nxt[8 + (idx >> 3)], nxt[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = nsc[r];
+    slot = next, sbuf ^= 1;
+    // a register that vector code wrote (a copy above) may be an MFMA's operand two wait states later
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 1");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ void store(int m0, int n0) {
+    store_tile<8, 8>(xa, acc, m0 + wm * 128, n0 + wn * 128, li, lg);
+  }
+};
+
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) mxfp4_big_kernel(const XArgs xa) {
+  using T = BigLoop<9>;
+  __shared__ __attribute__((aligned(1024))) char smem[T::RING + 2 * T::SBUF];
+  T t(xa, smem);
+  // XCD x = b % 8 takes a contiguous share of the tiles, its workgroups in turn
+  const int xcd = blockIdx.x & 7, per = xa.full >> 3, rem = xa.full & 7;
+  const int first = xcd * per + min(xcd, rem);
+  t.wgs = ((int)gridDim.x - xcd + 7) >> 3;
+  t.end = first + per + (xcd < rem);
+  t.L = first + (int)(blockIdx.x >> 3);
+  if (t.L >= t.end) return;
+  int L = t.L;  // the tile that is multiplied
+  t.begin();
+  for (;;) {
+    int d = 1;
+    t.template block<0, true>();
+    t.advance();
+    for (; d + 1 < t.nd; d += 2) {
+      t.template block<1, false>();
+      t.advance();
+      t.template block<0, false>();
+      t.advance();
+    }
+    if (d < t.nd) {
+      t.template block<1, false>();
+      t.advance();
+    }
+    mfma_settle<true>(t.acc);
+    int tm, tn;
+    grouped_tile(L, t.tmc, t.tnc, tm, tn);
+    t.store(tm * 256, tn * 256);
+    L += t.wgs;
+    if (L >= t.end) break;
+  }
+  // every wave drains its loads before the workgroup ends
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 }
 
 int round4(int32_t rows) { return (int)(((int64_t)rows + 3) / 4 * 4); }
@@ -522,21 +745,23 @@ XArgs product_args(void *out, const uint8_t *a, const uint8_t *a_scale, const ui
                    const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb, int64_t ldo) {
   return XArgs{a, b, (const uint32_t *)a_scale, (const uint32_t *)b_scale, (uint16_t *)out, (const uint16_t *)bias,
                m, n, k, round4(m), round4(n), lda, ldb, ldo,
-               (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0), (int32_t)((uintptr_t)out % 16 == 0 && ldo % 8 == 0)};
+               (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0), (int32_t)((uintptr_t)out % 16 == 0 && ldo % 8 == 0), 0};
 }
 
 // The product of checked arguments.
 int launch_product(const char *what, void *out, const uint8_t *a, const uint8_t *a_scale, const uint8_t *b,
                    const uint8_t *b_scale, const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb,
                    int64_t ldo, hipStream_t s) {
-  const XArgs xa = product_args(out, a, a_scale, b, b_scale, bias, m, n, k, lda, ldb, ldo);
+  XArgs xa = product_args(out, a, a_scale, b, b_scale, bias, m, n, k, lda, ldb, ldo);
   const unsigned nt = (unsigned)((n + 15) / 16);
   // the tiles take 32-bit row and scale offsets
   const bool wide = (int64_t)(m - 1) * lda + k < (int64_t)1 << 32 && (int64_t)(n - 1) * ldb + k < (int64_t)1 << 32;
   if (wide && m > 64) {
     const int64_t big = ((int64_t)(m + 255) / 256) * ((n + 255) / 256);
-    if (big >= 128)
-      hipLaunchKernelGGL((mxfp4_tile_kernel<128, 128, 2, 1>), dim3((unsigned)big), dim3(256), 0, s, xa);
+    if (big >= 128) {
+      xa.full = (int32_t)big;
+      hipLaunchKernelGGL(mxfp4_big_kernel, dim3((unsigned)std::min<int64_t>(big, std::max(device_cus(), 8))), dim3(256), 0, s, xa);
+    }
     else
       hipLaunchKernelGGL((mxfp4_tile_kernel<64, 64, 4, 1>), dim3((unsigned)(((int64_t)(m + 127) / 128) * ((n + 127) / 128))),
                          dim3(256), 0, s, xa);

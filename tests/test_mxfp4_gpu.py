@@ -189,7 +189,8 @@ def test_on_another_stream_and_in_a_graph(torch_mod, dev):
 
 # tiles of 256 and of 128, one and more blocks of k, odd numbers of them, k ending inside a block, ragged edges
 TILED = [(257, 128, 32), (256, 256, 256), (256, 256, 512), (65, 128, 768), (129, 131, 800), (300, 4112, 1312),
-         (3000, 3000, 544), (2100, 5000, 1280), (4500, 2000, 64)]
+         (3000, 3000, 544), (2100, 5000, 1280), (4500, 2000, 64),
+         (4900, 5003, 1056), (2049, 8200, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", TILED)
