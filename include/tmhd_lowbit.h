@@ -57,6 +57,23 @@ int tmhd_gemm_mxfp4(void *out, const uint8_t *a, const uint8_t *b, const uint8_t
                     void *stream);
 
 /*
+ * The form that an m x n x k product takes on a device of `cus` CUs (0: the
+ * current one; 32-bit offsets): 16 x 16 tiles straight from memory, or tiles of the
+ * stated rows x columns (X2: two workgroups a CU), which may stand behind whole
+ * rounds of 256 x 256 tiles.  -1 for sizes that no product has.  Launches
+ * nothing, and needs no GPU if cus > 0.
+ */
+enum {
+  TMHD_MXFP4_ROWS,
+  TMHD_MXFP4_64X64,
+  TMHD_MXFP4_128X64,
+  TMHD_MXFP4_128X128,
+  TMHD_MXFP4_128X128X2,
+  TMHD_MXFP4_256X256
+};
+int tmhd_gemm_mxfp4_form(int32_t m, int32_t n, int32_t k, int32_t cus);
+
+/*
  * tmhd_mxfp4_quant of x [m][k] (bf16, ldx elements between rows) and the product
  * with b, with the same results: in one launch for few rows, whose blocks the
  * product quantizes as it reads them, else in two with the rows' codes and

@@ -214,80 +214,62 @@ __device__ __forceinline__ uint32_t quant32(const i32x4 (&x)[4], i32x4 &codes) {
   return byte;
 }
 
-// Few rows: 16 columns of n and 16 MB rows of m a workgroup, its W waves take
-// the 512-column blocks of k in turn, straight from global memory to the MFMA
-// (each code is used once or by MB MFMAs), and add their sums through LDS in
-// wave order.  QUANT: the rows are bf16 (xa.a, lda in elements); a lane's
+// Few rows: 16 columns of n and 16 rows of m a workgroup, its four waves take the
+// 512-column blocks of k in turn, straight from global memory to the MFMA (each
+// code is used once), and add their sums through LDS in wave order.  (Also the
+// form of matrices beyond 32-bit offsets.)  QUANT: the rows are bf16 (xa.a, lda in elements); a lane's
 // operand is a whole 32-column block, so it finds the block's scale and codes
 // by itself.
-template <int MB, int W, bool QUANT>
-__global__ void __launch_bounds__(64 * W) mxfp4_rows_kernel(const XArgs xa) {
-  __shared__ f32x4 part[W][MB][64];
+template <bool QUANT>
+__global__ void __launch_bounds__(256) mxfp4_rows_kernel(const XArgs xa) {
+  constexpr int W = 4;
+  __shared__ f32x4 part[W][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
+  const int tiles_n = (xa.n + 15) / 16;
+  const int n0 = (int)(blockIdx.x % tiles_n) * 16, m0 = (int)(blockIdx.x / tiles_n) * 16;
   const int chunks = xa.k >> 5, blocks = (xa.k + kSuper - 1) / kSuper;
-  const int brow = min(n0 + li, xa.n - 1);
+  const int brow = min(n0 + li, xa.n - 1), arow = min(m0 + li, xa.m - 1);
   const uint8_t *bp = xa.b + (int64_t)brow * xa.ldb + lg * 16;
-  const uint8_t *ap[MB];
-  int arow[MB];
-#pragma unroll
-  for (int j = 0; j < MB; ++j) {
-    arow[j] = min(m0 + j * 16 + li, xa.m - 1);
-    ap[j] = xa.a + (int64_t)arow[j] * xa.lda * (QUANT ? 2 : 1) + lg * (QUANT ? 64 : 16);
-  }
-  f32x4 acc[MB];
-#pragma unroll
-  for (int j = 0; j < MB; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint8_t *ap = xa.a + (int64_t)arow * xa.lda * (QUANT ? 2 : 1) + lg * (QUANT ? 64 : 16);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int s = w; s < blocks; s += W) {
     // chunk 16 s + 4 t + lg; behind the last column: zero codes (their scale bytes are zero too)
     const int64_t at = (int64_t)s * (kSuper / 2);
-    i32x4 bv[4], av[MB][4];
-    int sa[MB];
+    i32x4 bv[4], av[4];
     const int sb = (int)xa.bs[scale_word(s, lg, brow, xa.bn4)];
+    int sa;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const bool in = 16 * s + 4 * t + lg < chunks;
       bv[t] = in ? *(const i32x4 *)(bp + at + 64 * t) : i32x4{0, 0, 0, 0};
     }
     if constexpr (QUANT) {
+      sa = 0;
+      i32x4 x[4][4];
 #pragma unroll
-      for (int j = 0; j < MB; ++j) {
-        sa[j] = 0;
-        i32x4 x[4][4];
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int e = 0; e < 4; ++e)
+          x[t][e] = 16 * s + 4 * t + lg < chunks ? *(const i32x4 *)(ap + 4 * (at + 64 * t) + 16 * e) : i32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[t][e] = 16 * s + 4 * t + lg < chunks ? *(const i32x4 *)(ap[j] + 4 * (at + 64 * t) + 16 * e) : i32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < 4; ++t) sa[j] |= (int)(quant32(x[t], av[j][t]) << (8 * t));
-      }
+      for (int t = 0; t < 4; ++t) sa |= (int)(quant32(x[t], av[t]) << (8 * t));
     } else {
 #pragma unroll
-      for (int j = 0; j < MB; ++j) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          av[j][t] = 16 * s + 4 * t + lg < chunks ? *(const i32x4 *)(ap[j] + at + 64 * t) : i32x4{0, 0, 0, 0};
-        sa[j] = (int)xa.as[scale_word(s, lg, arow[j], xa.am4)];
-      }
+      for (int t = 0; t < 4; ++t)
+        av[t] = 16 * s + 4 * t + lg < chunks ? *(const i32x4 *)(ap + at + 64 * t) : i32x4{0, 0, 0, 0};
+      sa = (int)xa.as[scale_word(s, lg, arow, xa.am4)];
     }
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      acc[j] = mfma_fp4<0>(bv[0], av[j][0], acc[j], sb, sa[j]);
-      acc[j] = mfma_fp4<1>(bv[1], av[j][1], acc[j], sb, sa[j]);
-      acc[j] = mfma_fp4<2>(bv[2], av[j][2], acc[j], sb, sa[j]);
-      acc[j] = mfma_fp4<3>(bv[3], av[j][3], acc[j], sb, sa[j]);
-    }
+    acc = mfma_fp4<0>(bv[0], av[0], acc, sb, sa);
+    acc = mfma_fp4<1>(bv[1], av[1], acc, sb, sa);
+    acc = mfma_fp4<2>(bv[2], av[2], acc, sb, sa);
+    acc = mfma_fp4<3>(bv[3], av[3], acc, sb, sa);
   }
-#pragma unroll
-  for (int j = 0; j < MB; ++j) part[w][j][lane] = acc[j];
+  part[w][lane] = acc;
   __syncthreads();
-  for (int j = w; j < MB; j += W) {
-    f32x4 sum = part[0][j][lane];
+  if (w) return;
 #pragma unroll
-    for (int i = 1; i < W; ++i) sum += part[i][j][lane];
-    store_quad(xa, sum, m0 + j * 16 + li, n0 + 4 * lg);
-  }
+  for (int i = 1; i < W; ++i) acc += part[i][lane];
+  store_quad(xa, acc, m0 + li, n0 + 4 * lg);
 }
 
 // ---------------------------------------------------------------------------
@@ -318,38 +300,62 @@ __device__ __forceinline__ void load_lds16_any(const void *base, uint32_t off, u
 
 // A wave's sums, rounded to bf16 and stored from registers: rows m0 .., columns n0 ...  A
 // pair of 16-column blocks trades halves between neighbouring lane groups, so that a
-// lane holds 8 consecutive columns of one block (16 bytes).
-template <int NB, int MB>
-__device__ __forceinline__ void store_tile(const XArgs &xa, const f32x4 (&acc)[NB][MB], int m0, int n0, int li, int lg) {
+// lane holds 8 consecutive columns of one block (16 bytes).  WHOLE: every row and
+// column is inside the matrix and rows are 16-byte aligned: one address a row.
+template <int NB, int MB, bool BIAS, bool WHOLE>
+__device__ __forceinline__ void store_blocks(const XArgs &xa, const f32x4 (&acc)[NB][MB], int m0, int n0, int li, int lg) {
+  const int n1 = n0 + (lg & 1) * 16 + 8 * (lg >> 1);  // first of the lane's stored columns
+  float bf[NB][4];
+  if constexpr (BIAS) {
 #pragma unroll
-  for (int i = 0; i < NB; i += 2) {
-    const int n = n0 + i * 16 + 4 * lg;  // of the lane's own columns, in block i
-    float bf[2][4];
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + i * 16 + 4 * lg + e;
+        bf[i][e] = bf16_bits_to_f32(xa.bias[WHOLE ? n : min(n, xa.n - 1)]);
+      }
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bf[h][e] = xa.bias ? bf16_bits_to_f32(xa.bias[min(n + 16 * h + e, xa.n - 1)]) : 0.0f;
-    const int nn = n0 + (i + (lg & 1)) * 16 + 8 * (lg >> 1);  // of what it stores
+  for (int j = 0; j < MB; ++j) {
+    const int m = m0 + j * 16 + li;
+    uint16_t *row = xa.out + (int64_t)m * xa.ldo + n1;
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
+    for (int i = 0; i < NB; i += 2) {
       uint32_t p[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          p[h][e] = pack_bf16_rne(acc[i + h][j][2 * e] + bf[h][2 * e], acc[i + h][j][2 * e + 1] + bf[h][2 * e + 1]);
+          p[h][e] = BIAS ? pack_bf16_rne(acc[i + h][j][2 * e] + bf[i + h][2 * e], acc[i + h][j][2 * e + 1] + bf[i + h][2 * e + 1])
+                         : pack_bf16_rne(acc[i + h][j][2 * e], acc[i + h][j][2 * e + 1]);
       const auto lo = __builtin_amdgcn_permlane16_swap(p[0][0], p[1][0], false, false);
       const auto hi = __builtin_amdgcn_permlane16_swap(p[0][1], p[1][1], false, false);
       const i32x4 v = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
-      const int m = m0 + j * 16 + li;
-      if (m < xa.m && nn < xa.n) {
-        uint16_t *op = xa.out + (int64_t)m * xa.ldo + nn;
+      if constexpr (WHOLE) {
+        *(i32x4 *)(row + i * 16) = v;
+      } else {
+        const int nn = n1 + i * 16;
+        if (m >= xa.m || nn >= xa.n) continue;
         if (xa.st16_ok && nn + 7 < xa.n)
-          *(i32x4 *)op = v;
+          *(i32x4 *)(row + i * 16) = v;
         else
-          for (int e = 0; e < 8 && nn + e < xa.n; ++e) op[e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+          for (int e = 0; e < 8 && nn + e < xa.n; ++e) row[i * 16 + e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
       }
     }
+  }
+}
+
+template <int NB, int MB>
+__device__ __forceinline__ void store_tile(const XArgs &xa, const f32x4 (&acc)[NB][MB], int m0, int n0, int li, int lg) {
+  if (xa.st16_ok && m0 + MB * 16 <= xa.m && n0 + NB * 16 <= xa.n) {
+    if (xa.bias)
+      store_blocks<NB, MB, true, true>(xa, acc, m0, n0, li, lg);
+    else
+      store_blocks<NB, MB, false, true>(xa, acc, m0, n0, li, lg);
+  } else if (xa.bias) {
+    store_blocks<NB, MB, true, false>(xa, acc, m0, n0, li, lg);
+  } else {
+    store_blocks<NB, MB, false, false>(xa, acc, m0, n0, li, lg);
   }
 }
 
@@ -500,25 +506,35 @@ struct TileLoop {
     mfma_settle<AG>(acc);
     __syncthreads();
   }
-  __device__ __forceinline__ void store(int m0, int n0) {
-    store_tile<NB, MB>(xa, acc, m0 + wm * MH, n0 + wn * NH, li, lg);
-  }
 };
 
-// Tiles of a launch of its own (few workgroups): one tile each.
+// Tiles smaller than 256 x 256, one a workgroup: all of the matrix (xa.full < 0), or
+// the parts of the 256 x 256 tiles from xa.full on.
 template <int MH, int NH, int NBUF, int WPE>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) mxfp4_tile_kernel(const XArgs xa) {
   using T = TileLoop<MH, NH, NBUF>;
   __shared__ __attribute__((aligned(1024))) char smem[NBUF * T::BUF];
   T t(xa, smem);
-  int tm, tn;
-  grouped_tile(xcd_logical_id(blockIdx.x, gridDim.x), (xa.m + T::BM - 1) / T::BM, (xa.n + T::BN - 1) / T::BN, tm, tn);
-  t.at(tm * T::BM, tn * T::BN);
+  const int L = xcd_logical_id(blockIdx.x, gridDim.x);
+  int m0, n0;
+  if (xa.full >= 0) {
+    // consecutive ids, which run on one XCD, are parts of one tile
+    constexpr int PM = 256 / T::BM, PN = 256 / T::BN;
+    int tm, tn;
+    grouped_tile(xa.full + L / (PM * PN), (xa.m + 255) / 256, (xa.n + 255) / 256, tm, tn);
+    m0 = tm * 256 + L % (PM * PN) / PN * T::BM, n0 = tn * 256 + L % PN * T::BN;
+    if (m0 >= xa.m || n0 >= xa.n) return;  // the whole workgroup: no barrier is left waiting
+  } else {
+    // the row tiles that share a weight panel run next to each other
+    const int tmc = (xa.m + T::BM - 1) / T::BM;
+    m0 = L % tmc * T::BM, n0 = L / tmc * T::BN;
+  }
+  t.at(m0, n0);
   t.first_loads();
   __builtin_amdgcn_s_waitcnt(vmcnt_imm((NBUF - 1) * T::LPB));
   __syncthreads();
   t.run();
-  t.store(tm * T::BM, tn * T::BN);
+  store_tile<T::NB, T::MB>(xa, t.acc, m0 + t.wm * MH, n0 + t.wn * NH, t.li, t.lg);
 }
 
 // 256 x 256 tiles [0, xa.full), 4 waves as 2 x 2 of 128 x 128 (256 sums a lane, in
@@ -527,14 +543,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
 // under the last MFMAs of a tile and land while it is stored.
 // k moves in blocks of 128 bytes.  A block's operands are four units of 128 rows
 // (A rows 0 .., B rows 0 .., A rows 128 .., B rows 128 ..; rows and swizzle as in
-// TileLoop) in a ring of nine; its scale words, 8 KiB, in one of two buffers: all
-// of the LDS.  Block d: step 0 multiplies operands that are in registers, reads
-// step 1's and loads the first unit of block d + 2 (the ninth slot); behind the
-// wait for block d + 1 and the barrier, step 1 reads block d + 1's first operands
-// and scale words and loads the other three units and the scale words of block
-// d + 2.  With whole blocks in two buffers instead, all loads in half a step, the
-// loads came in bursts that the L1 took 1,150 cycles and more to deliver, and the
-// matrix units were busy 41% of the time.
+// TileLoop) in a ring of nine; the scale words of two blocks, 8 KiB, in one of two
+// buffers: all of the LDS.  Block d: step 0 multiplies operands that are in
+// registers, reads step 1's and loads the first unit of block d + 2 (the ninth
+// slot); behind the wait for block d + 1 and the barrier, step 1 reads block d + 1's
+// first operands (and its scale words, if they are new) and loads the other three
+// units of block d + 2 (and its scale words).
+// A scaled MFMA takes 16 cycles and two of the wave's issue slots of 4; the other
+// two are all that the loop's remaining instructions have.  With scale words read
+// and copied for every block, addresses added per load and two buffers of whole
+// blocks there were 2.2 of them per MFMA, and the matrix units were busy 41-45% of
+// the time.
 template <int UNITS>
 struct BigLoop {
   static constexpr int UNIT = 128 * KB, RING = UNITS * UNIT, SBUF = 512 * 16;
@@ -544,14 +563,16 @@ struct BigLoop {
   char *smem;
   uint32_t lds0;
   int w, wm, wn, lane, li, lg, lch, chunks, nd, tmc, tnc;
-  int L, end, wgs;           // the tile whose blocks are loaded, and the workgroup's others
-  int lb;                    // its next block
-  int tm, tn;                // its place
-  int slot, sbuf;            // ring slot of the current block's first unit, its scale buffer
-  uint32_t doff[4][4], soff[2], rdq[2], rds[16];
-  f32x4 acc[8][8];           // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
-  i32x4 cur[16], nxt[16];    // operands: A blocks 0 .. 7, B blocks 0 .. 7
-  int sc[16], nsc[16];
+  int L, end, wgs;             // the tile whose blocks are loaded, and the workgroup's others
+  int lb;                      // its next block
+  const uint8_t *abase, *bbase;  // the codes from that block on
+  int slot;                    // ring slot of the current block's first unit
+  int sload;                   // buffer of the next scale words
+  int sread, rb;               // where the next block's scale bytes are read, and its number in its tile
+  uint32_t doff[4][4], soff[2], rdq[2], rds[2][4];
+  f32x4 acc[8][8];             // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
+  i32x4 cur[16], nxt[16];      // operands: A blocks 0 .. 7, B blocks 0 .. 7
+  int sc[16];                  // their scale words
 
   __device__ __forceinline__ BigLoop(const XArgs &args, char *lds) : xa(args), smem(lds) {
     lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
@@ -561,112 +582,150 @@ struct BigLoop {
     lch = (lane & 7) ^ ((4 * (w & 1) + (lane >> 4)) & 7);
 #pragma unroll
     for (int q = 0; q < 2; ++q) rdq[q] = (uint32_t)(li * KB + (((4 * q + lg) ^ ((li >> 1) & 7)) * 16));
+    // scale word of entry g, row r: word r ^ 16 g of the entry's 256 (a read of 16
+    // rows and 4 entries meets 64 banks); rds: by r / 16 mod 4
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = (r < 8 ? wm * 128 + r * 16 : wn * 128 + (r - 8) * 16) + li;
-      rds[r] = (uint32_t)(RING + (r < 8 ? 0 : 4096) + (lg * 256 + (row + 16 * lg) % 256) * 4);
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t word = (uint32_t)(RING + lg * 1024 + ((c ^ lg) * 16 + li) * 4);
+      rds[0][c] = word + wm * 512, rds[1][c] = word + 4096 + wn * 512;
     }
     tmc = (xa.m + 255) / 256, tnc = (xa.n + 255) / 256;
   }
-  // Where tile L's rows and scale words lie (see TileLoop::at)
+  // Where tile L's rows and scale words lie (see TileLoop::at), from its first block
   __device__ __forceinline__ void at() {
+    int tm, tn;
     grouped_tile(L, tmc, tnc, tm, tn);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = (j >> 1) * 128 + (w + 4 * i) * 8 + (lane >> 3);
-        doff[j][i] = j & 1 ? (uint32_t)((int64_t)min(tn * 256 + r, xa.n - 1) * xa.ldb)
-                           : (uint32_t)((int64_t)min(tm * 256 + r, xa.m - 1) * xa.lda);
+        doff[j][i] = (j & 1 ? (uint32_t)((int64_t)min(tn * 256 + r, xa.n - 1) * xa.ldb)
+                            : (uint32_t)((int64_t)min(tm * 256 + r, xa.m - 1) * xa.lda)) + lch * 16;
       }
-    const int r = (lane * 4 - 16 * w + 256) % 256;  // entry g = w of A's words, then of B's
+    const int r = (lane * 4) ^ (16 * w);  // entry g = w of A's words, then of B's
     soff[0] = (uint32_t)(((int64_t)w * xa.am4 + min(tm * 256 + r, xa.am4 - 4)) * 4);
     soff[1] = (uint32_t)(((int64_t)w * xa.bn4 + min(tn * 256 + r, xa.bn4 - 4)) * 4);
+    lb = 0, abase = xa.a, bbase = xa.b;
+    if (nd == 1) last_block();
+  }
+  // the load cursor is at the row's last block: chunks past the row's end repeat its last
+  __device__ __forceinline__ void last_block() {
+    const uint32_t back = (uint32_t)max(8 * (nd - 1) + lch - (chunks - 1), 0) * 16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) doff[j][i] -= back;
   }
   // load i of unit j of the block at the load cursor, into ring slot s
-  __device__ __forceinline__ void load_data(int s, int j, int i, uint32_t koff) {
-    load_lds16_any(j & 1 ? xa.b : xa.a, doff[j][i] + koff, lds0 + (uint32_t)(s * UNIT + (w + 4 * i) * 1024));
+  __device__ __forceinline__ void load_data(int s, int j, int i) {
+    load_lds16_any(j & 1 ? bbase : abase, doff[j][i], lds0 + (uint32_t)(s * UNIT + (w + 4 * i) * 1024));
   }
-  __device__ __forceinline__ void load_scale(int buf, int i) {
-    const uint32_t *base = i ? xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4 : xa.as + (int64_t)(lb >> 1) * 4 * xa.am4;
-    load_lds16_any(base, soff[i], lds0 + (uint32_t)(RING + buf * SBUF + i * 4096 + w * 1024));
+  __device__ __forceinline__ void load_scales() {
+    const uint32_t to = lds0 + (uint32_t)(RING + sload * SBUF + w * 1024);
+    load_lds16_any(xa.as + (int64_t)(lb >> 1) * 4 * xa.am4, soff[0], to);
+    load_lds16_any(xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4, soff[1], to + 4096);
+    sload ^= 1;
   }
-  __device__ __forceinline__ uint32_t koff() const { return (uint32_t)(min(8 * lb + lch, chunks - 1) * 16); }
   // the load cursor's next block: of this tile, of the workgroup's next one, or
   // (none left) the same again, into slots that nobody reads
   __device__ __forceinline__ void advance() {
     if (lb + 1 < nd) {
       ++lb;
+      abase += KB, bbase += KB;
+      if (lb + 1 == nd && (chunks & 7)) last_block();
     } else if (L + wgs < end) {
       L += wgs;
-      lb = 0;
       at();
     }
   }
   static __device__ __forceinline__ int wrap(int s) { return s >= UNITS ? s - UNITS : s; }
-  __device__ __forceinline__ i32x4 read_op(int s, int q, int r) const {  // s: slot of the block's first unit
-    const int unit = r < 8 ? 2 * wm : 2 * wn + 1;
-    return *(const i32x4 *)(smem + (uint32_t)(wrap(s + unit) * UNIT) + rdq[q] + (r & 7) * 16 * KB);
+  // operand r (A blocks 0 .. 7, then B's) of step q of the block whose units start at ring slot s
+  __device__ __forceinline__ uint32_t op_base(int s, int q, bool b) const {
+    return (uint32_t)(wrap(s + (b ? 2 * wn + 1 : 2 * wm)) * UNIT) + rdq[q];
   }
-  __device__ __forceinline__ int read_scale(int buf, int r) const { return *(const int *)(smem + (uint32_t)(buf * SBUF) + rds[r]); }
+  __device__ __forceinline__ i32x4 read_op(uint32_t base, int r) const { return *(const i32x4 *)(smem + base + (r & 7) * 16 * KB); }
+  // scale bytes of operand r for the block whose bytes start at `from` of the buffers: step 0's, then step 1's
+  __device__ __forceinline__ int read_scale(const uint32_t (&at)[2][4], int r) const {
+    return *(const uint16_t *)(smem + at[r >> 3][r & 3] + ((r & 7) >> 2) * 256);
+  }
+  // where the next block's scale bytes are read: the other two bytes of the words, or the other buffer's first two
+  __device__ __forceinline__ void next_scales() { sread = rb & 1 ? (sread ^ SBUF) & ~2 : rb + 1 == nd ? sread ^ SBUF : sread | 2, rb = rb + 1 == nd ? 0 : rb + 1; }
 
   // the first tile's first two blocks on their way, the first in registers
   __device__ __forceinline__ void begin() {
-    slot = 0, sbuf = 0, lb = 0;
+    slot = 0, sload = 0;
     at();
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
-      const uint32_t ko = koff();
+      if ((lb & 1) == 0) load_scales();
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_data(4 * d + j, j, i, ko);
-      load_scale(d, 0);
-      load_scale(d, 1);
+        for (int i = 0; i < 4; ++i) load_data(4 * d + j, j, i);
       advance();
     }
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(18));
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(16));
     __syncthreads();
+    const uint32_t a = op_base(0, 0, false), b = op_base(0, 0, true);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      cur[r] = read_op(0, 0, r);
-      sc[r] = read_scale(0, r);
+      cur[r] = read_op(r < 8 ? a : b, r);
+      sc[r] = read_scale(rds, r);
     }
+    sread = 0, rb = 0;
+    next_scales();
+    clear();
   }
-  template <int ODD, bool FIRST>
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
   __device__ __forceinline__ void block() {
     const int next = wrap(slot + 4), over = wrap(next + 4);  // over: block d + 2's first unit
-    uint32_t ko = koff();
+    {
+      const uint32_t a = op_base(slot, 1, false), b = op_base(slot, 1, true);
 #pragma unroll
-    for (int idx = 0; idx < 64; ++idx) {
-      if (idx % 4 == 0) nxt[idx / 4] = read_op(slot, 1, idx / 4);
-      if (idx % 16 == 2) load_data(over, 0, idx / 16, ko);
-      mfma_fp4_into<2 * ODD, true, FIRST>(acc[idx >> 3][idx & 7], cur[8 + (idx >> 3)], cur[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int idx = 0; idx < 64; ++idx) {
+        if (idx % 4 == 0) nxt[idx / 4] = read_op(idx / 4 < 8 ? a : b, idx / 4);
+        if (idx % 16 == 2) load_data(over, 0, idx / 16);
+        mfma_fp4_into<0, true>(acc[idx >> 3][idx & 7], cur[8 + (idx >> 3)], cur[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(4));
     __syncthreads();
+    if ((lb & 1) == 0) load_scales();
+    int asc[8];  // the A rows' next scale bytes (B's replace the old ones, each after its last use)
+    {
+      const uint32_t a = op_base(next, 0, false), b = op_base(next, 0, true);
+      uint32_t at[2][4];
 #pragma unroll
-    for (int idx = 0; idx < 64; ++idx) {
-      if (idx % 4 == 0) {
-        cur[idx / 4] = read_op(next, 0, idx / 4);
-        nsc[idx / 4] = read_scale(sbuf ^ 1, idx / 4);
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) at[h][c] = rds[h][c] + sread;
+#pragma unroll
+      for (int idx = 0; idx < 64; ++idx) {
+        if (idx % 4 == 0) cur[idx / 4] = read_op(idx / 4 < 8 ? a : b, idx / 4);
+        if (idx % 8 == 1) asc[idx / 8] = read_scale(at, idx / 8);
+        if (idx % 4 == 2 && idx / 4 < 12) load_data(wrap(over + 1 + idx / 16), 1 + idx / 16, idx / 4 % 4);
+        mfma_fp4_into<1, true>(acc[idx >> 3][idx & 7], nxt[8 + (idx >> 3)], nxt[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (idx % 8 == 7) sc[8 + idx / 8] = read_scale(at, 8 + idx / 8);
       }
-      if (idx % 4 == 2 && idx / 4 < 12) load_data(wrap(over + 1 + idx / 16), 1 + idx / 16, idx / 4 % 4, ko);
-      if (idx % 4 == 2 && idx / 4 >= 12 && idx / 4 < 14) load_scale(sbuf, idx / 4 - 12);
-      mfma_fp4_into<2 * ODD + 1, true>(acc[idx >> 3][idx & 7], nxt[8 + (idx >> 3)], nxt[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
-      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sc[r] = nsc[r];
-    slot = next, sbuf ^= 1;
+    for (int r = 0; r < 8; ++r) sc[r] = asc[r];
+    next_scales();
+    slot = next;
+    advance();
     // a register that vector code wrote (a copy above) may be an MFMA's operand two wait states later
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 1");
     __builtin_amdgcn_sched_barrier(0);
-  }
-  __device__ __forceinline__ void store(int m0, int n0) {
-    store_tile<8, 8>(xa, acc, m0 + wm * 128, n0 + wn * 128, li, lg);
   }
 };
 
@@ -684,25 +743,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
   int L = t.L;  // the tile that is multiplied
   t.begin();
   for (;;) {
-    int d = 1;
-    t.template block<0, true>();
-    t.advance();
-    for (; d + 1 < t.nd; d += 2) {
-      t.template block<1, false>();
-      t.advance();
-      t.template block<0, false>();
-      t.advance();
-    }
-    if (d < t.nd) {
-      t.template block<1, false>();
-      t.advance();
-    }
+    for (int d = 0; d < t.nd; ++d) t.block();
     mfma_settle<true>(t.acc);
     int tm, tn;
     grouped_tile(L, t.tmc, t.tnc, tm, tn);
-    t.store(tm * 256, tn * 256);
+    store_tile<8, 8>(xa, t.acc, tm * 256 + t.wm * 128, tn * 256 + t.wn * 128, t.li, t.lg);
     L += t.wgs;
     if (L >= t.end) break;
+    t.clear();
   }
   // every wave drains its loads before the workgroup ends
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -722,9 +770,6 @@ unsigned quant_grid(int32_t rows, int32_t cols) {
   return g <= INT32_MAX ? (unsigned)g : 0u;
 }
 
-// rows that mxfp4_rows_kernel quantizes itself
-constexpr int kFusedRows = 16;
-
 int64_t codes_bytes(int32_t rows, int32_t k) { return ((int64_t)rows * (k / 2) + 255) / 256 * 256; }
 int64_t scale_bytes(int32_t rows, int32_t k) { return ((int64_t)k + kSuper - 1) / kSuper * 16 * round4(rows); }
 
@@ -737,7 +782,6 @@ int check_product(const char *what, const void *out, const uint8_t *b, const uin
     return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
   if (ldb % 16 || ldb < k / 2 || ldo < n)
     return set_error(TMHD_ERR_INVALID, "%s: row strides %lld, %lld", what, (long long)ldb, (long long)ldo);
-  if ((m + 63) / 64 > 65535) return set_error(TMHD_ERR_UNSUPPORTED, "%s: m %d is too large", what, m);
   return TMHD_OK;
 }
 
@@ -748,27 +792,119 @@ XArgs product_args(void *out, const uint8_t *a, const uint8_t *a_scale, const ui
                (int32_t)((uintptr_t)out % 8 == 0 && ldo % 4 == 0), (int32_t)((uintptr_t)out % 16 == 0 && ldo % 8 == 0), 0};
 }
 
+// Tiles of 2 MH x 2 NH: the parts of the last `tiles` 256 x 256 tiles, or (0) all of the matrix.
+template <int MH, int NH, int NBUF, int WPE>
+void launch_tiles(XArgs xa, int64_t tiles, hipStream_t s) {
+  const int64_t wgs = tiles ? tiles * (256 / (2 * MH)) * (256 / (2 * NH))
+                            : (int64_t)((xa.m + 2 * MH - 1) / (2 * MH)) * ((xa.n + 2 * NH - 1) / (2 * NH));
+  if (!tiles) xa.full = -1;
+  hipLaunchKernelGGL((mxfp4_tile_kernel<MH, NH, NBUF, WPE>), dim3((unsigned)wgs), dim3(256), 0, s, xa);
+}
+
+// The tiled forms and, per 256 columns of k, the microseconds of a round of them:
+// `one` + `fill` * (share of the CUs in use), or `two` with a second workgroup on
+// each CU.  Fitted to every form forced on products of 1 to 12,252 rows and weights
+// of 640 x 2,048 to 13,824 x 5,120 that were not read shortly before; us, rows on
+// 13,824 x 5,120 (and on 5,376 x 5,376):
+//   rows          1            64           200          331          1,024        2,048
+//   64 x 64       7.8  (7.2)   8.7  (7.7)   21.6 (11.7)  30.7 (12.4)  70   (30.7)  177  (71)
+//   128 x 64      10.3 (9.9)   11.0 (10.3)  21.0 (11.0)  30.6 (11.5)  67   (29.9)  144  (63)
+//   128 x 128     13.1 (12.9)  13.8 (13.3)  15.9 (14.3)  27.5 (14.4)  57.6 (28.2)  105  (46)
+//   128 x 128, 2  14.7 (14.2)  15.4 (14.5)  16.6 (15.2)  22.8 (15.3)  44.2 (21.8)  86   (41)
+//   256 x 256     35.9 (35.4)  36.7 (36.2)  38.5 (37.7)  41.9 (38.3)  45.9 (40.2)  88   (41)
+struct TileCost {
+  int form, bm, bn, per_cu;
+  double one, fill, two;
+};
+constexpr TileCost kTiles[] = {
+    {TMHD_MXFP4_64X64, 64, 64, 2, 0.20, 0.03, 0.46},
+    {TMHD_MXFP4_128X64, 128, 64, 1, 0.37, 0.02, 0.0},
+    {TMHD_MXFP4_128X128, 128, 128, 1, 0.52, 0.10, 0.0},
+    {TMHD_MXFP4_128X128X2, 128, 128, 2, 0.58, 0.08, 1.08},
+    {TMHD_MXFP4_256X256, 256, 256, 1, 1.65, 0.35, 0.0},
+};
+constexpr double kLaunchUs = 3.5;  // first loads, stores and the launch itself
+
+double tiles_us(const TileCost &c, int64_t wgs, double blocks, int cus) {
+  const int64_t slots = (int64_t)cus * c.per_cu, rest = wgs % slots;
+  const double full = c.per_cu == 2 ? c.two : c.one + c.fill;
+  const double last = rest == 0 ? 0.0 : rest <= cus ? c.one + c.fill * (double)rest / cus : c.two;
+  return kLaunchUs + blocks * ((double)(wgs / slots) * full + last);
+}
+
+// The cheapest form of an m x n x k product: `rows` or tiles of one kind, or 256 x
+// 256 tiles in whole rounds and `tail` tiles of another kind behind them.
+struct Form {
+  int form;
+  int64_t tail;  // 256 x 256 tiles that `form` runs in parts; 0: `form` runs all
+};
+Form pick_form(int32_t m, int32_t n, int32_t k, int cus) {
+  // 16 x 16 tiles straight from memory: up to 16 rows and about a workgroup and a
+  // half per CU (1 row on 5,376 x 5,376: 5.6 us, 64 x 64 tiles 7.2; on 13,824 x
+  // 5,120 8.7 and 7.8; on 640 x 2,048 4.0 and 4.5)
+  if (m <= 16 && (n + 15) / 16 <= cus * 3 / 2) return {TMHD_MXFP4_ROWS, 0};
+  const double blocks = (double)((k + 255) / 256);
+  const int64_t big = (int64_t)((m + 255) / 256) * ((n + 255) / 256);
+  Form best{TMHD_MXFP4_256X256, 0};
+  double us = 1e30;
+  for (const TileCost &c : kTiles) {
+    const double t = tiles_us(c, (int64_t)((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn), blocks, cus);
+    if (t < us) us = t, best = {c.form, 0};
+  }
+  const int64_t tail = big % cus;
+  if (big > cus && tail) {
+    const double whole = blocks * (double)(big / cus) * 2.0;
+    for (const TileCost &c : kTiles) {
+      if (c.form != TMHD_MXFP4_64X64 && c.form != TMHD_MXFP4_128X64 && c.form != TMHD_MXFP4_128X128) continue;
+      const double t = kLaunchUs + whole + tiles_us(c, tail * (256 / c.bm) * (256 / c.bn), blocks, cus);
+      if (t < us) us = t, best = {c.form, tail};
+    }
+  }
+  return best;
+}
+
+// Whether mxfp4_rows_kernel quantizes the rows itself: it takes the product, and its
+// waves have one block of k each.  A launch less (1 row on 640 x 2,048: 3.6 us
+// against 4.8, 16 rows 4.9 and 5.5), but every workgroup quantizes all of k: with
+// more of it a wave's blocks wait for each other (1 row on 5,376 x 5,376: 9.2 against
+// 8.1, 16 rows 15.8 and 10.3).
+bool fused_quant(int32_t m, int32_t n, int32_t k) {
+  return m <= 16 && k <= 4 * kSuper && pick_form(m, n, k, std::max(device_cus(), 8)).form == TMHD_MXFP4_ROWS;
+}
+
 // The product of checked arguments.
 int launch_product(const char *what, void *out, const uint8_t *a, const uint8_t *a_scale, const uint8_t *b,
                    const uint8_t *b_scale, const void *bias, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb,
                    int64_t ldo, hipStream_t s) {
   XArgs xa = product_args(out, a, a_scale, b, b_scale, bias, m, n, k, lda, ldb, ldo);
-  const unsigned nt = (unsigned)((n + 15) / 16);
+  const int cus = std::max(device_cus(), 8);
   // the tiles take 32-bit row and scale offsets
-  const bool wide = (int64_t)(m - 1) * lda + k < (int64_t)1 << 32 && (int64_t)(n - 1) * ldb + k < (int64_t)1 << 32;
-  if (wide && m > 64) {
-    const int64_t big = ((int64_t)(m + 255) / 256) * ((n + 255) / 256);
-    if (big >= 128) {
-      xa.full = (int32_t)big;
-      hipLaunchKernelGGL(mxfp4_big_kernel, dim3((unsigned)std::min<int64_t>(big, std::max(device_cus(), 8))), dim3(256), 0, s, xa);
-    }
-    else
-      hipLaunchKernelGGL((mxfp4_tile_kernel<64, 64, 4, 1>), dim3((unsigned)(((int64_t)(m + 127) / 128) * ((n + 127) / 128))),
-                         dim3(256), 0, s, xa);
-  } else if (m <= 16)
-    hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4, false>), dim3(nt, 1), dim3(256), 0, s, xa);
-  else
-    hipLaunchKernelGGL((mxfp4_rows_kernel<4, 4, false>), dim3(nt, (unsigned)((m + 63) / 64)), dim3(256), 0, s, xa);
+  const bool narrow = (int64_t)(m - 1) * lda + k < (int64_t)1 << 32 && (int64_t)(n - 1) * ldb + k < (int64_t)1 << 32;
+  const Form f = narrow ? pick_form(m, n, k, cus) : Form{TMHD_MXFP4_ROWS, 0};
+  const int64_t big = (int64_t)((m + 255) / 256) * ((n + 255) / 256);
+  const int64_t rows_grid = (int64_t)((m + 15) / 16) * ((n + 15) / 16);
+  if (f.form == TMHD_MXFP4_ROWS ? rows_grid > INT32_MAX : big > INT32_MAX / 16)
+    return set_error(TMHD_ERR_UNSUPPORTED, "%s: %d x %d is too large", what, m, n);
+  if (f.tail || f.form == TMHD_MXFP4_256X256) {
+    xa.full = (int32_t)(big - f.tail);
+    hipLaunchKernelGGL(mxfp4_big_kernel, dim3((unsigned)std::min<int64_t>(xa.full, cus)), dim3(256), 0, s, xa);
+  }
+  switch (f.form) {
+    case TMHD_MXFP4_ROWS:
+      hipLaunchKernelGGL(mxfp4_rows_kernel<false>, dim3((unsigned)rows_grid), dim3(256), 0, s, xa);
+      break;
+    case TMHD_MXFP4_64X64:
+      launch_tiles<32, 32, 4, 2>(xa, f.tail, s);
+      break;
+    case TMHD_MXFP4_128X64:
+      launch_tiles<64, 32, 5, 1>(xa, f.tail, s);
+      break;
+    case TMHD_MXFP4_128X128:
+      launch_tiles<64, 64, 4, 1>(xa, f.tail, s);
+      break;
+    case TMHD_MXFP4_128X128X2:
+      launch_tiles<64, 64, 2, 2>(xa, f.tail, s);
+  }
   return check_launch(what);
 }
 
@@ -820,8 +956,7 @@ extern "C" int tmhd_gemm_mxfp4(void *out, const uint8_t *a, const uint8_t *b, co
 }
 
 extern "C" int64_t tmhd_linear_mxfp4_workspace_bytes(int32_t m, int32_t n, int32_t k) {
-  (void)n;
-  if (m <= tmhd::kFusedRows || k <= 0 || k % 32) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || k % 32 || tmhd::fused_quant(m, n, k)) return 0;
   return tmhd::codes_bytes(m, k) + tmhd::scale_bytes(m, k);
 }
 
@@ -835,9 +970,9 @@ extern "C" int tmhd_linear_mxfp4(void *out, const void *x, const uint8_t *b, con
   if (!x || (uintptr_t)x % 16) return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
   if (ldx % 8 || ldx < k) return set_error(TMHD_ERR_INVALID, "%s: row stride %lld", what, (long long)ldx);
   hipStream_t s = (hipStream_t)stream;
-  if (m <= kFusedRows) {
+  if (fused_quant(m, n, k)) {
     const XArgs xa = product_args(out, (const uint8_t *)x, nullptr, b, b_scale, bias, m, n, k, ldx, ldb, ldo);
-    hipLaunchKernelGGL((mxfp4_rows_kernel<1, 4, true>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, xa);
+    hipLaunchKernelGGL(mxfp4_rows_kernel<true>, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, xa);
     return check_launch(what);
   }
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < codes_bytes(m, k) + scale_bytes(m, k))
@@ -845,4 +980,10 @@ extern "C" int tmhd_linear_mxfp4(void *out, const void *x, const uint8_t *b, con
   uint8_t *q = (uint8_t *)workspace, *scale = q + codes_bytes(m, k);
   if (int st = tmhd_mxfp4_quant(q, scale, x, m, k, ldx, stream)) return st;
   return launch_product(what, out, q, scale, b, b_scale, bias, m, n, k, k / 2, ldb, ldo, s);
+}
+
+extern "C" int tmhd_gemm_mxfp4_form(int32_t m, int32_t n, int32_t k, int32_t cus) {
+  using namespace tmhd;
+  if (m <= 0 || n <= 0 || k <= 0 || k % 32) return -1;
+  return pick_form(m, n, k, cus > 0 ? cus : std::max(device_cus(), 8)).form;
 }

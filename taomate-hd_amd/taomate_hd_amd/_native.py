@@ -29,6 +29,10 @@ TMHD_ERR_HIP = 3
 GEMM_WHOLE, GEMM_SPLIT_K, GEMM_64X64, GEMM_64X128, GEMM_128X128, GEMM_192X128, GEMM_256X128 = range(7)
 
 
+# tmhd_gemm_mxfp4_form
+MXFP4_ROWS, MXFP4_64X64, MXFP4_128X64, MXFP4_128X128, MXFP4_128X128X2, MXFP4_256X256 = range(6)
+
+
 class KVSegment(ctypes.Structure):
     _fields_ = [
         ("k", c_void_p),
@@ -262,6 +266,7 @@ _LOWBIT_SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_int64,
          c_int64, c_void_p],
     ),
+    "tmhd_gemm_mxfp4_form": (c_int, [c_int32, c_int32, c_int32, c_int32]),
     "tmhd_linear_mxfp4": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64,

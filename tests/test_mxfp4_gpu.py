@@ -187,25 +187,53 @@ def test_on_another_stream_and_in_a_graph(torch_mod, dev):
         assert torch.equal(out, mxfp4_linear(new, w, ws))
 
 
-# tiles of 256 and of 128, one and more blocks of k, odd numbers of them, k ending inside a block, ragged edges
-TILED = [(257, 128, 32), (256, 256, 256), (256, 256, 512), (65, 128, 768), (129, 131, 800), (300, 4112, 1312),
-         (3000, 3000, 544), (2100, 5000, 1280), (4500, 2000, 64),
-         (4900, 5003, 1056), (2049, 8200, 256)]
+# Products that take each form: one and more blocks of k, odd numbers of them, k ending inside a block and inside a
+# scale word, ragged edges, one and several tiles a workgroup, last rounds in parts
+TILED = {
+    "ROWS": [(16, 640, 2080), (5, 4000, 96)],
+    "64X64": [(17, 130, 32), (65, 128, 768), (129, 131, 800), (1, 13824, 1056), (1000, 640, 544)],
+    "128X64": [(200, 5376, 512), (331, 5300, 1312), (2048, 640, 2048)],
+    "128X128": [(200, 10752, 544), (512, 5376, 1024), (700, 5003, 288)],
+    "128X128X2": [(331, 13824, 256), (2048, 5376, 1056), (1030, 8200, 32)],
+    "256X256": [(12252, 5376, 512), (12252, 5376, 2336), (12000, 5200, 64)],
+}
 
 
-@pytest.mark.parametrize("m,n,k", TILED)
-def test_tiled_product(torch_mod, dev, m, n, k):
-    """Whole products of the tiled kernels, against an fp64 product on the GPU."""
+@pytest.mark.parametrize("form,m,n,k", [(f, *size) for f, sizes in TILED.items() for size in sizes])
+def test_forms_of_the_product(torch_mod, dev, form, m, n, k):
+    from taomate_hd_amd import _native
+
+    assert _native.load().tmhd_gemm_mxfp4_form(m, n, k, 0) == getattr(_native, f"MXFP4_{form}")
+    _check_whole(torch_mod, dev, m, n, k)
+
+
+# 256 x 256 tiles in whole rounds, the last ones in parts
+@pytest.mark.parametrize("m,n,k", [(4836, 10752, 5376), (12252, 13824, 1056), (4352, 4000, 2080)])
+def test_last_rounds_in_parts(torch_mod, dev, m, n, k):
+    from taomate_hd_amd import _native
+
+    assert -(-m // 256) * -(-n // 256) > 256
+    assert _native.load().tmhd_gemm_mxfp4_form(m, n, k, 0) in (
+        _native.MXFP4_64X64, _native.MXFP4_128X64, _native.MXFP4_128X128)
+    _check_whole(torch_mod, dev, m, n, k)
+
+
+def _check_whole(torch, dev, m, n, k):
+    """A whole product against an fp64 product on the GPU, and the row behind it left alone."""
     from taomate_hd_amd import mxfp4_dequant, mxfp4_quant, mxfp4_scaled_mm_out
 
-    torch = torch_mod
     x, w, b = _rows(torch, m, k, 1, dev, spread=1), _rows(torch, n, k, 2, dev, spread=1), _rows(torch, 1, n, 3, dev)[0]
     (a, sa), (wq, sw) = mxfp4_quant(x), mxfp4_quant(w)
     av, wv = mxfp4_dequant(a, sa).double(), mxfp4_dequant(wq, sw).double()
-    want = av @ wv.t() + b.double()
-    slack = (k + 1) * 2.0 ** -23 * (av.abs() @ wv.abs().t() + b.double().abs())
-    out = torch.full((m + 1, n), 7.0, dtype=torch.bfloat16, device=dev)
-    mxfp4_scaled_mm_out(out[:m], a, wq.t(), sa, sw, b)
-    err = (out[:m].double() - want).abs()
-    assert bool((err <= HALF_BF16 * (want.abs() + slack) + slack).all())
-    assert bool((out[m] == 7.0).all())
+    for bias in (b, None):
+        want = av @ wv.t()
+        slack = av.abs() @ wv.abs().t()
+        if bias is not None:
+            want += b.double()
+            slack += b.double().abs()
+        slack *= (k + 1) * 2.0 ** -23
+        out = torch.full((m + 1, n), 7.0, dtype=torch.bfloat16, device=dev)
+        mxfp4_scaled_mm_out(out[:m], a, wq.t(), sa, sw, bias)
+        err = (out[:m].double() - want).abs()
+        assert bool((err <= HALF_BF16 * (want.abs() + slack) + slack).all())
+        assert bool((out[m] == 7.0).all())
