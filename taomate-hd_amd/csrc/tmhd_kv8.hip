@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(2 * D) kv8_token_major_kernel(const View vw, u
   }
 }
 
-// ---- attention of few query rows
+// ---- attention
 
 struct Seg8 {
   const uint8_t *k, *v, *ks, *vs;
@@ -282,230 +282,256 @@ struct Call8 {
   int64_t qts, qhs, ots, ohs;
   const int32_t *q_rows, *o_rows;
   int32_t q_row0, o_row0, lq;
-  int32_t seg0, nseg, blocks;        // its segments, and their 64-token blocks in all
-  int32_t row_tiles, splits, first;  // first: of the launch's workgroups
-  int32_t part0;                     // first partial result (splits > 1)
+  int32_t seg0, blocks;     // its first segment, and its segments' 64-token blocks in all
+  int32_t row_tiles, first;  // first: of the launch's units of work (item, block)
 };
 struct Args8 {
   Call8 call[kMaxCalls];
   Seg8 seg[kMaxSegs];
   int32_t n_calls, heads;
-  float scale2;  // |softmax scale| times log2 e
-  int32_t flip;  // sign bits to change in Q: a negative scale's
+  int32_t units, wgs;  // the launch's units of work, and the workgroups they are dealt to
+  float scale2;        // |softmax scale| times log2 e
+  int32_t flip;        // sign bits to change in Q: a negative scale's
   float *ws;
 };
 
+// The work is one item per (call, head, tile of query rows), of its call's 64-token
+// blocks each; the items' blocks in a row are dealt evenly to the workgroups,
+// which so all end at about the same time.  An item that lies in one workgroup's
+// range is written out; the parts of a cut one go to ws, two slots a workgroup
+// (its range may begin and end inside an item), and are merged afterwards.
+__device__ __forceinline__ int range_begin(const Args8 &aa, int wg) { return (int)((int64_t)aa.units * wg / aa.wgs); }
+
+// The range of a workgroup where neighbouring ranges share keys: runs on one XCD
+__device__ __forceinline__ int xcd_wg(int wgs) {
+  const int b = (int)blockIdx.x, xcd = b & 7, per = wgs >> 3, rem = wgs & 7;
+  return (b >> 3) + xcd * per + min(xcd, rem);
+}
+
+struct Piece {
+  int call, head, tile, b_begin, b_end;  // blocks of the item
+  bool whole;
+};
+// The piece of work that starts at unit x of a range that ends at `end`
+__device__ __forceinline__ Piece piece_at(const Args8 &aa, int x, int end) {
+  Piece p;
+  p.call = 0;
+  while (p.call + 1 < aa.n_calls && x >= aa.call[p.call + 1].first) ++p.call;
+  const Call8 &cl = aa.call[p.call];
+  const int rel = x - cl.first, item = rel / cl.blocks;
+  p.b_begin = rel - item * cl.blocks;
+  p.b_end = min(cl.blocks, p.b_begin + end - x);
+  p.head = item / cl.row_tiles, p.tile = item - p.head * cl.row_tiles;
+  p.whole = p.b_begin == 0 && p.b_end == cl.blocks;
+  return p;
+}
+
+// The segment that holds block b of a call, going on from segment si, whose first block is `first`
+__device__ __forceinline__ void find_segment(const Args8 &aa, int b, int &si, int &first) {
+  for (;;) {
+    const int n = (aa.seg[si].tokens + kBlock - 1) / kBlock;
+    if (b - first < n) return;
+    first += n;
+    ++si;
+  }
+}
+
+// floats of a partial result: ROWS of D sums, then the references and the weights' sums
+template <int D, int ROWS>
+constexpr int part_floats() { return ROWS * (D + 2); }
+
+// Q operands of 32 rows from row r0 on, PERM: in the channel order of the K chunks
+template <int D, bool PERM>
+__device__ __forceinline__ void load_q(const Args8 &aa, const Call8 &cl, int head, int r0, int lr, int g, bf16x8 (&qf)[D / 16]) {
+  const int r = min(r0 + lr, cl.lq - 1);
+  const int64_t row = cl.q_rows ? cl.q_rows[r] : cl.q_row0 + r;
+  const uint16_t *qp = cl.q + row * cl.qts + (int64_t)head * cl.qhs;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) {
+    i32x4 v = *(const i32x4 *)(qp + (PERM ? 32 * (t >> 1) + 16 * g + 8 * (t & 1) : 16 * t + 8 * g));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] ^= aa.flip;
+    qf[t] = __builtin_bit_cast(bf16x8, v);
+  }
+}
+
+__device__ __forceinline__ i32x2 pack4(const f32x4 &v, float f) {
+  return i32x2{(int)pack_bf16_rne(v[0] * f, v[1] * f), (int)pack_bf16_rne(v[2] * f, v[3] * f)};
+}
+
+// The number of valid keys, as only a branch that few tiles take sees it: the
+// compiler may not run the branch's instructions (two per score) for every tile.
+__device__ __forceinline__ int in_branch(int keys) {
+  asm volatile("" : "+s"(keys));
+  return keys;
+}
+
 constexpr int kWaves8 = 4;
 
-// Rows of a partial result: QB * 32 of D sums, then the maxima and the weights' sums.
-template <int D, int QB>
-constexpr int part_floats() { return QB * 32 * (D + 2); }
-
-// A workgroup takes 32 QB query rows of one head over a range of 64-token blocks;
-// its four waves take the blocks in turn and merge through LDS.  Per 32 keys a
-// lane loads the 16-byte chunks that are its MFMA operands (no LDS on the way:
-// each code is used once, by all query rows) and turns them into bf16, exactly;
-// S^T = K Q^T leaves 16 keys of one query in a lane, in the order in which the
-// V chunks hold them, so P feeds the second product from registers.  A block's K
-// scale joins the softmax scale, its V scale multiplies P (both powers of two).
-// Bound by HBM: 64 rows need 1024 MFMA cycles per 8 KiB and wave, 32 bytes a
-// clock for a CU, against about 11 that HBM delivers to it.
-template <int D, int QB, bool E4M3>
-__global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_eu(QB == 1 ? 2 : 1, QB == 1 ? 2 : 1)))
-kv8_attn_kernel(const Args8 aa) {
-  constexpr int KC = D / 32;   // 16-byte K chunks of a lane per 32 keys, and V chunks (32-channel blocks)
-  constexpr int RS = D + 4;    // floats of a staged row
+// Up to 32 query rows an item.  The four waves of a workgroup take an item's
+// blocks in turn and merge through LDS.  Per 32 keys a lane loads the 16-byte
+// chunks that are its MFMA operands (no LDS on the way: each code is used once)
+// and turns them into bf16, exactly; S^T = K Q^T leaves 16 keys of one query in a
+// lane, in the order in which the V chunks hold them, so P feeds the second
+// product from registers.  A block's K scale joins the softmax scale, its V scale
+// the conversion (e4m3) or P (int8).  Bound by HBM: two waves a SIMD keep two
+// tiles each in flight.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_rows_kernel(const Args8 aa) {
+  constexpr int KC = D / 32;  // 16-byte K chunks of a lane per 32 keys, and V chunks (32-channel blocks)
+  constexpr int RS = D + 4;   // floats of a staged row
   __shared__ __attribute__((aligned(16))) float stage[kWaves8 * 32 * RS];
   __shared__ float stat[2][kWaves8][32];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, g = lane >> 5;
-  int ci = 0;
-  while (ci + 1 < aa.n_calls && (int)blockIdx.x >= aa.call[ci + 1].first) ++ci;
-  const Call8 &cl = aa.call[ci];
-  int at = (int)blockIdx.x - cl.first;
-  const int split = at % cl.splits;
-  at /= cl.splits;
-  const int tile = at % cl.row_tiles, h = at / cl.row_tiles;
-  const int r0 = tile * 32 * QB;
-  const int b_begin = (int)((int64_t)cl.blocks * split / cl.splits), b_end = (int)((int64_t)cl.blocks * (split + 1) / cl.splits);
-
-  // Q operands: channel 32 j + 16 g + 8 half + e
-  bf16x8 qf[QB][2 * KC];
-#pragma unroll
-  for (int c = 0; c < QB; ++c) {
-    const int r = min(r0 + 32 * c + lr, cl.lq - 1);
-    const int64_t row = cl.q_rows ? cl.q_rows[r] : cl.q_row0 + r;
-    const uint16_t *qp = cl.q + row * cl.qts + (int64_t)h * cl.qhs + 16 * g;
-#pragma unroll
-    for (int t = 0; t < 2 * KC; ++t) {
-      i32x4 v = *(const i32x4 *)(qp + 32 * (t >> 1) + 8 * (t & 1));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] ^= aa.flip;
-      qf[c][t] = __builtin_bit_cast(bf16x8, v);
-    }
-  }
-  f32x16 acc[QB][KC];
-  float mx[QB], sum[QB];
-#pragma unroll
-  for (int c = 0; c < QB; ++c) {
-    mx[c] = -__builtin_inff();
-    sum[c] = 0.f;
+  const int x0 = range_begin(aa, blockIdx.x), end = range_begin(aa, blockIdx.x + 1);
+  for (int x = x0; x < end;) {
+    const Piece pc = piece_at(aa, x, end);
+    const Call8 &cl = aa.call[pc.call];
+    const int h = pc.head, r0 = pc.tile * 32;
+    if (x != x0) __syncthreads();  // the staging area is read out
+    bf16x8 qf[2 * KC];
+    load_q<D, true>(aa, cl, h, r0, lr, g, qf);
+    f32x16 acc[KC];
+    float mx = -__builtin_inff(), sum = 0.f;
 #pragma unroll
     for (int d = 0; d < KC; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[c][d][i] = 0.f;
-  }
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-  // The wave's tiles of 32 keys, in order: where the next one's chunks lie, the
-  // softmax factor and the V scale of its block, its valid keys.  The next
-  // tile's K and V chunks are loaded as soon as the current ones are operands.
-  int si = cl.seg0, s_first = 0, b = b_begin + w, t = 0;
-  const uint8_t *kp = nullptr, *vp = nullptr;
-  // (scale bytes as loaded: turning them into factors here would wait for every load in flight)
-  uint32_t kb = 0, vb = 0;
-  int left = 0;
-  auto locate = [&]() {  // block b of the call, tile 0
-    while (b - s_first >= (aa.seg[si].tokens + kBlock - 1) / kBlock) {
-      s_first += (aa.seg[si].tokens + kBlock - 1) / kBlock;
-      ++si;
-    }
-    const Seg8 &sg = aa.seg[si];
-    const int sb = b - s_first;
-    const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D, s_at = (int64_t)h * (sg.cap / kBlock) + sb;
-    kp = sg.k + off + lane * 16, vp = sg.v + off + lane * 16;
-    left = sg.tokens - sb * kBlock;  // 1 or more
-    kb = sg.ks[s_at], vb = sg.vs[s_at];
-    t = 0;
-  };
-  i32x4 kr[KC], vr[KC];
-  if (b < b_end) {
-    locate();
-#pragma unroll
-    for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
-#pragma unroll
-    for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
-  }
-  while (b < b_end) {
-    const int here = left;  // valid keys from the tile's first
-    const uint32_t kb_now = kb, vb_now = vb;
-    // the next tile: the block's second, or the first of the wave's next block
-    if (t == 0 && left > 32) {
-      t = 1, left -= 32, kp += 32 * D, vp += 32 * D;
-    } else {
-      b += kWaves8;
-      if (b < b_end) locate();
-    }
-    f32x16 s[QB];
-#pragma unroll
-    for (int c = 0; c < QB; ++c)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[c][i] = 0.f;
-    auto operand = [](const i32x4 &raw, int half, float scale) {
-      const i32x2 lo = decode4<E4M3>((uint32_t)raw[2 * half], scale, false);
-      const i32x2 hi = decode4<E4M3>((uint32_t)raw[2 * half + 1], scale, false);
-      return __builtin_bit_cast(bf16x8, i32x4{lo[0], lo[1], hi[0], hi[1]});
+    // The wave's tiles of 32 keys, in order: where the next one's chunks lie, the
+    // scale bytes of its block, its valid keys.  The next tile's K and V chunks are
+    // loaded as soon as the current ones are operands.
+    int si = cl.seg0, s_first = 0, b = pc.b_begin + w, t = 0;
+    const uint8_t *kp = nullptr, *vp = nullptr;
+    // (scale bytes as loaded: turning them into factors here would wait for every load in flight)
+    uint32_t kb = 0, vb = 0;
+    int left = 0;
+    auto locate = [&]() {  // block b of the call, tile 0
+      find_segment(aa, b, si, s_first);
+      const Seg8 &sg = aa.seg[si];
+      const int sb = b - s_first;
+      const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D, s_at = (int64_t)h * (sg.cap / kBlock) + sb;
+      kp = sg.k + off + lane * 16, vp = sg.v + off + lane * 16;
+      left = sg.tokens - sb * kBlock;  // 1 or more
+      kb = sg.ks[s_at], vb = sg.vs[s_at];
+      t = 0;
     };
+    i32x4 kr[KC], vr[KC];
+    if (b < pc.b_end) {
+      locate();
 #pragma unroll
-    for (int j = 0; j < 2 * KC; ++j) {
-      const bf16x8 kf = operand(kr[j >> 1], j & 1, 1.0f);
+      for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
 #pragma unroll
-      for (int c = 0; c < QB; ++c) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c][j], s[c], 0, 0, 0);
+      for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
     }
-    const float kc_now = scale_of(kb_now) * aa.scale2, vc_now = scale_of(vb_now);
-    // (after the last tile: its own chunks again)
+    while (b < pc.b_end) {
+      const int here = left;  // valid keys from the tile's first
+      const uint32_t kb_now = kb, vb_now = vb;
+      // the next tile: the block's second, or the first of the wave's next block
+      if (t == 0 && left > 32) {
+        t = 1, left -= 32, kp += 32 * D, vp += 32 * D;
+      } else {
+        b += kWaves8;
+        if (b < pc.b_end) locate();
+      }
+      f32x16 s;
 #pragma unroll
-    for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
-    bf16x8 pf[QB][2];
+      for (int i = 0; i < 16; ++i) s[i] = 0.f;
+      auto operand = [](const i32x4 &raw, int half, float scale) {
+        const i32x2 lo = decode4<E4M3>((uint32_t)raw[2 * half], scale, false);
+        const i32x2 hi = decode4<E4M3>((uint32_t)raw[2 * half + 1], scale, false);
+        return __builtin_bit_cast(bf16x8, i32x4{lo[0], lo[1], hi[0], hi[1]});
+      };
 #pragma unroll
-    for (int c = 0; c < QB; ++c) {
-      if (here < 32) {  // keys past the last: out of the maximum, weight 0 below
+      for (int j = 0; j < 2 * KC; ++j)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(kr[j >> 1], j & 1, 1.0f), qf[j], s, 0, 0, 0);
+      const float kc = scale_of(kb_now) * aa.scale2, vc = scale_of(vb_now);
+      // (after the last tile: its own chunks again)
+#pragma unroll
+      for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
+      if (here < 32) {
+        const int keys = in_branch(here);  // keys past the last: out of the maximum, weight 0 below
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (8 * (i >> 2) + 4 * g + (i & 3) >= here) s[c][i] = -3.4e38f;
+          if (8 * (i >> 2) + 4 * g + (i & 3) >= keys) s[i] = -3.4e38f;
       }
-      float top = fmaxf(s[c][0], s[c][1]);
+      float top = fmaxf(s[0], s[1]);
 #pragma unroll
-      for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[c][i]), s[c][i + 1]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * kc_now;
+      for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * kc;
       // the reference moves only where a score passes it by 8 (weights up to 2^8)
-      if (__any(top > mx[c] + 8.0f)) {
-        const float m = fmaxf(mx[c], top);
-        const float f = m == mx[c] ? 1.0f : __builtin_amdgcn_exp2f(mx[c] - m);
-        mx[c] = m;
-        sum[c] *= f;
+      if (__any(top > mx + 8.0f)) {
+        const float m = fmaxf(mx, top);
+        const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
+        mx = m;
+        sum *= f;
 #pragma unroll
         for (int d = 0; d < KC; ++d)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c][d][i] *= f;
+          for (int i = 0; i < 16; ++i) acc[d][i] *= f;
       }
       float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][i], kc_now, -mx[c]));
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kc, -mx));
       if (here < 32) {
+        const int keys = in_branch(here);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (8 * (i >> 2) + 4 * g + (i & 3) >= here) p[i] = 0.f;
+          if (8 * (i >> 2) + 4 * g + (i & 3) >= keys) p[i] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum[c] += p[i];
+      for (int i = 0; i < 16; ++i) sum += p[i];
+      bf16x8 pf[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         i32x4 pk;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           pk[e] = E4M3 ? (int)pack_bf16_rne(p[8 * m + 2 * e], p[8 * m + 2 * e + 1])
-                       : (int)pack_bf16_rne(p[8 * m + 2 * e] * vc_now, p[8 * m + 2 * e + 1] * vc_now);
-        pf[c][m] = __builtin_bit_cast(bf16x8, pk);
+                       : (int)pack_bf16_rne(p[8 * m + 2 * e] * vc, p[8 * m + 2 * e + 1] * vc);
+        pf[m] = __builtin_bit_cast(bf16x8, pk);
       }
+#pragma unroll
+      for (int d = 0; d < KC; ++d)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(vr[d], m, E4M3 ? vc : 1.0f), pf[m], acc[d], 0, 0, 0);
+      if (E4M3 && vc != vc) sum = vc;  // (the conversion's scale operand has no NaN)
+#pragma unroll
+      for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
     }
-#pragma unroll
-    for (int d = 0; d < KC; ++d)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const bf16x8 vf = operand(vr[d], m, E4M3 ? vc_now : 1.0f);
-#pragma unroll
-        for (int c = 0; c < QB; ++c) acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[c][m], acc[c][d], 0, 0, 0);
-      }
-    if (E4M3 && vc_now != vc_now)  // (the conversion's scale operand has no NaN)
-#pragma unroll
-      for (int c = 0; c < QB; ++c) sum[c] = vc_now;
-#pragma unroll
-    for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
-  }
 
-  // merge of the four waves, 32 rows at a time, in wave order
-#pragma unroll
-  for (int c = 0; c < QB; ++c) {
-    const float l = sum[c] + __shfl_xor(sum[c], 32);
-    if (c) __syncthreads();
-    if (g == 0) stat[0][w][lr] = mx[c], stat[1][w][lr] = l;
+    // merge of the four waves, in wave order
+    const float l = sum + __shfl_xor(sum, 32);
+    if (g == 0) stat[0][w][lr] = mx, stat[1][w][lr] = l;
 #pragma unroll
     for (int d = 0; d < KC; ++d)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         *(f32x4 *)&stage[(w * 32 + lr) * RS + d * 32 + 8 * u + 4 * g] =
-            f32x4{acc[c][d][4 * u], acc[c][d][4 * u + 1], acc[c][d][4 * u + 2], acc[c][d][4 * u + 3]};
+            f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
     __syncthreads();
     // thread: row tid / 8, channels 4 (tid % 8) + 32 j ..
-    const int r = threadIdx.x >> 3, dq = threadIdx.x & 7, row = r0 + 32 * c + r;
+    const int r = threadIdx.x >> 3, dq = threadIdx.x & 7, row = r0 + r;
     if (row < cl.lq) {
       float m = stat[0][0][r], f[kWaves8], ls = 0.f;
 #pragma unroll
       for (int i = 1; i < kWaves8; ++i) m = fmaxf(m, stat[0][i][r]);
 #pragma unroll
       for (int i = 0; i < kWaves8; ++i) {
-        // a wave without blocks has the maximum -inf and sums 0
+        // a wave without blocks has the reference -inf and sums 0
         f[i] = stat[0][i][r] == m ? 1.0f : __builtin_amdgcn_exp2f(stat[0][i][r] - m);
         ls += f[i] * stat[1][i][r];
       }
-      float *ws = aa.ws + (int64_t)(cl.part0 + (h * cl.row_tiles + tile) * cl.splits + split) * part_floats<D, QB>();
+      float *ws = aa.ws + (int64_t)(2 * blockIdx.x + (x != x0)) * part_floats<D, 32>();
       const float inv = 1.0f / ls;
       uint16_t *op = nullptr;
-      if (cl.splits == 1) {
+      if (pc.whole) {
         const int64_t orow = cl.o_rows ? cl.o_rows[row] : cl.o_row0 + row;
         op = cl.o + orow * cl.ots + (int64_t)h * cl.ohs;
       } else if (dq == 0) {
-        ws[QB * 32 * D + 32 * c + r] = m;
-        ws[QB * 32 * (D + 1) + 32 * c + r] = ls;
+        ws[32 * D + r] = m;
+        ws[32 * (D + 1) + r] = ls;
       }
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
@@ -514,62 +540,260 @@ kv8_attn_kernel(const Args8 aa) {
 #pragma unroll
         for (int i = 0; i < kWaves8; ++i) v += f[i] * *(const f32x4 *)&stage[(i * 32 + r) * RS + d];
         if (op)
-          *(i32x2 *)(op + d) = i32x2{(int)pack_bf16_rne(v[0] * inv, v[1] * inv), (int)pack_bf16_rne(v[2] * inv, v[3] * inv)};
+          *(i32x2 *)(op + d) = pack4(v, inv);
         else
-          *(f32x4 *)&ws[(32 * c + r) * D + d] = v;
+          *(f32x4 *)&ws[r * D + d] = v;
       }
     }
+    x += pc.b_end - pc.b_begin;
   }
 }
 
-// Merge of a call's key ranges: a workgroup per query row of a head, its 256
-// threads as 1024 / D groups of D / 4 (four channels each); a group takes every
-// (1024 / D)-th range, and the groups' sums are added through LDS in order.  The
-// ranges' maxima and sums are read once, by all threads at a time.
-constexpr int kMaxSplits = 1024;
-template <int D, int QB>
-__global__ void __launch_bounds__(256) kv8_merge_kernel(const Args8 aa) {
-  constexpr int PF = part_floats<D, QB>(), Q4 = D / 4, G = 256 / Q4;
-  __shared__ f32x4 part[G][Q4];
-  __shared__ float lsum[G], top[kMaxSplits], wmax[4];
-  int at = (int)blockIdx.x, ci = 0;
-  for (;; ++ci) {  // the grid counts the rows of the split calls
-    const int items = aa.call[ci].splits > 1 ? aa.heads * aa.call[ci].lq : 0;
-    if (at < items) break;
-    at -= items;
+// 32 RW query rows an item: RW waves of 32 rows, two waves a SIMD.  A block of 64
+// tokens is turned into bf16 once, its scales included (exact), by all threads,
+// into MFMA operand order in LDS (chunks of 16 bytes, a wave's read 1 KiB in a row);
+// then every wave multiplies its rows with it.  Two buffers: while block b is
+// multiplied, block b + 1 (in registers since the block before) is converted and
+// block b + 2 loaded; one barrier a block.  Per block and wave: 32 MFMAs of 32
+// cycles, about as many cycles of vector work (32 exponentials of 16, 32 of
+// everything else) and 32 KiB of LDS reads: the three are close to balance, and the
+// second wave of the SIMD fills the gaps.
+template <int D, int RW, bool E4M3>
+__global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_tile_kernel(const Args8 aa) {
+  constexpr int KC = D / 32, T = RW * 64, ROWS = 32 * RW;
+  constexpr int HALF = kBlock * D * 2;             // bytes of a block's K (or V) in bf16
+  constexpr int CH = kBlock * D / 8 / T;           // 16-byte chunks of codes a thread converts, of K then of V
+  constexpr int KCH = kBlock * D / 16;             // chunks of K
+  static_assert(CH >= 1 && CH * T * 8 == kBlock * D, "the threads share a block's chunks");
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * HALF];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, g = lane >> 5;
+  const int x0 = range_begin(aa, xcd_wg(aa.wgs)), end = range_begin(aa, xcd_wg(aa.wgs) + 1);
+  for (int x = x0; x < end;) {
+    const Piece pc = piece_at(aa, x, end);
+    const Call8 &cl = aa.call[pc.call];
+    const int h = pc.head, r0 = pc.tile * ROWS + 32 * w;
+    bf16x8 qf[2 * KC];
+    load_q<D, false>(aa, cl, h, r0, lr, g, qf);
+    f32x16 acc[KC];
+    float mx = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+    for (int d = 0; d < KC; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+
+    // the block that is loaded next, its segment, and the valid keys of the
+    // blocks that are loaded and converted
+    int lb = pc.b_begin, si = cl.seg0, s_first = 0;
+    i32x4 raw[CH];
+    uint32_t kb = 0, vb = 0;
+    int raw_left = 0;
+    auto load = [&]() {  // block lb (the last one again behind it)
+      find_segment(aa, lb, si, s_first);
+      const Seg8 &sg = aa.seg[si];
+      const int sb = lb - s_first;
+      const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D, s_at = (int64_t)h * (sg.cap / kBlock) + sb;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int c = i * T + tid;
+        raw[i] = *(const i32x4 *)((c < KCH ? sg.k + off : sg.v + off - KCH * 16) + c * 16);
+      }
+      kb = sg.ks[s_at], vb = sg.vs[s_at];
+      raw_left = sg.tokens - sb * kBlock;
+      if (lb + 1 < pc.b_end) ++lb;
+    };
+    // K chunk (tile, 16 channels, key): two chunks of 8 channels, 512 bytes apart; V
+    // chunk (tile, 32 channels, key group, channel): two of 8 keys, 1 KiB apart
+    auto convert = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int c = i * T + tid;
+        const bool is_v = c >= KCH;
+        const uint32_t byte = is_v ? vb : kb;
+        const float f = scale_of(byte);
+        const bool nan = byte == 255u;
+        i32x4 o[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const i32x2 lo = decode4<E4M3>((uint32_t)raw[i][2 * m], f, nan), hi = decode4<E4M3>((uint32_t)raw[i][2 * m + 1], f, nan);
+          o[m] = i32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+        const int cc = is_v ? c - KCH : c;
+        // K: [tile][D / 8][32 keys]; V: [tile][D / 32][2][2 groups][32 channels]
+        const int at = is_v ? HALF + (cc >> 6) * 2048 + (cc & 63) * 16 : (cc >> 5) * 1024 + (cc & 31) * 16;
+        char *to = smem + buf * 2 * HALF + at;
+        *(i32x4 *)to = o[0];
+        *(i32x4 *)(to + (is_v ? 1024 : 512)) = o[1];
+      }
+    };
+    if (x != x0) __syncthreads();  // the last piece's buffers are read out
+    load();
+    int left = raw_left;  // valid keys from block b's first on
+    convert(0);
+    load();
+    const int blocks = pc.b_end - pc.b_begin;
+    for (int b = 0; b < blocks; ++b) {
+      const int buf = b & 1, next_left = raw_left;
+      __syncthreads();
+      // operands half a block ahead of their MFMAs: K's first half behind the
+      // barrier, V's behind the scores, so that it lands under the softmax
+      const char *kt = smem + buf * 2 * HALF + lane * 16, *vt = kt + HALF;
+      bf16x8 op[2 * KC];
+      auto k_op = [&](int i) { return *(const bf16x8 *)(kt + (i & 1) * (HALF / 2) + (i >> 1) * 1024); };
+      auto v_op = [&](int i) { return *(const bf16x8 *)(vt + i / (2 * KC) * (HALF / 2) + i / KC % 2 * 1024 + i % KC * 2048); };
+#pragma unroll
+      for (int i = 0; i < 2 * KC; ++i) op[i] = k_op(i);
+      __builtin_amdgcn_sched_barrier(0);
+      const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      f32x16 s[2];
+#pragma unroll
+      for (int i = 0; i < 4 * KC; ++i) {
+        s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % (2 * KC)], qf[i >> 1], i < 2 ? zero : s[i & 1], 0, 0, 0);
+        op[i % (2 * KC)] = i < 2 * KC ? k_op(i + 2 * KC) : v_op(i - 2 * KC);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (left < kBlock) {
+        const int keys = in_branch(left);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * t + 8 * (i >> 2) + 4 * g + (i & 3) >= keys) s[t][i] = -3.4e38f;
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * aa.scale2;
+      // the reference moves only where a score passes it by 8 (weights up to 2^8)
+      if (__any(top > mx + 8.0f)) {
+        const float m = fmaxf(mx, top);
+        const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
+        mx = m;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < KC; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+      }
+      bf16x8 pf[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], aa.scale2, -mx));
+        if (left < kBlock) {
+        const int keys = in_branch(left);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * t + 8 * (i >> 2) + 4 * g + (i & 3) >= keys) p[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += p[i];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          i32x4 pk;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pk[e] = (int)pack_bf16_rne(p[8 * m + 2 * e], p[8 * m + 2 * e + 1]);
+          pf[t][m] = __builtin_bit_cast(bf16x8, pk);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * KC; ++i) {
+        acc[i % KC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % (2 * KC)], pf[i / (2 * KC)][i / KC % 2], acc[i % KC], 0, 0, 0);
+        if (i < 2 * KC) op[i % (2 * KC)] = v_op(i + 2 * KC);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // (the last MFMAs run meanwhile, and the scores' registers are free)
+      if (b + 1 < blocks) {
+        convert(buf ^ 1);
+        load();
+      }
+      left = next_left;
+    }
+
+    const float l = sum + __shfl_xor(sum, 32);
+    const int row = r0 + lr;
+    if (row < cl.lq) {
+      if (pc.whole) {
+        const int64_t orow = cl.o_rows ? cl.o_rows[row] : cl.o_row0 + row;
+        uint16_t *op = cl.o + orow * cl.ots + (int64_t)h * cl.ohs + 4 * g;
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < KC; ++d)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *(i32x2 *)(op + 32 * d + 8 * u) = pack4(f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]}, inv);
+      } else {
+        const int r = 32 * w + lr;
+        float *ws = aa.ws + (int64_t)(2 * xcd_wg(aa.wgs) + (x != x0)) * part_floats<D, ROWS>();
+        if (g == 0) ws[ROWS * D + r] = mx, ws[ROWS * (D + 1) + r] = l;
+#pragma unroll
+        for (int d = 0; d < KC; ++d)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *(f32x4 *)&ws[r * D + 32 * d + 8 * u + 4 * g] =
+                f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
+      }
+    }
+    x += blocks;
   }
+}
+
+// Merge of the cut items, RPW rows of an item a workgroup: 256 threads as RPW x PG x
+// D / 4, where PG threads share a row's parts and add through LDS, in order.
+template <int D, int ROWS, int RPW>
+__global__ void __launch_bounds__(256) kv8_merge_kernel(const Args8 aa, int32_t groups_of_rows) {
+  constexpr int PF = part_floats<D, ROWS>(), Q4 = D / 4, PG = 256 / Q4 / RPW;
+  static_assert(PG * Q4 * RPW == 256, "the threads share the rows");
+  __shared__ f32x4 part[RPW][PG][Q4];
+  __shared__ float lsum[RPW][PG], rtop[RPW][PG];
+  int item = (int)blockIdx.x / groups_of_rows, rg = (int)blockIdx.x % groups_of_rows, ci = 0;
+  while (item >= aa.heads * aa.call[ci].row_tiles) item -= aa.heads * aa.call[ci++].row_tiles;
   const Call8 &cl = aa.call[ci];
-  const int h = at / cl.lq, row = at - h * cl.lq, tile = row / (32 * QB), r = row % (32 * QB);
-  const float *ws = aa.ws + (int64_t)(cl.part0 + (h * cl.row_tiles + tile) * cl.splits) * PF;
-  const int d4 = threadIdx.x % Q4, grp = threadIdx.x / Q4;
+  const int head = item / cl.row_tiles, tile = item - head * cl.row_tiles;
+  if (tile * ROWS + rg * RPW >= cl.lq) return;
+  const int begin = cl.first + item * cl.blocks, end = begin + cl.blocks;  // the item's units
+  // parts: from the range that holds its first unit to that of its last
+  int first_wg = (int)((int64_t)begin * aa.wgs / aa.units);
+  while (range_begin(aa, first_wg + 1) <= begin) ++first_wg;
+  while (range_begin(aa, first_wg) > begin) --first_wg;
+  if (range_begin(aa, first_wg + 1) >= end) return;  // whole
+  int last_wg = first_wg + 1;
+  while (range_begin(aa, last_wg + 1) < end) ++last_wg;
+  const int late = range_begin(aa, first_wg) < begin;  // not the first piece of that range
+  auto slot = [&](int wg) { return aa.ws + (int64_t)(2 * wg + (wg == first_wg ? late : 0)) * PF; };
+  const int d4 = threadIdx.x % Q4, pg = threadIdx.x / Q4 % PG, rr = threadIdx.x / Q4 / PG;
+  const int r = rg * RPW + rr, row = tile * ROWS + r;
   float m = -__builtin_inff();
-  for (int s = threadIdx.x; s < cl.splits; s += 256) m = fmaxf(m, top[s] = ws[(int64_t)s * PF + QB * 32 * D + r]);
-  m = wave_max(m);
-  if (threadIdx.x % 64 == 0) wmax[threadIdx.x / 64] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+  for (int wg = first_wg + pg; wg <= last_wg; wg += PG) m = fmaxf(m, slot(wg)[ROWS * D + r]);
+  if (PG > 1) {
+    if (d4 == 0) rtop[rr][pg] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PG; ++i) m = fmaxf(m, rtop[rr][i]);
+  }
   float l = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = grp; s < cl.splits; s += G) {
-    const float *p = ws + (int64_t)s * PF;
-    const float f = top[s] == m ? 1.0f : __builtin_amdgcn_exp2f(top[s] - m);
-    l += f * p[QB * 32 * (D + 1) + r];
+  for (int wg = first_wg + pg; wg <= last_wg; wg += PG) {
+    const float *p = slot(wg);
+    const float top = p[ROWS * D + r], f = top == m ? 1.0f : __builtin_amdgcn_exp2f(top - m);
+    l += f * p[ROWS * (D + 1) + r];
     v += f * *(const f32x4 *)&p[r * D + 4 * d4];
   }
-  part[grp][d4] = v;
-  if (d4 == 0) lsum[grp] = l;
-  __syncthreads();
-  if (grp) return;
+  if (PG > 1) {
+    part[rr][pg][d4] = v;
+    if (d4 == 0) lsum[rr][pg] = l;
+    __syncthreads();
+    if (pg) return;
 #pragma unroll
-  for (int i = 1; i < G; ++i) {
-    v += part[i][d4];
-    l += lsum[i];
+    for (int i = 1; i < PG; ++i) {
+      v += part[rr][i][d4];
+      l += lsum[rr][i];
+    }
   }
+  if (row >= cl.lq) return;
   const int64_t orow = cl.o_rows ? cl.o_rows[row] : cl.o_row0 + row;
-  const float inv = 1.0f / l;
-  *(i32x2 *)(cl.o + orow * cl.ots + (int64_t)h * cl.ohs + 4 * d4) =
-      i32x2{(int)pack_bf16_rne(v[0] * inv, v[1] * inv), (int)pack_bf16_rne(v[2] * inv, v[3] * inv)};
+  *(i32x2 *)(cl.o + orow * cl.ots + (int64_t)head * cl.ohs + 4 * d4) = pack4(v, 1.0f / l);
 }
 
 // ---- host side
@@ -610,47 +834,39 @@ void dispatch(int D, int format, F &&f) {
     format == TMHD_KV8_E4M3 ? f(integral_constant<int, 64>{}, std::true_type{}) : f(integral_constant<int, 64>{}, std::false_type{});
 }
 
-// How many query rows a workgroup takes (32 QB), and the key ranges of each call.
-struct Plan8 {
-  int qb;
-  int64_t wgs, parts, merge_items;
-};
-
 int blocks_of(const tmhd_kv8_call &c) {
   int64_t b = 0;
   for (int i = 0; i < c.n_segments; ++i) b += (c.seg[i].tokens + kBlock - 1) / kBlock;
   return (int)std::min<int64_t>(b, INT32_MAX);
 }
 
-// The calls [0, n) of one launch.  The blocks of all items are dealt to about
-// two workgroups per CU (one with 64 rows), at least two blocks a wave.
+// Rows of an item, the units of work (item, block) and the workgroups they are dealt to.
+struct Plan8 {
+  int rows;
+  int64_t items, units;
+  int wgs;
+  int most;  // query rows of the longest call
+};
+
+// The calls of one launch.  Up to 32 rows: items of 32, two workgroups a CU; else
+// of 128 (two a CU) or, beyond 128 rows, of 256.  A workgroup takes at least 8 blocks
+// (two for each wave that loads blocks of its own) or 4.
 Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
-  Plan8 p{1, 0, 0, 0};
-  int32_t most = 0;
-  for (int i = 0; i < n; ++i) most = std::max(most, calls[i].lq);
-  p.qb = most > 32 ? 2 : 1;
-  int64_t total = 0;
-  for (int i = 0; i < n; ++i)
-    total += (int64_t)heads * ((calls[i].lq + 32 * p.qb - 1) / (32 * p.qb)) * blocks_of(calls[i]);
-  const int64_t room = (int64_t)std::max(device_cus(), 1) * (p.qb == 1 ? 2 : 1);
-  int64_t each = std::max<int64_t>(2 * kWaves8, (total + room - 1) / room);
-  for (int i = 0; i < n; ++i) each = std::max<int64_t>(each, (blocks_of(calls[i]) + kMaxSplits - 1) / kMaxSplits);
+  Plan8 p{32, 0, 0, 0, 0};
+  for (int i = 0; i < n; ++i) p.most = std::max(p.most, calls[i].lq);
+  p.rows = p.most <= 32 ? 32 : p.most <= 128 ? 128 : 256;
   for (int i = 0; i < n; ++i) {
     Call8 c{};
     c.lq = calls[i].lq;
     c.blocks = blocks_of(calls[i]);
-    c.row_tiles = (int32_t)(((int64_t)c.lq + 32 * p.qb - 1) / (32 * p.qb));
-    c.splits = c.lq > 0 ? (int32_t)((c.blocks + each - 1) / each) : 1;
-    c.first = (int32_t)std::min<int64_t>(p.wgs, INT32_MAX);
-    c.part0 = (int32_t)std::min<int64_t>(p.parts, INT32_MAX);
-    const int64_t items = (int64_t)heads * c.row_tiles;
-    p.wgs += items * c.splits;
-    if (c.splits > 1) {
-      p.parts += items * c.splits;
-      p.merge_items += (int64_t)heads * c.lq;
-    }
+    c.row_tiles = (int32_t)(((int64_t)c.lq + p.rows - 1) / p.rows);
+    c.first = (int32_t)std::min<int64_t>(p.units, INT32_MAX);
+    p.items += (int64_t)heads * c.row_tiles;
+    p.units += (int64_t)heads * c.row_tiles * c.blocks;
     if (out) out[i] = c;
   }
+  const int64_t room = (int64_t)std::max(device_cus(), 8) * (p.rows == 256 ? 1 : 2), least = p.rows == 32 ? 2 * kWaves8 : 4;
+  p.wgs = (int)std::min<int64_t>(room, (p.units + least - 1) / least);
   return p;
 }
 
@@ -682,20 +898,35 @@ int check_calls(const char *what, const tmhd_kv8_call *calls, int n) {
   return TMHD_OK;
 }
 
-template <int D, bool E4M3>
-void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
-  if (p.qb == 1)
-    hipLaunchKernelGGL((kv8_attn_kernel<D, 1, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
+template <int D, int ROWS>
+void launch_merge(const Args8 &aa, const Plan8 &p, hipStream_t s) {
+  if (p.wgs <= 1) return;
+  const int rows = std::min(p.most, ROWS);
+  // items of many parts: a row to a workgroup, its parts shared by 1024 / D threads; else 1024 / D rows
+  constexpr int RPW = 1024 / D;
+  const int groups = p.wgs > 4 * p.items ? rows : (rows + RPW - 1) / RPW;
+  if (p.wgs > 4 * p.items)
+    hipLaunchKernelGGL((kv8_merge_kernel<D, ROWS, 1>), dim3((unsigned)(p.items * groups)), dim3(256), 0, s, aa, groups);
   else
-    hipLaunchKernelGGL((kv8_attn_kernel<D, 2, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
-  if (p.merge_items == 0) return;
-  if (p.qb == 1)
-    hipLaunchKernelGGL((kv8_merge_kernel<D, 1>), dim3((unsigned)p.merge_items), dim3(256), 0, s, aa);
-  else
-    hipLaunchKernelGGL((kv8_merge_kernel<D, 2>), dim3((unsigned)p.merge_items), dim3(256), 0, s, aa);
+    hipLaunchKernelGGL((kv8_merge_kernel<D, ROWS, RPW>), dim3((unsigned)(p.items * groups)), dim3(256), 0, s, aa, groups);
 }
 
-int64_t parts_bytes(const Plan8 &p, int D) { return p.parts * (32 * p.qb) * (D + 2) * 4; }
+template <int D, bool E4M3>
+void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
+  if (p.rows == 32) {
+    hipLaunchKernelGGL((kv8_rows_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
+    launch_merge<D, 32>(aa, p, s);
+  } else if (p.rows == 128) {
+    hipLaunchKernelGGL((kv8_tile_kernel<D, 4, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
+    launch_merge<D, 128>(aa, p, s);
+  } else {
+    hipLaunchKernelGGL((kv8_tile_kernel<D, 8, E4M3>), dim3((unsigned)p.wgs), dim3(512), 0, s, aa);
+    launch_merge<D, 256>(aa, p, s);
+  }
+}
+
+// two slots for each workgroup (none if one takes all)
+int64_t parts_bytes(const Plan8 &p, int D) { return p.wgs > 1 ? (int64_t)p.wgs * 2 * p.rows * (D + 2) * 4 : 0; }
 
 }  // namespace
 }  // namespace tmhd
@@ -822,12 +1053,13 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
     const int e = group_end(calls, n, i);
     Args8 aa{};
     const Plan8 p = plan(calls + i, e - i, heads, aa.call);
-    if (p.wgs > INT32_MAX || p.parts > INT32_MAX || p.merge_items > INT32_MAX) return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows", what);
+    if (p.units > INT32_MAX || p.items * p.rows > INT32_MAX) return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows and keys", what);
     if (parts_bytes(p, head_dim) > (workspace ? workspace_bytes : 0))
       return set_error(TMHD_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,
                        (long long)parts_bytes(p, head_dim));
     aa.n_calls = e - i;
     aa.heads = heads;
+    aa.units = (int32_t)p.units, aa.wgs = p.wgs;
     aa.scale2 = fabsf(scale) * 1.4426950408889634f;
     aa.flip = scale < 0.f ? (int32_t)0x80008000u : 0;
     aa.ws = (float *)workspace;
@@ -838,7 +1070,7 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
       o.q = (const uint16_t *)in.q, o.o = (uint16_t *)in.o;
       o.qts = in.q_token_stride, o.qhs = in.q_head_stride, o.ots = in.o_token_stride, o.ohs = in.o_head_stride;
       o.q_rows = in.q_rows, o.o_rows = in.o_rows, o.q_row0 = in.q_row0, o.o_row0 = in.o_row0;
-      o.seg0 = segs, o.nseg = in.n_segments;
+      o.seg0 = segs;
       for (int j = 0; j < in.n_segments; ++j) {
         const View vw = view_of(in.seg[j], head_dim);
         aa.seg[segs++] = Seg8{vw.k, vw.v, vw.ks, vw.vs, vw.cap, vw.tokens};

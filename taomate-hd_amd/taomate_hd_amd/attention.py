@@ -25,7 +25,7 @@ from .profiling import ComponentTimer, maybe_region
 from .slots import KV_TILE, KVSlot, KVSlot8, SlotView, expand_views, round_up, vt_columns
 
 BACKENDS = ("bf16", "i8qk")
-KV8_ROWS = 64  # query rows up to which 8-bit segments are read in place
+KV8_ROWS = 1 << 30  # query rows up to which 8-bit segments are read in place
 
 
 class QKQuantWorkspace:

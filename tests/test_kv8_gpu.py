@@ -160,12 +160,14 @@ def _want(q, segments, scale):
 
 
 CASES = [(1, 1, 64, [1]), (1, 3, 128, [33]), (5, 2, 64, [64, 1, 130]), (32, 4, 128, [500]), (33, 2, 128, [65]),
-         (64, 3, 64, [1000, 70]), (1, 14, 128, [9000, 777, 64]), (17, 1, 128, [20000])]
+         (64, 3, 64, [1000, 70]), (1, 14, 128, [9000, 777, 64]), (17, 1, 128, [20000]), (40, 1, 128, [30]),
+         (100, 5, 128, [64, 700, 33]), (128, 2, 64, [2000]), (129, 3, 128, [1]), (300, 2, 64, [65, 128]),
+         (256, 9, 128, [500, 640]), (700, 1, 128, [5000, 64])]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rows,heads,dim,sizes", CASES)
-def test_attention_of_few_rows(torch_mod, dev, rows, heads, dim, sizes, fmt):
+def test_attention_over_codes(torch_mod, dev, rows, heads, dim, sizes, fmt):
     from taomate_hd_amd import segment_attention
 
     torch = torch_mod
@@ -181,9 +183,9 @@ def test_attention_of_few_rows(torch_mod, dev, rows, heads, dim, sizes, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_many_rows_equal_attention_over_the_expanded_slot(torch_mod, dev, fmt):
-    """Beyond the rows read in place, and with the INT8-QK backend, a call gives the bits of the same call over a
-    bf16 slot packed with the 8-bit slot's values."""
+def test_expanded_calls_equal_calls_over_bf16_slots(torch_mod, dev, fmt):
+    """With bf16 segments beside the 8-bit ones, and with the INT8-QK backend, a call gives the bits of the same call
+    over a bf16 slot packed with the 8-bit slot's values."""
     from taomate_hd_amd import segment_attention
     from taomate_hd_amd.slots import KVSlot
 
@@ -192,10 +194,12 @@ def test_many_rows_equal_attention_over_the_expanded_slot(torch_mod, dev, fmt):
     slot = _slot(torch, k, v, fmt, dev)
     plain = KVSlot(torch, heads=4, head_dim=128, capacity=700, device=dev)
     plain.pack(*slot.token_major())
+    beside = KVSlot(torch, heads=4, head_dim=128, capacity=90, device=dev)
+    beside.pack(*_kv(torch, 90, 4, 128, 3, dev))
     q = _kv(torch, 300, 4, 128, 2, dev)[0]
-    for backend, rows in (("bf16", 300), ("i8qk", 300), ("i8qk", 3)):
-        a = segment_attention(torch, q[:rows], [slot.view()], scale=0.1, backend=backend)
-        b = segment_attention(torch, q[:rows], [plain.view()], scale=0.1, backend=backend)
+    for backend, rows, more in (("bf16", 300, [beside.view()]), ("bf16", 2, [beside.view()]), ("i8qk", 300, []), ("i8qk", 3, [])):
+        a = segment_attention(torch, q[:rows], [slot.view(), *more], scale=0.1, backend=backend)
+        b = segment_attention(torch, q[:rows], [plain.view(), *more], scale=0.1, backend=backend)
         assert torch.equal(a, b)
 
 
