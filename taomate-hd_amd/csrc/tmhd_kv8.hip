@@ -450,10 +450,10 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
 #pragma unroll
       for (int j = 0; j < KC; ++j) kr[j] = *(const i32x4 *)(kp + j * 1024);
       if (here < 32) {
-        const int keys = in_branch(here);  // keys past the last: out of the maximum, weight 0 below
+        const int keys = in_branch(here) - 4 * g;  // keys past the last: out of the maximum, weight 0 below
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (8 * (i >> 2) + 4 * g + (i & 3) >= keys) s[i] = -3.4e38f;
+          if (8 * (i >> 2) + (i & 3) >= keys) s[i] = -3.4e38f;
       }
       float top = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -474,10 +474,10 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kc, -mx));
       if (here < 32) {
-        const int keys = in_branch(here);
+        const int keys = in_branch(here) - 4 * g;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (8 * (i >> 2) + 4 * g + (i & 3) >= keys) p[i] = 0.f;
+          if (8 * (i >> 2) + (i & 3) >= keys) p[i] = 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum += p[i];
@@ -608,6 +608,7 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
       for (int i = 0; i < CH; ++i) {
         const int c = i * T + tid;
         const bool is_v = c >= KCH;
+        asm volatile("" : "+v"(raw[i]));  // (converted here, not where it was loaded: four times the registers)
         const uint32_t byte = is_v ? vb : kb;
         const float f = scale_of(byte);
         const bool nan = byte == 255u;
@@ -623,6 +624,7 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
         char *to = smem + buf * 2 * HALF + at;
         *(i32x4 *)to = o[0];
         *(i32x4 *)(to + (is_v ? 1024 : 512)) = o[1];
+        __builtin_amdgcn_sched_barrier(0);  // (a chunk's registers at a time)
       }
     };
     if (x != x0) __syncthreads();  // the last piece's buffers are read out
@@ -652,12 +654,12 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
         __builtin_amdgcn_sched_barrier(0);
       }
       if (left < kBlock) {
-        const int keys = in_branch(left);
+        const int keys = in_branch(left) - 4 * g;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (32 * t + 8 * (i >> 2) + 4 * g + (i & 3) >= keys) s[t][i] = -3.4e38f;
+            if (32 * t + 8 * (i >> 2) + (i & 3) >= keys) s[t][i] = -3.4e38f;
       }
       float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -681,10 +683,10 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], aa.scale2, -mx));
         if (left < kBlock) {
-        const int keys = in_branch(left);
+        const int keys = in_branch(left) - 4 * g;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (32 * t + 8 * (i >> 2) + 4 * g + (i & 3) >= keys) p[i] = 0.f;
+            if (32 * t + 8 * (i >> 2) + (i & 3) >= keys) p[i] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += p[i];
