@@ -8,10 +8,11 @@ does over the concatenated K/V in the reference
 the SageAttention-style variant (smooth-K, per-128-block INT8 Q/K, bf16 P.V;
 ref attention_hook.py:335-371, inference/sage_value_padding.py:79-97).
 
-Segments may lie in slots held in 8 bits (``KVSlot8``).  A ``"bf16"`` call of
-up to ``KV8_ROWS`` query rows whose segments all do, in one format, reads their
-codes in place (``tmhd_attn_fwd_kv8``); for any other call they are expanded
-to bf16 first, which is exact, and the call runs as over bf16 slots.
+Segments may lie in slots held in 8 bits (``KVSlot8``).  A ``"bf16"`` call
+whose segments all do, in one format, reads their codes in place
+(``tmhd_attn_fwd_kv8``) where it has up to ``KV8_ROWS`` query rows or the batch
+is small; for any other call they are expanded to bf16 first, which is exact,
+and the call runs as over bf16 slots.
 """
 
 from __future__ import annotations
@@ -25,7 +26,17 @@ from .profiling import ComponentTimer, maybe_region
 from .slots import KV_TILE, KVSlot, KVSlot8, SlotView, expand_views, round_up, vt_columns
 
 BACKENDS = ("bf16", "i8qk")
-KV8_ROWS = 1 << 30  # query rows up to which 8-bit segments are read in place
+# 8-bit segments are read in place by calls of up to KV8_ROWS query rows, and by
+# batches of up to KV8_WORK (query row, token, channel) products.  The kernel that
+# reads codes turns every block into bf16 for 256 rows at a time and multiplies at
+# 0.85 PFLOPS; expanding costs a pass over the cache and a launch, the bf16 kernel
+# then runs at up to 1.35.  Measured, e4m3, in place / expanded, us: 14 heads of 128
+# over 41,000 tokens 109/190 at 256 rows, 182/230 at 512, 331/347 at 1,024, 450/453 at
+# 1,536, 735/696 at 2,560; 11,000 tokens 59/68, 80/75, 128/104; 2,800 tokens (2.6e9
+# products) 54/49 at 512; 700 tokens (1.3e9) 38/50 at 1,024 and 50/47 at 2,560; 4 heads
+# of 64 over 41,000 tokens 58/73 at 512, 89/76 at 1,024.  int8 is 2 to 5% slower in place.
+KV8_ROWS = 512
+KV8_WORK = 3 << 29
 
 
 class QKQuantWorkspace:
@@ -227,7 +238,7 @@ def segment_attention(
     rows_checked: bool = False,
 ) -> Any:
     """Attention of the selected query rows over ``segments`` (no mask; bf16 slots are
-    read in place, 8-bit ones too by a ``"bf16"`` call of few query rows).
+    read in place, 8-bit ones by the rule at ``KV8_ROWS``).
 
     Query row ``i`` is ``query[q_rows[i]]`` (or ``query[q_row0 + i]``); its
     output goes to ``out[o_rows[i]]`` (or ``out[o_row0 + i]``).  Without
@@ -330,22 +341,32 @@ def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: l
 
 
 def _in_place_format(call: AttentionCall) -> str | None:
-    """The format of the 8-bit segments that a ``"bf16"`` call reads in place, if it does."""
+    """The format of the call's segments, if all are 8-bit ones of one format and no more than one launch takes."""
     fmt, count = None, 0
     for s in call.segments:
         if s.tokens > 0:
             if not isinstance(s.slot, KVSlot8) or fmt not in (None, s.slot.format):
                 return None
             fmt, count = s.slot.format, count + 1
+    return fmt if count <= _native.MAX_SEGMENTS else None
+
+
+def _call_rows(call: AttentionCall) -> int:
+    """A call's query rows (its arguments are checked later)."""
     if call.q_rows is not None:
-        rows = call.q_rows.numel() if hasattr(call.q_rows, "numel") else KV8_ROWS + 1  # (refused later)
-    else:
-        rows = call.query.shape[0] - call.q_row0 if call.lq is None else call.lq
-    return fmt if rows <= KV8_ROWS and count <= _native.MAX_SEGMENTS else None
+        return int(call.q_rows.numel()) if hasattr(call.q_rows, "numel") else 0
+    return int(call.query.shape[0] - call.q_row0 if call.lq is None else call.lq)
+
+
+def _in_place_formats(calls: Sequence[AttentionCall]) -> list[str | None]:
+    """For each ``"bf16"`` call the format of the segments that it reads in place, None where they are expanded."""
+    rows = [_call_rows(call) for call in calls]
+    work = sum(n * sum(s.tokens * s.slot.heads * s.slot.head_dim for s in call.segments) for n, call in zip(rows, calls))
+    return [_in_place_format(call) if n <= KV8_ROWS or work <= KV8_WORK else None for n, call in zip(rows, calls)]
 
 
 def _attend_in_place(torch: Any, calls: Sequence[AttentionCall], scale: float, timer: ComponentTimer | None) -> list[Any]:
-    """Calls of few query rows over 8-bit segments of one format, in one launch (per 16 calls and 24 segments)."""
+    """Calls over 8-bit segments of one format, in one launch (per 16 calls and 24 segments)."""
     keep: list[Any] = []
     n = len(calls)
     args = (_native.KV8Call * n)()
@@ -370,7 +391,7 @@ def _attend_in_place(torch: Any, calls: Sequence[AttentionCall], scale: float, t
 def _attend_8bit(torch: Any, calls: list[AttentionCall], **options: Any) -> tuple[list[Any], list[dict[str, Any]]]:
     """``segment_attention_batch`` of calls some of whose segments are held in 8 bits."""
     scale, timer = float(options["scale"]), options["timer"]
-    formats = [_in_place_format(call) if options["backend"] == "bf16" else None for call in calls]
+    formats = _in_place_formats(calls) if options["backend"] == "bf16" else [None] * len(calls)
     kinds = set(formats)
     if len(kinds) == 1 and None not in kinds:
         return _attend_in_place(torch, calls, scale, timer), []

@@ -183,6 +183,27 @@ def test_attention_over_codes(torch_mod, dev, rows, heads, dim, sizes, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_calls_on_both_sides_of_the_in_place_rule(torch_mod, dev, fmt):
+    """One row more and the slot is expanded: the call is one over a bf16 slot, bit for bit."""
+    from taomate_hd_amd import KVSlot, attention, segment_attention
+
+    torch = torch_mod
+    heads, dim, tokens, most = 6, 128, 4264, attention.KV8_ROWS
+    assert (most + 1) * tokens * heads * dim > attention.KV8_WORK
+    k, v = _kv(torch, tokens, heads, dim, 8, dev)
+    slot = _slot(torch, k, v, fmt, dev)
+    plain = KVSlot(torch, heads=heads, head_dim=dim, capacity=tokens, device=dev)
+    plain.pack(*slot.token_major())
+    q = _kv(torch, most + 1, heads, dim, 9, dev)[0]
+    in_place = segment_attention(torch, q[:most], [slot.view()], scale=dim ** -0.5)
+    want, bound = _want(q[:most], [slot.view()], dim ** -0.5)
+    assert (np.abs(_f64(in_place) - want) <= bound).all()
+    expanded = segment_attention(torch, q, [slot.view()], scale=dim ** -0.5)
+    assert torch.equal(expanded, segment_attention(torch, q, [plain.view()], scale=dim ** -0.5))
+    assert not torch.equal(expanded[:most], in_place)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_expanded_calls_equal_calls_over_bf16_slots(torch_mod, dev, fmt):
     """With bf16 segments beside the 8-bit ones, and with the INT8-QK backend, a call gives the bits of the same call
     over a bf16 slot packed with the 8-bit slot's values."""
