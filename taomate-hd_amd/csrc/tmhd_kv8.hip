@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
     const Piece pc = piece_at(aa, x, end);
     const Call8 &cl = aa.call[pc.call];
     const int h = pc.head, r0 = pc.tile * ROWS + 32 * w;
+    const bool live = r0 < cl.lq;  // a wave without rows only converts
     bf16x8 qf[2 * KC];
     load_q<D, false>(aa, cl, h, r0, lr, g, qf);
     f32x16 acc[KC];
@@ -641,73 +642,75 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
     for (int b = 0; b < blocks; ++b) {
       const int buf = b & 1, next_left = raw_left;
       __syncthreads();
-      // operands half a block ahead of their MFMAs: K's first half behind the
-      // barrier, V's behind the scores, so that it lands under the softmax
-      const char *kt = smem + buf * 2 * HALF + lane * 16, *vt = kt + HALF;
-      bf16x8 op[2 * KC];
-      auto k_op = [&](int i) { return *(const bf16x8 *)(kt + (i & 1) * (HALF / 2) + (i >> 1) * 1024); };
-      auto v_op = [&](int i) { return *(const bf16x8 *)(vt + i / (2 * KC) * (HALF / 2) + i / KC % 2 * 1024 + i % KC * 2048); };
+      if (live) {
+        // operands half a block ahead of their MFMAs: K's first half behind the
+        // barrier, V's behind the scores, so that it lands under the softmax
+        const char *kt = smem + buf * 2 * HALF + lane * 16, *vt = kt + HALF;
+        bf16x8 op[2 * KC];
+        auto k_op = [&](int i) { return *(const bf16x8 *)(kt + (i & 1) * (HALF / 2) + (i >> 1) * 1024); };
+        auto v_op = [&](int i) { return *(const bf16x8 *)(vt + i / (2 * KC) * (HALF / 2) + i / KC % 2 * 1024 + i % KC * 2048); };
 #pragma unroll
-      for (int i = 0; i < 2 * KC; ++i) op[i] = k_op(i);
-      __builtin_amdgcn_sched_barrier(0);
-      const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      f32x16 s[2];
-#pragma unroll
-      for (int i = 0; i < 4 * KC; ++i) {
-        s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % (2 * KC)], qf[i >> 1], i < 2 ? zero : s[i & 1], 0, 0, 0);
-        op[i % (2 * KC)] = i < 2 * KC ? k_op(i + 2 * KC) : v_op(i - 2 * KC);
+        for (int i = 0; i < 2 * KC; ++i) op[i] = k_op(i);
         __builtin_amdgcn_sched_barrier(0);
-      }
-      if (left < kBlock) {
-        const int keys = in_branch(left) - 4 * g;
+        const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        f32x16 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * t + 8 * (i >> 2) + (i & 3) >= keys) s[t][i] = -3.4e38f;
-      }
-      float top = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * aa.scale2;
-      // the reference moves only where a score passes it by 8 (weights up to 2^8)
-      if (__any(top > mx + 8.0f)) {
-        const float m = fmaxf(mx, top);
-        const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
-        mx = m;
-        sum *= f;
-#pragma unroll
-        for (int d = 0; d < KC; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[d][i] *= f;
-      }
-      bf16x8 pf[2][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float p[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], aa.scale2, -mx));
+        for (int i = 0; i < 4 * KC; ++i) {
+          s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % (2 * KC)], qf[i >> 1], i < 2 ? zero : s[i & 1], 0, 0, 0);
+          op[i % (2 * KC)] = i < 2 * KC ? k_op(i + 2 * KC) : v_op(i - 2 * KC);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         if (left < kBlock) {
-        const int keys = in_branch(left) - 4 * g;
+          const int keys = in_branch(left) - 4 * g;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * t + 8 * (i >> 2) + (i & 3) >= keys) p[i] = 0.f;
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (32 * t + 8 * (i >> 2) + (i & 3) >= keys) s[t][i] = -3.4e38f;
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * aa.scale2;
+        // the reference moves only where a score passes it by 8 (weights up to 2^8)
+        if (__any(top > mx + 8.0f)) {
+          const float m = fmaxf(mx, top);
+          const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
+          mx = m;
+          sum *= f;
+#pragma unroll
+          for (int d = 0; d < KC; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+        }
+        bf16x8 pf[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], aa.scale2, -mx));
+          if (left < kBlock) {
+            const int keys = in_branch(left) - 4 * g;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (32 * t + 8 * (i >> 2) + (i & 3) >= keys) p[i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += p[i];
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            i32x4 pk;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pk[e] = (int)pack_bf16_rne(p[8 * m + 2 * e], p[8 * m + 2 * e + 1]);
+            pf[t][m] = __builtin_bit_cast(bf16x8, pk);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += p[i];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          i32x4 pk;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pk[e] = (int)pack_bf16_rne(p[8 * m + 2 * e], p[8 * m + 2 * e + 1]);
-          pf[t][m] = __builtin_bit_cast(bf16x8, pk);
+        for (int i = 0; i < 4 * KC; ++i) {
+          acc[i % KC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % (2 * KC)], pf[i / (2 * KC)][i / KC % 2], acc[i % KC], 0, 0, 0);
+          if (i < 2 * KC) op[i % (2 * KC)] = v_op(i + 2 * KC);
+          __builtin_amdgcn_sched_barrier(0);
         }
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * KC; ++i) {
-        acc[i % KC] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[i % (2 * KC)], pf[i / (2 * KC)][i / KC % 2], acc[i % KC], 0, 0, 0);
-        if (i < 2 * KC) op[i % (2 * KC)] = v_op(i + 2 * KC);
-        __builtin_amdgcn_sched_barrier(0);
       }
       // (the last MFMAs run meanwhile, and the scores' registers are free)
       if (b + 1 < blocks) {
@@ -770,8 +773,19 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Args8 aa, int32_t 
   auto slot = [&](int wg) { return aa.ws + (int64_t)(2 * wg + (wg == first_wg ? late : 0)) * PF; };
   const int d4 = threadIdx.x % Q4, pg = threadIdx.x / Q4 % PG, rr = threadIdx.x / Q4 / PG;
   const int r = rg * RPW + rr, row = tile * ROWS + r;
+  // a thread's first parts are read whole before the row's reference is known
+  constexpr int AHEAD = 4;
+  float top[AHEAD], sums[AHEAD];
+  f32x4 vals[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) {
+    const float *p = slot(min(first_wg + pg + i * PG, last_wg));
+    top[i] = p[ROWS * D + r], sums[i] = p[ROWS * (D + 1) + r], vals[i] = *(const f32x4 *)&p[r * D + 4 * d4];
+  }
   float m = -__builtin_inff();
-  for (int wg = first_wg + pg; wg <= last_wg; wg += PG) m = fmaxf(m, slot(wg)[ROWS * D + r]);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) m = fmaxf(m, top[i]);  // (the last part's again behind it)
+  for (int wg = first_wg + pg + AHEAD * PG; wg <= last_wg; wg += PG) m = fmaxf(m, slot(wg)[ROWS * D + r]);
   if (PG > 1) {
     if (d4 == 0) rtop[rr][pg] = m;
     __syncthreads();
@@ -780,12 +794,18 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Args8 aa, int32_t 
   }
   float l = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float t, float s, const f32x4 &x) {
+    const float f = t == m ? 1.0f : __builtin_amdgcn_exp2f(t - m);
+    l += f * s;
+    v += f * x;
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (first_wg + pg + i * PG <= last_wg) add(top[i], sums[i], vals[i]);
 #pragma unroll 4
-  for (int wg = first_wg + pg; wg <= last_wg; wg += PG) {
+  for (int wg = first_wg + pg + AHEAD * PG; wg <= last_wg; wg += PG) {
     const float *p = slot(wg);
-    const float top = p[ROWS * D + r], f = top == m ? 1.0f : __builtin_amdgcn_exp2f(top - m);
-    l += f * p[ROWS * (D + 1) + r];
-    v += f * *(const f32x4 *)&p[r * D + 4 * d4];
+    add(p[ROWS * D + r], p[ROWS * (D + 1) + r], *(const f32x4 *)&p[r * D + 4 * d4]);
   }
   if (PG > 1) {
     part[rr][pg][d4] = v;
@@ -909,10 +929,14 @@ template <int D, int ROWS>
 void launch_merge(const Args8 &aa, const Plan8 &p, hipStream_t s) {
   if (p.wgs <= 1) return;
   const int rows = std::min(p.most, ROWS);
-  // items of many parts: a row to a workgroup, its parts shared by 1024 / D threads; else 1024 / D rows
+  // Items of many parts: a row to a workgroup, its parts shared by 1024 / D threads; else
+  // 1024 / D rows to a workgroup.  Whole call of 14 heads of 128 over 40,788 tokens (36
+  // parts), us: 1 row 34 against 46, 64 rows 57 against 64; 256 rows (18 parts) 105
+  // against 99; 40 heads, 91 rows over 11,232 tokens (13 parts) 62 against 54.
   constexpr int RPW = 1024 / D;
-  const int groups = p.wgs > 4 * p.items ? rows : (rows + RPW - 1) / RPW;
-  if (p.wgs > 4 * p.items)
+  const bool many = p.wgs > 24 * p.items;
+  const int groups = many ? rows : (rows + RPW - 1) / RPW;
+  if (many)
     hipLaunchKernelGGL((kv8_merge_kernel<D, ROWS, 1>), dim3((unsigned)(p.items * groups)), dim3(256), 0, s, aa, groups);
   else
     hipLaunchKernelGGL((kv8_merge_kernel<D, ROWS, RPW>), dim3((unsigned)(p.items * groups)), dim3(256), 0, s, aa, groups);
