@@ -1084,7 +1084,9 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
     const int e = group_end(calls, n, i);
     Args8 aa{};
     const Plan8 p = plan(calls + i, e - i, heads, aa.call);
-    if (p.units > INT32_MAX || p.items * p.rows > INT32_MAX) return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows and keys", what);
+    // (the merge's workgroups, 1024 / head_dim rows each, within what a launch holds)
+    if (p.units > INT32_MAX || p.items * (p.rows * head_dim / 1024) >= 1 << 24)
+      return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows and keys", what);
     if (parts_bytes(p, head_dim) > (workspace ? workspace_bytes : 0))
       return set_error(TMHD_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes,
                        (long long)parts_bytes(p, head_dim));

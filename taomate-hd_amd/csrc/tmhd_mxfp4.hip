@@ -177,19 +177,24 @@ __device__ __forceinline__ void mfma_fp4_into(f32x4 &c, const i32x4 &b, const i3
 #undef TMHD_MFMA
 }
 
-// The wait states between the last MFMAs and code that reads their results.
+// The wait states between the last MFMAs and code that reads their results (the
+// sums named on both sides, so that neither may move across).
 template <bool IN_AGPR, int NB, int MB>
 __device__ __forceinline__ void mfma_settle(f32x4 (&acc)[NB][MB]) {
+  auto hold = [&]() {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) {
+        if constexpr (IN_AGPR)
+          asm volatile("" : "+a"(acc[i][j]));
+        else
+          asm volatile("" : "+v"(acc[i][j]));
+      }
+  };
+  hold();
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      if constexpr (IN_AGPR)
-        asm volatile("" : "+a"(acc[i][j]));
-      else
-        asm volatile("" : "+v"(acc[i][j]));
-    }
+  hold();
 }
 
 // Four columns n .. n + 3 of row m, bias added, rounded once.
@@ -759,15 +764,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
 int round4(int32_t rows) { return (int)(((int64_t)rows + 3) / 4 * 4); }
 
 int check_matrix(const char *what, int32_t rows, int32_t cols) {
-  if (rows < 0 || rows > INT32_MAX - 64) return set_error(TMHD_ERR_INVALID, "%s: rows %d", what, rows);
+  if (rows < 0 || rows > INT32_MAX - 256) return set_error(TMHD_ERR_INVALID, "%s: rows %d", what, rows);
   if (cols <= 0 || cols % 32) return set_error(TMHD_ERR_UNSUPPORTED, "%s: columns %d must be a positive multiple of 32", what, cols);
   return TMHD_OK;
 }
 
+constexpr int64_t kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads that a launch holds
+
 // Workgroups of 4 RQ rows x 512 columns; 0: more than a launch holds.
 unsigned quant_grid(int32_t rows, int32_t cols) {
   const int64_t g = (((int64_t)rows + 4 * RQ - 1) / (4 * RQ)) * ((cols + kSuper - 1) / kSuper);
-  return g <= INT32_MAX ? (unsigned)g : 0u;
+  return g <= kMaxGrid ? (unsigned)g : 0u;
 }
 
 int64_t codes_bytes(int32_t rows, int32_t k) { return ((int64_t)rows * (k / 2) + 255) / 256 * 256; }
@@ -776,7 +783,7 @@ int64_t scale_bytes(int32_t rows, int32_t k) { return ((int64_t)k + kSuper - 1) 
 int check_product(const char *what, const void *out, const uint8_t *b, const uint8_t *b_scale, const void *bias, int32_t m,
                   int32_t n, int32_t k, int64_t ldb, int64_t ldo) {
   if (int st = check_matrix(what, m, k)) return st;
-  if (n <= 0 || n > INT32_MAX - 64) return set_error(TMHD_ERR_INVALID, "%s: n %d", what, n);
+  if (n <= 0 || n > INT32_MAX - 256) return set_error(TMHD_ERR_INVALID, "%s: n %d", what, n);
   if (m == 0) return TMHD_OK;
   if (!out || !b || !b_scale || (uintptr_t)b % 16 || (uintptr_t)b_scale % 16 || (uintptr_t)out % 2 || (uintptr_t)bias % 2)
     return set_error(TMHD_ERR_INVALID, "%s: null or misaligned pointer", what);
@@ -883,7 +890,7 @@ int launch_product(const char *what, void *out, const uint8_t *a, const uint8_t 
   const Form f = narrow ? pick_form(m, n, k, cus) : Form{TMHD_MXFP4_ROWS, 0};
   const int64_t big = (int64_t)((m + 255) / 256) * ((n + 255) / 256);
   const int64_t rows_grid = (int64_t)((m + 15) / 16) * ((n + 15) / 16);
-  if (f.form == TMHD_MXFP4_ROWS ? rows_grid > INT32_MAX : big > INT32_MAX / 16)
+  if (f.form == TMHD_MXFP4_ROWS ? rows_grid > kMaxGrid : big > kMaxGrid / 16)
     return set_error(TMHD_ERR_UNSUPPORTED, "%s: %d x %d is too large", what, m, n);
   if (f.tail || f.form == TMHD_MXFP4_256X256) {
     xa.full = (int32_t)(big - f.tail);
