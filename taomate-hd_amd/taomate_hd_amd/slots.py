@@ -297,35 +297,47 @@ class KVSlot8(KVSlot):
 
 def expand_views(torch: Any, views: Sequence[SlotView]) -> list[SlotView]:
     """The 8-bit views among ``views`` (one head count, head_dim and device)
-    as views of one new bf16 slot, each distinct one expanded once, in one
-    launch per 24; bf16 views are returned as they are."""
-    places: dict[tuple[int, int, int], tuple[SlotView, int]] = {}
-    total = 0
+    as views of new bf16 slots (one, or as many as ``MAX_SLOT_CAPACITY`` asks
+    for), each distinct one expanded once, in one launch per slot, format and
+    24 views; bf16 views are returned as they are."""
+    groups: list[list[SlotView]] = []  # of a slot each
+    places: dict[tuple[int, int, int], tuple[int, int]] = {}  # slot, first row
+    totals: list[int] = []
     for view in views:
-        if isinstance(view.slot, KVSlot8):
-            key = (id(view.slot), int(view.row0), int(view.tokens))
-            if key not in places:
-                places[key] = (view, total)
-                total += round_up(view.tokens, KV_TILE)
-    if not places:
-        return list(views)
-    first = next(iter(places.values()))[0].slot
-    out = KVSlot(torch, heads=first.heads, head_dim=first.head_dim, capacity=total, device=first.device)
-    table = (_native.KV8Segment * len(places))()
-    dst = (_native.c_int32 * len(places))()
-    for i, (view, at) in enumerate(places.values()):
-        view.slot.fill_segment8(table, i, view.row0, view.tokens)
-        dst[i] = at
-    stride = out.capacity * out.head_dim
-    with _native.device_of(torch, out.k):
-        status = _native.load().tmhd_kv8_expand(
-            table, dst, len(places), _native.ptr(out.k), _native.ptr(out.vt), stride, stride, out.capacity, out.heads,
-            out.head_dim, _native.stream_ptr(torch, out.device),
-        )
-    _native.check(status, "tmhd_kv8_expand")
-    out.tokens = total
-    return [SlotView(out, view.tokens, places[id(view.slot), int(view.row0), int(view.tokens)][1])
-            if isinstance(view.slot, KVSlot8) else view for view in views]
+        key = (id(view.slot), int(view.row0), int(view.tokens))
+        if not isinstance(view.slot, KVSlot8) or key in places:
+            continue
+        rows = round_up(view.tokens, KV_TILE)
+        if not groups or totals[-1] + rows > MAX_SLOT_CAPACITY:
+            groups.append([])
+            totals.append(0)
+        places[key] = (len(groups) - 1, totals[-1])
+        groups[-1].append(view)
+        totals[-1] += rows
+    slots = []
+    for group, total in zip(groups, totals):
+        first = group[0].slot
+        out = KVSlot(torch, heads=first.heads, head_dim=first.head_dim, capacity=total, device=first.device)
+        table = (_native.KV8Segment * len(group))()
+        dst = (_native.c_int32 * len(group))()
+        for i, view in enumerate(group):
+            view.slot.fill_segment8(table, i, view.row0, view.tokens)
+            dst[i] = places[id(view.slot), int(view.row0), int(view.tokens)][1]
+        stride = out.capacity * out.head_dim
+        with _native.device_of(torch, out.k):
+            status = _native.load().tmhd_kv8_expand(
+                table, dst, len(group), _native.ptr(out.k), _native.ptr(out.vt), stride, stride, out.capacity, out.heads,
+                out.head_dim, _native.stream_ptr(torch, out.device),
+            )
+        _native.check(status, "tmhd_kv8_expand")
+        out.tokens = total
+        slots.append(out)
+
+    def moved(view: SlotView) -> SlotView:
+        at, row0 = places[id(view.slot), int(view.row0), int(view.tokens)]
+        return SlotView(slots[at], view.tokens, row0)
+
+    return [moved(view) if isinstance(view.slot, KVSlot8) else view for view in views]
 
 
 def make_slot(torch: Any, storage: str, **shape: Any) -> KVSlot:

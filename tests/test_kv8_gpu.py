@@ -121,6 +121,23 @@ def test_expand_equals_a_bf16_pack_of_the_values(torch_mod, dev, fmt, dim):
         assert torch.equal(got.slot.vt[:, :, at : at + cap], want.vt[:, :, :cap])
 
 
+def test_expand_of_more_rows_than_a_slot_holds(torch_mod, dev, monkeypatch):
+    """The views then lie in several bf16 slots, in the order given, the same view again in the same place."""
+    from taomate_hd_amd import slots
+
+    torch = torch_mod
+    views = [_slot(torch, *_kv(torch, n, 2, 64, n, dev), "int8", dev).view() for n in (100, 64, 130, 1)]
+    views += [views[1]]
+    whole = slots.expand_views(torch, views)
+    monkeypatch.setattr(slots, "MAX_SLOT_CAPACITY", 256)
+    parts = slots.expand_views(torch, views)
+    assert len({id(v.slot) for v in whole}) == 1 and len({id(v.slot) for v in parts}) == 2 and parts[4] == parts[1]
+    for a, b in zip(whole, parts):
+        assert a.tokens == b.tokens
+        for x, y in zip(a.slot.token_major(), b.slot.token_major()):
+            assert torch.equal(x[a.row0 : a.row0 + a.tokens], y[b.row0 : b.row0 + b.tokens])
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_blocks_without_finite_values(torch_mod, dev, fmt):
     """An infinity or NaN makes its block and head NaN, in every reader, and nothing else."""
