@@ -336,6 +336,36 @@ __device__ __forceinline__ void find_segment(const Args8 &aa, int b, int &si, in
   }
 }
 
+// A walk over a call's blocks of one head's K or V: the block's codes, its scale byte
+// and the valid tokens from its first on.  The segment's own numbers are read where a
+// segment begins: read for every block, their latency is the loop's.
+template <int D, bool V>
+struct Walk {
+  const uint8_t *p, *s;
+  int left, b, si;
+  __device__ __forceinline__ void enter(const Args8 &aa, int h, int at) {  // block `at` of segment si
+    const Seg8 &sg = aa.seg[si];
+    p = (V ? sg.v : sg.k) + ((int64_t)h * sg.cap + (int64_t)at * kBlock) * D;
+    s = (V ? sg.vs : sg.ks) + (int64_t)h * (sg.cap / kBlock) + at;
+    left = sg.tokens - at * kBlock;
+  }
+  __device__ __forceinline__ Walk(const Args8 &aa, const Call8 &cl, int h, int first) : b(first), si(cl.seg0) {
+    int seg_first = 0;
+    find_segment(aa, b, si, seg_first);
+    enter(aa, h, b - seg_first);
+  }
+  __device__ __forceinline__ void next(const Args8 &aa, int h, int b_end) {  // (stays on the last one)
+    if (b + 1 >= b_end) return;
+    ++b;
+    if (left > kBlock) {
+      p += kBlock * D, ++s, left -= kBlock;
+    } else {
+      ++si;
+      enter(aa, h, 0);
+    }
+  }
+};
+
 // floats of a partial result: ROWS of D sums, then the references and the weights' sums
 template <int D, int ROWS>
 constexpr int part_floats() { return ROWS * (D + 2); }
@@ -458,10 +488,11 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
       float top = fmaxf(s[0], s[1]);
 #pragma unroll
       for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * kc;
-      // the reference moves only where a score passes it by 8 (weights up to 2^8)
+      top *= kc;
+      // the reference moves only where a score passes it by 8 (weights up to 2^8); a row's
+      // two lanes have half of its scores each
       if (__any(top > mx + 8.0f)) {
-        const float m = fmaxf(mx, top);
+        const float m = fmaxf(mx, fmaxf(top, __shfl_xor(top, 32)));
         const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
         mx = m;
         sum *= f;
@@ -587,25 +618,22 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-    // the block that is loaded next, its segment, and the valid keys of the
-    // blocks that are loaded and converted
-    int lb = pc.b_begin, si = cl.seg0, s_first = 0;
+    // the block that is loaded next (the last one again behind it)
+    Walk<D, false> kw(aa, cl, h, pc.b_begin);
+    Walk<D, true> vw(aa, cl, h, pc.b_begin);
     i32x4 raw[CH];
     uint32_t kb = 0, vb = 0;
-    int raw_left = 0;
-    auto load = [&]() {  // block lb (the last one again behind it)
-      find_segment(aa, lb, si, s_first);
-      const Seg8 &sg = aa.seg[si];
-      const int sb = lb - s_first;
-      const int64_t off = ((int64_t)h * sg.cap + (int64_t)sb * kBlock) * D, s_at = (int64_t)h * (sg.cap / kBlock) + sb;
+    int raw_left = 0;  // valid keys from its first on
+    auto load = [&]() {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = i * T + tid;
-        raw[i] = *(const i32x4 *)((c < KCH ? sg.k + off : sg.v + off - KCH * 16) + c * 16);
+        raw[i] = *(const i32x4 *)((c < KCH ? kw.p : vw.p - KCH * 16) + c * 16);
       }
-      kb = sg.ks[s_at], vb = sg.vs[s_at];
-      raw_left = sg.tokens - sb * kBlock;
-      if (lb + 1 < pc.b_end) ++lb;
+      kb = *kw.s, vb = *vw.s;
+      raw_left = kw.left;
+      kw.next(aa, h, pc.b_end);
+      vw.next(aa, h, pc.b_end);
     };
     // K chunk (tile, 16 channels, key): two chunks of 8 channels, 512 bytes apart; V
     // chunk (tile, 32 channels, key group, channel): two of 8 keys, 1 KiB apart
@@ -671,10 +699,10 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
         float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * aa.scale2;
-        // the reference moves only where a score passes it by 8 (weights up to 2^8)
+        top *= aa.scale2;
+        // (as in kv8_rows_kernel)
         if (__any(top > mx + 8.0f)) {
-          const float m = fmaxf(mx, top);
+          const float m = fmaxf(mx, fmaxf(top, __shfl_xor(top, 32)));
           const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - m);
           mx = m;
           sum *= f;
@@ -742,6 +770,280 @@ __global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2,
           for (int u = 0; u < 4; ++u)
             *(f32x4 *)&ws[r * D + 32 * d + 8 * u + 4 * g] =
                 f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
+      }
+    }
+    x += blocks;
+  }
+}
+
+// MFMAs of kv8_wide_kernel: volatile asm, so that they stay where the source has them
+// (the compiler gathers the vector work between builtins into one place) and the sums
+// and Q stay in AGPRs.  The compiler does not see the hazards: a weight that a vector
+// instruction wrote goes through two wait states (FRESH), results through settle().
+template <bool FIRST>
+__device__ __forceinline__ void mfma_scores(f32x16 &s, const bf16x8 &k, const bf16x8 &q) {
+  if constexpr (FIRST)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "a"(q));
+  else
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "a"(q));
+}
+template <bool FRESH>
+__device__ __forceinline__ void mfma_output(f32x16 &o, const bf16x8 &v, const bf16x8 &p) {
+  if constexpr (FRESH)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(v), "v"(p));
+  else
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(v), "v"(p));
+}
+// An MFMA of 8 passes wrote the scores: 11 wait states and more before they are read
+__device__ __forceinline__ void settle(f32x16 (&s)[2]) { asm volatile("s_nop 15" : "+v"(s[0]), "+v"(s[1])); }
+template <int KC>
+__device__ __forceinline__ void settle(f32x16 (&o)[2][KC]) {  // (and after vector writes to them)
+#pragma unroll
+  for (int d = 0; d < KC; ++d) asm volatile("s_nop 7" : "+a"(o[0][d]), "+a"(o[1][d]));
+}
+
+// 256 query rows an item, two blocks of 32 rows for each of four waves, one wave a
+// SIMD: an operand read from LDS serves two MFMAs, half of kv8_tile_kernel's reads.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) kv8_wide_kernel(const Args8 aa) {
+  constexpr int KC = D / 32, T = 256, ROWS = 256;
+  constexpr int HALF = kBlock * D * 2;    // bytes of a block's K (or V) in bf16
+  constexpr int CH = kBlock * D / 8 / T;  // 16-byte chunks of codes a thread converts: the first half K, then V
+  constexpr int NQ = 2 * KC, NS = 4 * KC, LA = 4;  // slots of a 32-key tile: scores, then outputs; operands read ahead
+  __shared__ __attribute__((aligned(1024))) char smem[5 * HALF];  // three of K, two of V
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, g = lane >> 5;
+  const int x0 = range_begin(aa, xcd_wg(aa.wgs)), end = range_begin(aa, xcd_wg(aa.wgs) + 1);
+  // (-inf, a masked score, times it stays -inf)
+  const float scale2 = fmaxf(aa.scale2, __uint_as_float(1u));
+  for (int x = x0; x < end;) {
+    const Piece pc = piece_at(aa, x, end);
+    const Call8 &cl = aa.call[pc.call];
+    const int h = pc.head, r0 = pc.tile * ROWS + 64 * w, blocks = pc.b_end - pc.b_begin;
+    bf16x8 qf[2][NQ];
+    load_q<D, false>(aa, cl, h, r0, lr, g, qf[0]);
+    load_q<D, false>(aa, cl, h, r0 + 32, lr, g, qf[1]);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) asm volatile("" : "+a"(qf[0][i]), "+a"(qf[1][i]));
+    f32x16 acc[2][KC];
+    float mx[2] = {-__builtin_inff(), -__builtin_inff()}, sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < KC; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[0][d][i] = acc[1][d][i] = 0.f;
+
+    // the blocks whose K and whose V codes are loaded next (the last one again behind it)
+    Walk<D, false> kw(aa, cl, h, pc.b_begin);
+    Walk<D, true> vw(aa, cl, h, pc.b_begin);
+    i32x4 raw[CH];
+    uint32_t byte[2];
+    int raw_left = 0;  // valid keys from the first of the K block in raw on
+    auto load_k = [&]() {
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) raw[i] = *(const i32x4 *)(kw.p + (i * T + tid) * 16);
+      byte[0] = *kw.s;
+      raw_left = kw.left;
+      kw.next(aa, h, pc.b_end);
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) raw[CH / 2 + i] = *(const i32x4 *)(vw.p + (i * T + tid) * 16);
+      byte[1] = *vw.s;
+      vw.next(aa, h, pc.b_end);
+    };
+    // Half m of chunk i.  A block without finite values makes every output NaN: by way of
+    // `poison`, not of its values.
+    float poison = 0.f;
+    auto convert = [&](int i, int m, char *to) {
+      const bool v = i >= CH / 2;
+      int w0 = raw[i][2 * m], w1 = raw[i][2 * m + 1];
+      asm volatile("" : "+v"(w0), "+v"(w1));  // (converted here, not where it was loaded: four times the registers)
+      const float f = scale_of(byte[v]);
+      if (m == 0) poison += f == f ? 0.f : f;
+      const int c = (v ? i - CH / 2 : i) * T + tid;
+      const i32x2 lo = decode4<E4M3>((uint32_t)w0, f, false), hi = decode4<E4M3>((uint32_t)w1, f, false);
+      *(i32x4 *)(to + (v ? (c >> 6) * 2048 + (c & 63) * 16 + m * 1024 : (c >> 5) * 1024 + (c & 31) * 16 + m * 512)) =
+          i32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    auto mask = [&](f32x16 (&sc)[2], int left) {  // keys of a 32-key tile from `left` on
+      const int keys = in_branch(left) - 4 * g;
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + (i & 3) >= keys) sc[rb][i] = -__builtin_inff();
+    };
+    auto largest = [&](const f32x16 &sc) {
+      float m = sc[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) m = fmaxf(m, sc[i]);
+      return m;
+    };
+    auto move = [&](float (&top)[2]) {  // (as in kv8_rows_kernel)
+      top[0] *= scale2, top[1] *= scale2;
+      if (__any(top[0] > mx[0] + 8.0f || top[1] > mx[1] + 8.0f)) {
+        settle<KC>(acc);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          const float m = fmaxf(mx[rb], fmaxf(top[rb], __shfl_xor(top[rb], 32)));
+          const float f = m == mx[rb] ? 1.0f : __builtin_amdgcn_exp2f(mx[rb] - m);
+          mx[rb] = m;
+          sum[rb] *= f;
+#pragma unroll
+          for (int d = 0; d < KC; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[rb][d][i] *= f;
+        }
+        settle<KC>(acc);
+      }
+    };
+
+    bf16x8 op[NS + LA];
+    // Slot i of a 32-key tile: operand op[i] times both row blocks.  i < NQ: the scores
+    // of the next tile (kt: its keys), else this tile's weights times V (vt)
+    auto read_op = [&](int i, const char *kt, const char *vt) {
+      return i < NQ ? *(const bf16x8 *)(kt + i * 1024) : *(const bf16x8 *)(vt + (i - NQ) / KC * 1024 + (i - NQ) % KC * 2048);
+    };
+    // One tile: sc its scores, nx the next tile's (left: its valid keys); chunks c0 .. of
+    // the codes in raw are converted
+    auto tile = [&](f32x16 (&sc)[2], f32x16 (&nx)[2], const char *kt, const char *vt, const char *kt_next, int left, int c0,
+                    char *k_to, char *v_to) {
+      i32x4 pf[2][2];  // weights: [row block][16 keys]
+      float pe[16][2], top[2];
+      // Where the pairs of weights are computed (in the order in which the outputs' MFMAs
+      // need them): the exponentials, and one MFMA later the rest
+      auto pair_at = [](int u) { return u < 11 ? u * 2 * NQ / 11 : 2 * NQ + (u - 11) * 2 * KC / 5; };
+#pragma clang loop unroll(full)
+      for (int r = 0; r < 2 * NS; ++r) {  // what goes in front of MFMA r
+        const int i = r >> 1, rb = r & 1;
+        if (rb == 1) op[i + LA] = i + LA < NS ? read_op(i + LA, kt, vt) : read_op(i + LA - NS, kt_next, vt);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const int st = u >> 3, b = (u >> 2) & 1, q = u & 3;
+          if (pair_at(u) == r) {
+            pe[u][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][8 * st + 2 * q], scale2, -mx[b]));
+            pe[u][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][8 * st + 2 * q + 1], scale2, -mx[b]));
+            asm volatile("" : "+v"(pe[u][0]), "+v"(pe[u][1]));
+          }
+          if (pair_at(u) + 1 == r) {
+            int pk = (int)pack_bf16_rne(pe[u][0], pe[u][1]);
+            sum[b] += pe[u][0];
+            sum[b] += pe[u][1];
+            asm volatile("" : "+v"(pk), "+v"(sum[b]));
+            pf[b][st][q] = pk;
+          }
+        }
+        if (r == 2 * NQ + 2) settle(nx);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (r == 2 * NQ + 2 + u * (2 * NQ - 2) / 8) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float m = fmaxf(nx[b][2 * u], nx[b][2 * u + 1]);
+              top[b] = u ? fmaxf(top[b], m) : m;
+              asm volatile("" : "+v"(top[b]));
+            }
+          }
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          if (r == 2 * NQ + 2 * KC + c * 2 * KC / CH) convert(c0 + (c >> 1), c & 1, c0 ? v_to : k_to);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i == 0)
+          mfma_scores<true>(nx[rb], op[i], qf[rb][i]);
+        else if (i < NQ)
+          mfma_scores<false>(nx[rb], op[i], qf[rb][i]);
+        else if (i == NQ || i == NQ + KC)
+          mfma_output<true>(acc[rb][0], op[i], __builtin_bit_cast(bf16x8, pf[rb][(i - NQ) / KC]));
+        else
+          mfma_output<false>(acc[rb][(i - NQ) % KC], op[i], __builtin_bit_cast(bf16x8, pf[rb][(i - NQ) / KC]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < LA; ++i) op[i] = op[NS + i];
+      if (left < 32) {
+        mask(nx, left);
+        top[0] = largest(nx[0]), top[1] = largest(nx[1]);
+      }
+      move(top);
+    };
+
+    // K of blocks 0 and 1, V of block 0; the codes of block 2's K and block 1's V
+    if (x != x0) __syncthreads();  // the last piece's buffers are read out
+    char *const vb0 = smem + 3 * HALF;
+    load_k();
+    load_v();
+    int left0 = raw_left;  // valid keys from block b's first on, and from block b + 1's
+#pragma unroll
+    for (int i = 0; i < 2 * CH; ++i) convert(i >> 1, i & 1, i < CH ? smem : vb0);
+    load_k();
+    int left1 = raw_left;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) convert(i >> 1, i & 1, smem + HALF);
+    load_k();
+    load_v();
+    __syncthreads();
+    f32x16 sa[2], sb[2];
+    const char *const mine = smem + lane * 16;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const bf16x8 o = read_op(i, mine, mine);
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        if (i)
+          mfma_scores<false>(sa[rb], o, qf[rb][i]);
+        else
+          mfma_scores<true>(sa[rb], o, qf[rb][i]);
+      }
+    }
+    settle(sa);
+    if (left0 < 32) mask(sa, left0);
+    {
+      float top[2] = {largest(sa[0]), largest(sa[1])};
+      move(top);
+    }
+    int k0 = 0, k1 = HALF, k2 = 2 * HALF;  // the K buffers of blocks b, b + 1, b + 2
+#pragma unroll
+    for (int i = 0; i < LA; ++i) op[i] = read_op(i, mine + HALF / 2, mine);
+    for (int b = 0; b < blocks; ++b) {
+      const char *vt = mine + (3 + (b & 1)) * HALF;
+      char *v_to = vb0 + ((b & 1) ^ 1) * HALF;
+      if (b) __syncthreads();
+      tile(sa, sb, mine + k0 + HALF / 2, vt, mine + k1, left0 - 32, 0, smem + k2, v_to);
+      const int left2 = raw_left;
+      load_k();  // (a whole iteration ahead of its conversion, as V's)
+      tile(sb, sa, mine + k1, vt + HALF / 2, mine + k1 + HALF / 2, left1, CH / 2, smem + k2, v_to);
+      load_v();
+      left0 = left1, left1 = left2;
+      const int t = k0;
+      k0 = k1, k1 = k2, k2 = t;
+    }
+
+    settle<KC>(acc);
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      const float l = sum[rb] + __shfl_xor(sum[rb], 32) + poison;
+      const int row = r0 + 32 * rb + lr;
+      if (row < cl.lq) {
+        if (pc.whole) {
+          const int64_t orow = cl.o_rows ? cl.o_rows[row] : cl.o_row0 + row;
+          uint16_t *o = cl.o + orow * cl.ots + (int64_t)h * cl.ohs + 4 * g;
+          const float inv = 1.0f / l;
+#pragma unroll
+          for (int d = 0; d < KC; ++d)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *(i32x2 *)(o + 32 * d + 8 * u) =
+                  pack4(f32x4{acc[rb][d][4 * u], acc[rb][d][4 * u + 1], acc[rb][d][4 * u + 2], acc[rb][d][4 * u + 3]}, inv);
+        } else {
+          const int r = 64 * w + 32 * rb + lr;
+          float *ws = aa.ws + (int64_t)(2 * xcd_wg(aa.wgs) + (x != x0)) * part_floats<D, ROWS>();
+          if (g == 0) ws[ROWS * D + r] = mx[rb], ws[ROWS * (D + 1) + r] = l;
+#pragma unroll
+          for (int d = 0; d < KC; ++d)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *(f32x4 *)&ws[r * D + 32 * d + 8 * u + 4 * g] =
+                  f32x4{acc[rb][d][4 * u], acc[rb][d][4 * u + 1], acc[rb][d][4 * u + 2], acc[rb][d][4 * u + 3]};
+        }
       }
     }
     x += blocks;
@@ -951,7 +1253,7 @@ void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
     hipLaunchKernelGGL((kv8_tile_kernel<D, 4, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
     launch_merge<D, 128>(aa, p, s);
   } else {
-    hipLaunchKernelGGL((kv8_tile_kernel<D, 8, E4M3>), dim3((unsigned)p.wgs), dim3(512), 0, s, aa);
+    hipLaunchKernelGGL((kv8_wide_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
     launch_merge<D, 256>(aa, p, s);
   }
 }
