@@ -580,23 +580,18 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
   }
 }
 
-// 32 RW query rows an item: RW waves of 32 rows, two waves a SIMD.  A block of 64
+// 128 query rows an item: four waves of 32 rows, two workgroups a CU.  A block of 64
 // tokens is turned into bf16 once, its scales included (exact), by all threads,
 // into MFMA operand order in LDS (chunks of 16 bytes, a wave's read 1 KiB in a row);
 // then every wave multiplies its rows with it.  Two buffers: while block b is
 // multiplied, block b + 1 (in registers since the block before) is converted and
-// block b + 2 loaded; one barrier a block.  Per block and wave: 32 MFMAs of 32
-// cycles, about as many cycles of vector work (32 exponentials of 16, 32 of
-// everything else) and 32 KiB of LDS reads (256 cycles of the CU's LDS, 2048 for the
-// eight waves, as long as their MFMAs): the three are close to balance.  14 heads of
-// 128 over 40,788 tokens, e4m3: 128 rows 77 us, 256 rows 104 us (720 TFLOPS), 4,836
-// rows 1,356 us (1,040); MFMAs busy 46% of the time, waves waiting for operands or
-// the barrier 27%.  Scores of a block interleaved with the weights of the one before,
-// product by product, took 110 and 1,405 us; raised wave priority in the products
-// changed nothing.
-template <int D, int RW, bool E4M3>
-__global__ void __launch_bounds__(RW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_tile_kernel(const Args8 aa) {
-  constexpr int KC = D / 32, T = RW * 64, ROWS = 32 * RW;
+// block b + 2 loaded; one barrier a block.  Bound by the latencies between a block's
+// load, conversion, products and barrier, which the CU's other workgroup only
+// half fills: 14 heads of 128 over 40,788 tokens, e4m3: 64 rows 60 us (2.4 TB/s), 128
+// rows 76 us (490 TFLOPS); 40 heads, 91 rows over 11,232 tokens, int8: 55 us.
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_tile_kernel(const Args8 aa) {
+  constexpr int KC = D / 32, T = 256, ROWS = 128;
   constexpr int HALF = kBlock * D * 2;             // bytes of a block's K (or V) in bf16
   constexpr int CH = kBlock * D / 8 / T;           // 16-byte chunks of codes a thread converts, of K then of V
   constexpr int KCH = kBlock * D / 16;             // chunks of K
@@ -803,7 +798,18 @@ __device__ __forceinline__ void settle(f32x16 (&o)[2][KC]) {  // (and after vect
 }
 
 // 256 query rows an item, two blocks of 32 rows for each of four waves, one wave a
-// SIMD: an operand read from LDS serves two MFMAs, half of kv8_tile_kernel's reads.
+// SIMD: an operand read from LDS serves two MFMAs.  Codes become bf16 in LDS as in
+// kv8_tile_kernel.  A wave goes through tiles of 32 keys: while the scores of the next
+// tile are multiplied, the weights of this one are computed, a pair in front of two MFMAs
+// of three; then this tile's outputs, with the last weights, the next tile's maximum
+// and the conversion of block b + 2's K or block b + 1's V (loaded an iteration before)
+// in front of the MFMAs.  K in three buffers, V in two, one barrier for 64 keys.
+// 14 heads of 128 over 40,788 tokens, e4m3 (int8): 256 rows 102 us (108), 1,024 rows 305
+// (332; 983 TFLOPS), 4,836 rows 1,383 (1,479).  Bound by issue: MFMAs busy 48% of the
+// time, instructions issuing 59%; without the conversion (16 cycles for two values) 13%
+// less time, without the exponentials 9%, without the barrier 3%.  Eight waves of 32 rows
+// took 104, 339 and 1,356 us (int8 108, 353, 1,459) and read LDS for as long as they
+// multiplied; with segment numbers read for every block this one took 1,467 us.
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) kv8_wide_kernel(const Args8 aa) {
   constexpr int KC = D / 32, T = 256, ROWS = 256;
@@ -1178,8 +1184,8 @@ struct Plan8 {
 };
 
 // The calls of one launch.  Up to 32 rows: items of 32, two workgroups a CU; else
-// of 128 (two a CU) or, beyond 128 rows, of 256.  A workgroup takes at least 8 blocks
-// (two for each wave that loads blocks of its own) or 4.
+// of 128 (two a CU) or, beyond 128 rows, of 256 (one).  A workgroup takes at least 8
+// blocks (two for each wave that loads blocks of its own) or 4.
 Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
   Plan8 p{32, 0, 0, 0, 0};
   for (int i = 0; i < n; ++i) p.most = std::max(p.most, calls[i].lq);
@@ -1250,7 +1256,7 @@ void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
     hipLaunchKernelGGL((kv8_rows_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
     launch_merge<D, 32>(aa, p, s);
   } else if (p.rows == 128) {
-    hipLaunchKernelGGL((kv8_tile_kernel<D, 4, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
+    hipLaunchKernelGGL((kv8_tile_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
     launch_merge<D, 128>(aa, p, s);
   } else {
     hipLaunchKernelGGL((kv8_wide_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);

@@ -29,14 +29,15 @@ BACKENDS = ("bf16", "i8qk")
 # 8-bit segments are read in place by calls of up to KV8_ROWS query rows, and by
 # batches of up to KV8_WORK (query row, token, channel) products.  The kernel that
 # reads codes turns every block into bf16 for 256 rows at a time and multiplies at
-# 0.85 PFLOPS; expanding costs a pass over the cache and a launch, the bf16 kernel
+# 1.0 PFLOPS; expanding costs a pass over the cache and a launch, the bf16 kernel
 # then runs at up to 1.35.  Measured, e4m3, in place / expanded, us: 14 heads of 128
-# over 41,000 tokens 109/190 at 256 rows, 182/230 at 512, 331/347 at 1,024, 450/453 at
-# 1,536, 735/696 at 2,560; 11,000 tokens 59/68, 80/75, 128/104; 2,800 tokens (2.6e9
-# products) 54/49 at 512; 700 tokens (1.3e9) 38/50 at 1,024 and 50/47 at 2,560; 4 heads
-# of 64 over 41,000 tokens 58/73 at 512, 89/76 at 1,024.  int8 is 2 to 5% slower in place.
-KV8_ROWS = 512
-KV8_WORK = 3 << 29
+# over 41,000 tokens 105/189 at 256 rows, 300/351 at 1,024, 566/590 at 2,048, 1,386/1,223
+# at 5,120; 11,000 tokens 70/75 at 512, 108/105 at 1,024, 141/133 at 1,536; 2,800 tokens
+# 48/53 at 512; 700 tokens 47/50 at 1,536 (1.9e9 products), 53/50 at 2,560 (3.2e9); 4 heads
+# over 2,800 tokens 45/54 at 2,048 (2.9e9); 14 heads of 64 over 41,000 tokens 126/133 at
+# 512, 222/216 at 1,024, 320/288 at 1,536.  int8 is 5 to 10% slower in place.
+KV8_ROWS = 1024
+KV8_WORK = 5 << 29
 
 
 class QKQuantWorkspace:
