@@ -304,27 +304,47 @@ def test_more_calls_than_one_launch(torch_mod, dev):
         assert (np.abs(_f64(again) - want) <= bound).all()
 
 
-def test_large_scores_move_the_running_maximum(torch_mod, dev):
+@pytest.mark.parametrize("rows,dim", [(20, 128), (90, 128), (300, 128), (150, 64)])
+def test_large_scores_move_the_running_maximum(torch_mod, dev, rows, dim):
     from taomate_hd_amd import segment_attention
 
     torch = torch_mod
-    k, v = _kv(torch, 1500, 2, 128, 1, dev)
+    k, v = _kv(torch, 1500, 2, dim, 1, dev)
     k = k * torch.linspace(0.1, 6.0, 1500, device=dev).view(-1, 1, 1).to(torch.bfloat16)
     slot = _slot(torch, k, v, "int8", dev)
-    q = 8 * _kv(torch, 20, 2, 128, 2, dev)[0]
-    got = segment_attention(torch, q, [slot.view()], scale=128 ** -0.5)
-    want, bound = _want(q, [slot.view()], 128 ** -0.5)
+    q = 8 * _kv(torch, rows, 2, dim, 2, dev)[0]
+    got = segment_attention(torch, q, [slot.view()], scale=dim ** -0.5)
+    want, bound = _want(q, [slot.view()], dim ** -0.5)
     assert (np.abs(_f64(got) - want) <= bound).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 33, 200])
+def test_values_behind_a_view_that_overflow(torch_mod, dev, rows, fmt):
+    """Rows of the view's last block that it does not hold: their scores are infinite, their weights nothing."""
+    from taomate_hd_amd import segment_attention
+    from taomate_hd_amd.slots import SlotView
+
+    torch = torch_mod
+    k, v = _kv(torch, 192, 2, 64, 1, dev)
+    k[70:], v[70:] = 2.0 ** 100, 2.0 ** 100
+    slot = _slot(torch, k, v, fmt, dev)
+    q = 2.0 ** 40 * _kv(torch, rows, 2, 64, 2, dev)[0].abs()
+    for view in (SlotView(slot, 70, 0), SlotView(slot, 6, 64)):
+        got = segment_attention(torch, q, [view], scale=2.0 ** -43)
+        want, bound = _want(q, [view], 2.0 ** -43)
+        assert (np.abs(_f64(got) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("rows", [3, 33, 200])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 40.0])
-def test_any_softmax_scale(torch_mod, dev, scale):
+def test_any_softmax_scale(torch_mod, dev, scale, rows):
     """No scale (the mean of the values), a negative, a vanishing and a large one, with a ragged last tile."""
     from taomate_hd_amd import segment_attention
 
     torch = torch_mod
     slot = _slot(torch, *_kv(torch, 71, 2, 64, 1, dev), "int8", dev)
-    q = _kv(torch, 33, 2, 64, 2, dev)[0]
+    q = _kv(torch, rows, 2, 64, 2, dev)[0]
     got = segment_attention(torch, q, [slot.view()], scale=scale)
     want, bound = _want(q, [slot.view()], scale)
     assert (np.abs(_f64(got) - want) <= bound).all()
@@ -358,14 +378,15 @@ def test_refusals(torch_mod, dev):
         slot.view().to_segment()
 
 
-def test_streams_and_graph(torch_mod, dev):
+@pytest.mark.parametrize("rows", [2, 100, 400])
+def test_streams_and_graph(torch_mod, dev, rows):
     """A pack and a decode call on another stream, and captured and replayed with new K/V between eager calls."""
     from taomate_hd_amd import KVSlot8, segment_attention
 
     torch = torch_mod
     slot = KVSlot8(torch, heads=4, head_dim=128, capacity=5000, device=dev)
     k, v = _kv(torch, 5000, 4, 128, 1, dev)
-    q = _kv(torch, 2, 4, 128, 2, dev)[0]
+    q = _kv(torch, rows, 4, 128, 2, dev)[0]
 
     def step():
         slot.pack(k, v)
