@@ -398,7 +398,7 @@ __device__ __forceinline__ int in_branch(int keys) {
 
 constexpr int kWaves8 = 4;
 
-// Up to 32 query rows an item.  The four waves of a workgroup take an item's
+// 32 query rows an item.  The four waves of a workgroup take an item's
 // blocks in turn and merge through LDS.  Per 32 keys a lane loads the 16-byte
 // chunks that are its MFMA operands (no LDS on the way: each code is used once)
 // and turns them into bf16, exactly; S^T = K Q^T leaves 16 keys of one query in a
@@ -1183,13 +1183,25 @@ struct Plan8 {
   int most;  // query rows of the longest call
 };
 
-// The calls of one launch.  Up to 32 rows: items of 32, two workgroups a CU; else
-// of 128 (two a CU) or, beyond 128 rows, of 256 (one).  A workgroup takes at least 8
-// blocks (two for each wave that loads blocks of its own) or 4.
-Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
+// The calls of one launch: items of 32 rows (two workgroups a CU) for up to 32 rows, or
+// where they are up to 28 * 128 / D units a workgroup; else of 128 rows (two a CU) or,
+// beyond 128 rows, of 256 (one).  A workgroup of 32 rows turns the codes into bf16 for
+// them alone, but has no barriers and small parts to merge.  us, items of 32 against
+// wider ones, e4m3: 14 heads of 128, 200 rows over 400 tokens (1.3 units) 23/31, 400 rows
+// over 1,500 (8.5) 24/41, 256 over 6,000 (21) 36/49; 40 heads, 400 rows over 1,500 (24)
+// 36/46, 128 over 6,000 (29) 47/46, 91 over 12,000 (44) 65/53; 14 heads of 64, 256 rows
+// over 12,000 (41) 34/44, 400 over 12,000 (67) 48/52.
+// A workgroup takes at least 8 blocks (two for each wave that loads blocks of its
+// own) or 4.
+Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, Call8 *out) {
   Plan8 p{32, 0, 0, 0, 0};
-  for (int i = 0; i < n; ++i) p.most = std::max(p.most, calls[i].lq);
-  p.rows = p.most <= 32 ? 32 : p.most <= 128 ? 128 : 256;
+  const int64_t cus = std::max(device_cus(), 8);
+  int64_t units32 = 0;
+  for (int i = 0; i < n; ++i) {
+    p.most = std::max(p.most, calls[i].lq);
+    units32 += (int64_t)heads * (((int64_t)calls[i].lq + 31) / 32) * blocks_of(calls[i]);
+  }
+  p.rows = p.most <= 32 || units32 <= 2 * cus * 28 * 128 / D ? 32 : p.most <= 128 ? 128 : 256;
   for (int i = 0; i < n; ++i) {
     Call8 c{};
     c.lq = calls[i].lq;
@@ -1200,7 +1212,7 @@ Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, Call8 *out) {
     p.units += (int64_t)heads * c.row_tiles * c.blocks;
     if (out) out[i] = c;
   }
-  const int64_t room = (int64_t)std::max(device_cus(), 8) * (p.rows == 256 ? 1 : 2), least = p.rows == 32 ? 2 * kWaves8 : 4;
+  const int64_t room = cus * (p.rows == 256 ? 1 : 2), least = p.rows == 32 ? 2 * kWaves8 : 4;
   p.wgs = (int)std::min<int64_t>(room, (p.units + least - 1) / least);
   return p;
 }
@@ -1374,7 +1386,7 @@ extern "C" int64_t tmhd_attn_kv8_workspace_bytes(const tmhd_kv8_call *calls, int
   int64_t most = 0;
   for (int i = 0; i < n;) {
     const int e = group_end(calls, n, i);
-    most = std::max(most, parts_bytes(plan(calls + i, e - i, heads, nullptr), head_dim));
+    most = std::max(most, parts_bytes(plan(calls + i, e - i, heads, head_dim, nullptr), head_dim));
     i = e;
   }
   return most;
@@ -1391,7 +1403,7 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
   for (int i = 0; i < n;) {
     const int e = group_end(calls, n, i);
     Args8 aa{};
-    const Plan8 p = plan(calls + i, e - i, heads, aa.call);
+    const Plan8 p = plan(calls + i, e - i, heads, head_dim, aa.call);
     // (the merge's workgroups, 1024 / head_dim rows each, within what a launch holds)
     if (p.units > INT32_MAX || p.items * (p.rows * head_dim / 1024) >= 1 << 24)
       return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows and keys", what);

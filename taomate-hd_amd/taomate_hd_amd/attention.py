@@ -27,15 +27,15 @@ from .slots import KV_TILE, KVSlot, KVSlot8, SlotView, expand_views, round_up, v
 
 BACKENDS = ("bf16", "i8qk")
 # 8-bit segments are read in place by calls of up to KV8_ROWS query rows, and by
-# batches of up to KV8_WORK (query row, token, channel) products.  The kernel that
-# reads codes turns every block into bf16 for 256 rows at a time and multiplies at
+# batches of up to KV8_WORK (query row, token, channel) products.  The kernels that
+# read codes turn every block into bf16 for at most 256 rows at a time and multiply at
 # 1.0 PFLOPS; expanding costs a pass over the cache and a launch, the bf16 kernel
 # then runs at up to 1.35.  Measured, e4m3, in place / expanded, us: 14 heads of 128
-# over 41,000 tokens 105/189 at 256 rows, 300/351 at 1,024, 566/590 at 2,048, 1,386/1,223
-# at 5,120; 11,000 tokens 70/75 at 512, 108/105 at 1,024, 141/133 at 1,536; 2,800 tokens
-# 48/53 at 512; 700 tokens 47/50 at 1,536 (1.9e9 products), 53/50 at 2,560 (3.2e9); 4 heads
-# over 2,800 tokens 45/54 at 2,048 (2.9e9); 14 heads of 64 over 41,000 tokens 126/133 at
-# 512, 222/216 at 1,024, 320/288 at 1,536.  int8 is 5 to 10% slower in place.
+# over 41,000 tokens 108/187 at 256 rows, 301/348 at 1,024, 573/613 at 2,048, 1,418/1,227
+# at 5,120; 11,000 tokens 71/76 at 512, 109/106 at 1,024, 143/133 at 1,536; 2,800 tokens
+# 54/54 at 1,024; 700 tokens 35/50 at 1,536 (1.9e9 products), 52/51 at 2,560 (3.2e9); 4
+# heads over 2,800 tokens 30/54 at 2,048 (2.9e9); 14 heads of 64 over 41,000 tokens
+# 127/145 at 512, 222/223 at 1,024, 321/294 at 1,536.  int8 is 5 to 10% slower in place.
 KV8_ROWS = 1024
 KV8_WORK = 5 << 29
 
