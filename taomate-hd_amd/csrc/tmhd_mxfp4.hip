@@ -542,23 +542,25 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
   store_tile<T::NB, T::MB>(xa, t.acc, m0 + t.wm * MH, n0 + t.wn * NH, t.li, t.lg);
 }
 
-// 256 x 256 tiles [0, xa.full), 4 waves as 2 x 2 of 128 x 128 (256 sums a lane, in
-// AGPRs), by a grid that is resident at once: a workgroup takes one tile after the
-// other and its loads never pause, for the next tile's first blocks are loaded
+// 256 x 256 tiles [0, xa.full), 8 waves as 2 x 4 of 128 x 64 (128 sums a lane, in
+// AGPRs), two on a SIMD, by a grid that is resident at once: a workgroup takes one tile
+// after the other and its loads never pause, for the next tile's first blocks are loaded
 // under the last MFMAs of a tile and land while it is stored.
 // k moves in blocks of 128 bytes.  A block's operands are four units of 128 rows
 // (A rows 0 .., B rows 0 .., A rows 128 .., B rows 128 ..; rows and swizzle as in
 // TileLoop) in a ring of nine; the scale words of two blocks, 8 KiB, in one of two
-// buffers: all of the LDS.  Block d: step 0 multiplies operands that are in
-// registers, reads step 1's and loads the first unit of block d + 2 (the ninth
-// slot); behind the wait for block d + 1 and the barrier, step 1 reads block d + 1's
-// first operands (and its scale words, if they are new) and loads the other three
-// units of block d + 2 (and its scale words).
-// A scaled MFMA takes 16 cycles and two of the wave's issue slots of 4; the other
-// two are all that the loop's remaining instructions have.  With scale words read
-// and copied for every block, addresses added per load and two buffers of whole
-// blocks there were 2.2 of them per MFMA, and the matrix units were busy 41-45% of
-// the time.
+// buffers: all of the LDS.  An operand's register is read anew behind its last MFMA of
+// the step: in step 0 of block d for step 1, in step 1 for block d + 1 (with its scale
+// bytes), behind the wait for that block and the barrier, which come when step 1's
+// operands have long arrived.  Step 0 loads the first unit of block d + 2 (the ninth
+// slot), step 1 the other three and their scale words.
+// 12,252 x 13,824 x 5,120 404 us (4,290 TFLOPS), 4,836 x 10,752 x 5,376 132 us (4,220,
+// the last round in smaller tiles).  Four waves of 128 x 128, each step's operands read
+// a step ahead into a second set of registers, took 411 and 137 us, 2,717 x 5,376 x
+// 5,376 47 against 43.  Without stores it takes 352 us, without loads and stores 294, and
+// the MFMAs alone take 243 at the clock that the power limit leaves them: what the tile
+// moves costs time by its energy more than by its latency (the barrier, earlier or
+// later in the step, and wave priorities change nothing).
 template <int UNITS>
 struct BigLoop {
   static constexpr int UNIT = 128 * KB, RING = UNITS * UNIT, SBUF = 512 * 16;
@@ -574,15 +576,15 @@ struct BigLoop {
   int slot;                    // ring slot of the current block's first unit
   int sload;                   // buffer of the next scale words
   int sread, rb;               // where the next block's scale bytes are read, and its number in its tile
-  uint32_t doff[4][4], soff[2], rdq[2], rds[2][4];
-  f32x4 acc[8][8];             // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
-  i32x4 cur[16], nxt[16];      // operands: A blocks 0 .. 7, B blocks 0 .. 7
-  int sc[16];                  // their scale words
+  uint32_t doff[4][2], soff, rdq[2], rds[2][4];
+  f32x4 acc[4][8];             // D[n][m]: lane (j, g4) holds n = 16 nb + 4 g4 + (0..3), m = 16 mb + j
+  i32x4 cur[12];               // operands: A blocks 0 .. 7, B blocks 0 .. 3
+  int sc[12];                  // their scale words
 
   __device__ __forceinline__ BigLoop(const XArgs &args, char *lds) : xa(args), smem(lds) {
     lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     lane = threadIdx.x & 63, li = lane & 15, lg = lane >> 4;
-    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 1, wn = w & 1;
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = w >> 2, wn = w & 3;
     chunks = xa.k >> 5, nd = (xa.k + 255) >> 8;
     lch = (lane & 7) ^ ((4 * (w & 1) + (lane >> 4)) & 7);
 #pragma unroll
@@ -592,7 +594,7 @@ struct BigLoop {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint32_t word = (uint32_t)(RING + lg * 1024 + ((c ^ lg) * 16 + li) * 4);
-      rds[0][c] = word + wm * 512, rds[1][c] = word + 4096 + wn * 512;
+      rds[0][c] = word + wm * 512, rds[1][c] = word + 4096 + wn * 256;
     }
     tmc = (xa.m + 255) / 256, tnc = (xa.n + 255) / 256;
   }
@@ -603,14 +605,13 @@ struct BigLoop {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = (j >> 1) * 128 + (w + 4 * i) * 8 + (lane >> 3);
+      for (int i = 0; i < 2; ++i) {
+        const int r = (j >> 1) * 128 + (w + 8 * i) * 8 + (lane >> 3);
         doff[j][i] = (j & 1 ? (uint32_t)((int64_t)min(tn * 256 + r, xa.n - 1) * xa.ldb)
                             : (uint32_t)((int64_t)min(tm * 256 + r, xa.m - 1) * xa.lda)) + lch * 16;
       }
-    const int r = (lane * 4) ^ (16 * w);  // entry g = w of A's words, then of B's
-    soff[0] = (uint32_t)(((int64_t)w * xa.am4 + min(tm * 256 + r, xa.am4 - 4)) * 4);
-    soff[1] = (uint32_t)(((int64_t)w * xa.bn4 + min(tn * 256 + r, xa.bn4 - 4)) * 4);
+    const int e = w & 3, r = (lane * 4) ^ (16 * e);  // entry e of A's words (waves 0 .. 3) or of B's
+    soff = (uint32_t)(w < 4 ? ((int64_t)e * xa.am4 + min(tm * 256 + r, xa.am4 - 4)) * 4 : ((int64_t)e * xa.bn4 + min(tn * 256 + r, xa.bn4 - 4)) * 4);
     lb = 0, abase = xa.a, bbase = xa.b;
     if (nd == 1) last_block();
   }
@@ -620,16 +621,15 @@ struct BigLoop {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) doff[j][i] -= back;
+      for (int i = 0; i < 2; ++i) doff[j][i] -= back;
   }
   // load i of unit j of the block at the load cursor, into ring slot s
   __device__ __forceinline__ void load_data(int s, int j, int i) {
-    load_lds16_any(j & 1 ? bbase : abase, doff[j][i], lds0 + (uint32_t)(s * UNIT + (w + 4 * i) * 1024));
+    load_lds16_any(j & 1 ? bbase : abase, doff[j][i], lds0 + (uint32_t)(s * UNIT + (w + 8 * i) * 1024));
   }
   __device__ __forceinline__ void load_scales() {
     const uint32_t to = lds0 + (uint32_t)(RING + sload * SBUF + w * 1024);
-    load_lds16_any(xa.as + (int64_t)(lb >> 1) * 4 * xa.am4, soff[0], to);
-    load_lds16_any(xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4, soff[1], to + 4096);
+    load_lds16_any(w < 4 ? xa.as + (int64_t)(lb >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4, soff, to);
     sload ^= 1;
   }
   // the load cursor's next block: of this tile, of the workgroup's next one, or
@@ -647,7 +647,7 @@ struct BigLoop {
   static __device__ __forceinline__ int wrap(int s) { return s >= UNITS ? s - UNITS : s; }
   // operand r (A blocks 0 .. 7, then B's) of step q of the block whose units start at ring slot s
   __device__ __forceinline__ uint32_t op_base(int s, int q, bool b) const {
-    return (uint32_t)(wrap(s + (b ? 2 * wn + 1 : 2 * wm)) * UNIT) + rdq[q];
+    return (uint32_t)(wrap(s + (b ? (wn & 2) + 1 : 2 * wm)) * UNIT + (b ? (wn & 1) * 64 * KB : 0)) + rdq[q];
   }
   __device__ __forceinline__ i32x4 read_op(uint32_t base, int r) const { return *(const i32x4 *)(smem + base + (r & 7) * 16 * KB); }
   // scale bytes of operand r for the block whose bytes start at `from` of the buffers: step 0's, then step 1's
@@ -667,14 +667,14 @@ struct BigLoop {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_data(4 * d + j, j, i);
+        for (int i = 0; i < 2; ++i) load_data(4 * d + j, j, i);
       advance();
     }
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(16));
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(8));
     __syncthreads();
     const uint32_t a = op_base(0, 0, false), b = op_base(0, 0, true);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < 12; ++r) {
       cur[r] = read_op(r < 8 ? a : b, r);
       sc[r] = read_scale(rds, r);
     }
@@ -684,7 +684,7 @@ struct BigLoop {
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -694,47 +694,48 @@ struct BigLoop {
     {
       const uint32_t a = op_base(slot, 1, false), b = op_base(slot, 1, true);
 #pragma unroll
-      for (int idx = 0; idx < 64; ++idx) {
-        if (idx % 4 == 0) nxt[idx / 4] = read_op(idx / 4 < 8 ? a : b, idx / 4);
+      for (int idx = 0; idx < 32; ++idx) {
+        const int nb = idx >> 3, mb = idx & 7;
         if (idx % 16 == 2) load_data(over, 0, idx / 16);
-        mfma_fp4_into<0, true>(acc[idx >> 3][idx & 7], cur[8 + (idx >> 3)], cur[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
+        mfma_fp4_into<0, true>(acc[nb][mb], cur[8 + nb], cur[mb], sc[8 + nb], sc[mb]);
         __builtin_amdgcn_sched_barrier(0);
+        if (nb == 3) cur[mb] = read_op(a, mb);
+        if (mb == 7) cur[8 + nb] = read_op(b, 8 + nb);
       }
     }
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(4));
-    __syncthreads();
-    if ((lb & 1) == 0) load_scales();
-    int asc[8];  // the A rows' next scale bytes (B's replace the old ones, each after its last use)
+    uint32_t at[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) at[h][c] = rds[h][c] + sread;
     {
       const uint32_t a = op_base(next, 0, false), b = op_base(next, 0, true);
-      uint32_t at[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) at[h][c] = rds[h][c] + sread;
-#pragma unroll
-      for (int idx = 0; idx < 64; ++idx) {
-        if (idx % 4 == 0) cur[idx / 4] = read_op(idx / 4 < 8 ? a : b, idx / 4);
-        if (idx % 8 == 1) asc[idx / 8] = read_scale(at, idx / 8);
-        if (idx % 4 == 2 && idx / 4 < 12) load_data(wrap(over + 1 + idx / 16), 1 + idx / 16, idx / 4 % 4);
-        mfma_fp4_into<1, true>(acc[idx >> 3][idx & 7], nxt[8 + (idx >> 3)], nxt[idx & 7], sc[8 + (idx >> 3)], sc[idx & 7]);
+      for (int idx = 0; idx < 32; ++idx) {
+        const int nb = idx >> 3, mb = idx & 7;
+        if (idx == 6) {
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));
+          __syncthreads();
+          if ((lb & 1) == 0) load_scales();
+        }
+        if (idx >= 8 && idx % 4 == 0) load_data(wrap(over + 1 + (idx - 8) / 8), 1 + (idx - 8) / 8, (idx - 8) / 4 % 2);
+        mfma_fp4_into<1, true>(acc[nb][mb], cur[8 + nb], cur[mb], sc[8 + nb], sc[mb]);
         __builtin_amdgcn_sched_barrier(0);
-        if (idx % 8 == 7) sc[8 + idx / 8] = read_scale(at, 8 + idx / 8);
+        if (nb == 3) cur[mb] = read_op(a, mb), sc[mb] = read_scale(at, mb);
+        if (mb == 7) cur[8 + nb] = read_op(b, 8 + nb), sc[8 + nb] = read_scale(at, 8 + nb);
       }
     }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) sc[r] = asc[r];
     next_scales();
     slot = next;
     advance();
-    // a register that vector code wrote (a copy above) may be an MFMA's operand two wait states later
+    // a register that vector code wrote may be an MFMA's operand two wait states later
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 1");
     __builtin_amdgcn_sched_barrier(0);
   }
 };
 
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) mxfp4_big_kernel(const XArgs xa) {
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) mxfp4_big_kernel(const XArgs xa) {
   using T = BigLoop<9>;
   __shared__ __attribute__((aligned(1024))) char smem[T::RING + 2 * T::SBUF];
   T t(xa, smem);
@@ -752,7 +753,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
     mfma_settle<true>(t.acc);
     int tm, tn;
     grouped_tile(L, t.tmc, t.tnc, tm, tn);
-    store_tile<8, 8>(xa, t.acc, tm * 256 + t.wm * 128, tn * 256 + t.wn * 128, t.li, t.lg);
+    store_tile<4, 8>(xa, t.acc, tm * 256 + t.wm * 128, tn * 256 + t.wn * 64, t.li, t.lg);
     L += t.wgs;
     if (L >= t.end) break;
     t.clear();
@@ -818,7 +819,7 @@ void launch_tiles(XArgs xa, int64_t tiles, hipStream_t s) {
 //   128 x 64      10.3 (9.9)   11.0 (10.3)  21.0 (11.0)  30.6 (11.5)  67   (29.9)  144  (63)
 //   128 x 128     13.1 (12.9)  13.8 (13.3)  15.9 (14.3)  27.5 (14.4)  57.6 (28.2)  105  (46)
 //   128 x 128, 2  14.7 (14.2)  15.4 (14.5)  16.6 (15.2)  22.8 (15.3)  44.2 (21.8)  86   (41)
-//   256 x 256     35.9 (35.4)  36.7 (36.2)  38.5 (37.7)  41.9 (38.3)  45.9 (40.2)  88   (41)
+//   256 x 256     32.3 (31.7)  31.6 (31.9)  34.3 (34.2)  36.5 (35.6)  44.7 (38.4)  81   (42)
 struct TileCost {
   int form, bm, bn, per_cu;
   double one, fill, two;
@@ -827,8 +828,8 @@ constexpr TileCost kTiles[] = {
     {TMHD_MXFP4_64X64, 64, 64, 2, 0.20, 0.03, 0.46},
     {TMHD_MXFP4_128X64, 128, 64, 1, 0.37, 0.02, 0.0},
     {TMHD_MXFP4_128X128, 128, 128, 1, 0.52, 0.10, 0.0},
-    {TMHD_MXFP4_128X128X2, 128, 128, 2, 0.58, 0.08, 1.08},
-    {TMHD_MXFP4_256X256, 256, 256, 1, 1.65, 0.35, 0.0},
+    {TMHD_MXFP4_128X128X2, 128, 128, 2, 0.58, 0.08, 1.12},
+    {TMHD_MXFP4_256X256, 256, 256, 1, 1.32, 0.74, 0.0},
 };
 constexpr double kLaunchUs = 3.5;  // first loads, stores and the launch itself
 
@@ -860,7 +861,7 @@ Form pick_form(int32_t m, int32_t n, int32_t k, int cus) {
   }
   const int64_t tail = big % cus;
   if (big > cus && tail) {
-    const double whole = blocks * (double)(big / cus) * 2.0;
+    const double whole = blocks * (double)(big / cus) * 2.06;
     for (const TileCost &c : kTiles) {
       if (c.form != TMHD_MXFP4_64X64 && c.form != TMHD_MXFP4_128X64 && c.form != TMHD_MXFP4_128X128) continue;
       const double t = kLaunchUs + whole + tiles_us(c, tail * (256 / c.bm) * (256 / c.bn), blocks, cus);
@@ -894,7 +895,7 @@ int launch_product(const char *what, void *out, const uint8_t *a, const uint8_t 
     return set_error(TMHD_ERR_UNSUPPORTED, "%s: %d x %d is too large", what, m, n);
   if (f.tail || f.form == TMHD_MXFP4_256X256) {
     xa.full = (int32_t)(big - f.tail);
-    hipLaunchKernelGGL(mxfp4_big_kernel, dim3((unsigned)std::min<int64_t>(xa.full, cus)), dim3(256), 0, s, xa);
+    hipLaunchKernelGGL(mxfp4_big_kernel, dim3((unsigned)std::min<int64_t>(xa.full, cus)), dim3(512), 0, s, xa);
   }
   switch (f.form) {
     case TMHD_MXFP4_ROWS:

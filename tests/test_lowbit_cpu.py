@@ -191,8 +191,8 @@ def test_mxfp4_forms():
     assert _form(1, 13824, 5120) == n.MXFP4_64X64 and _form(17, 640, 2048) == n.MXFP4_64X64
     assert _form(100, 13824, 5120) == n.MXFP4_128X64 and _form(331, 5376, 5376) == n.MXFP4_128X64
     assert _form(331, 10752, 5376) == n.MXFP4_128X128 and _form(512, 5376, 5376) == n.MXFP4_128X128
-    assert _form(331, 13824, 5120) == n.MXFP4_128X128X2 and _form(2048, 13824, 5120) == n.MXFP4_128X128X2
-    assert _form(12252, 5376, 5376) == n.MXFP4_256X256
+    assert _form(331, 13824, 5120) == n.MXFP4_128X128X2 and _form(1500, 13824, 5120) == n.MXFP4_128X128X2
+    assert _form(12252, 5376, 5376) == n.MXFP4_256X256 and _form(2048, 13824, 5120) == n.MXFP4_256X256
     assert _form(12252, 13824, 5120) in (n.MXFP4_128X64, n.MXFP4_128X128)  # behind ten rounds of 256 x 256
     for bad in ((0, 16, 32), (1, 0, 32), (1, 16, 0), (1, 16, 48)):
         assert _form(*bad) == -1
