@@ -410,6 +410,46 @@ def test_streams_and_graph(torch_mod, dev, rows):
         assert torch.equal(out, step())
 
 
+def test_two_streams_at_once(torch_mod, dev):
+    """Calls over one slot, queued on two streams side by side: their parts do not meet."""
+    from taomate_hd_amd import segment_attention
+
+    torch = torch_mod
+    slot = _slot(torch, *_kv(torch, 9000, 4, 128, 1, dev), "e4m3", dev)
+    queries = [_kv(torch, rows, 4, 128, rows, dev)[0] for rows in (1, 700, 100, 5)]
+    want = [segment_attention(torch, q, [slot.view()], scale=0.1) for q in queries]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for i, q in enumerate(queries):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append((i, segment_attention(torch, q, [slot.view()], scale=0.1)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_end_of_the_longest_slot(torch_mod, dev, fmt):
+    """The last rows of a slot of all the tokens one can hold: codes, scales and values beyond 32-bit offsets."""
+    from taomate_hd_amd import KVSlot8, segment_attention
+    from taomate_hd_amd.slots import MAX_SLOT_CAPACITY, SlotView, expand_views
+
+    torch, heads, dim, n = torch_mod, 5, 128, 130
+    assert MAX_SLOT_CAPACITY * heads * dim > 1 << 32
+    slot = KVSlot8(torch, heads=heads, head_dim=dim, capacity=MAX_SLOT_CAPACITY, device=dev, fmt=fmt)
+    k, v = _kv(torch, n, heads, dim, 3, dev)
+    at = MAX_SLOT_CAPACITY - 192
+    slot.pack(k, v, dst=at)
+    near = _slot(torch, k, v, fmt, dev)
+    view = SlotView(slot, n, at)
+    for a, b in zip(expand_views(torch, [view])[0].slot.token_major(n), near.token_major()):
+        assert torch.equal(a, b)
+    for rows in (2, 300):
+        q = _kv(torch, rows, heads, dim, 4, dev)[0]
+        got = segment_attention(torch, q, [view], scale=0.1)
+        assert torch.equal(got, segment_attention(torch, q, [near.view()], scale=0.1))
+
+
 @pytest.mark.parametrize("backend", ["sdpa", "sage_attn"])
 @pytest.mark.parametrize("storage", FORMATS)
 def test_hook_over_an_8bit_cache(torch_mod, dev, storage, backend):

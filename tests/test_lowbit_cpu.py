@@ -86,6 +86,14 @@ def test_mxfp4_c_entries_refuse():
         assert g(*{**args, **change}.values(), None) == _native.TMHD_ERR_INVALID, change
     assert g(*{**args, "k": 48}.values(), None) == _native.TMHD_ERR_UNSUPPORTED
     assert g(*{**args, "m": 0}.values(), None) == _native.TMHD_OK
+    # more rows than an index or a launch holds
+    most = 2 ** 31 - 1
+    assert q(ok, ok, ok, most - 255, 32, 32, None) == _native.TMHD_ERR_INVALID
+    assert q(ok, ok, ok, most - 256, 32, 32, None) == _native.TMHD_ERR_UNSUPPORTED
+    assert d(ok, ok, ok, most - 256, 32, None) == _native.TMHD_ERR_UNSUPPORTED
+    wide = dict(k=32, lda=16, ldb=16, n=most - 256, ldo=most)
+    assert g(*{**args, **wide, "n": most - 255}.values(), None) == _native.TMHD_ERR_INVALID
+    assert g(*{**args, **wide, "m": 4096}.values(), None) == _native.TMHD_ERR_UNSUPPORTED
 
 
 def _view(**change):
@@ -140,6 +148,10 @@ def test_kv8_attention_c_entry_refuses():
     assert attend(dim=256) == _native.TMHD_ERR_UNSUPPORTED and attend(ws=ok + 4, ws_bytes=64) == inv
     # a long cache is dealt to key ranges: no workspace, no call
     assert attend(view=_view(cap=1 << 20, tokens=1 << 20), heads=1) == inv and "workspace" in lib.tmhd_last_error().decode()
+    # more rows than the merge's launch holds, and more (row tile, block) pairs than an index does
+    uns = _native.TMHD_ERR_UNSUPPORTED
+    assert attend(lq=1 << 22, heads=64, view=_view(tokens=64)) == uns and "too many" in lib.tmhd_last_error().decode()
+    assert attend(lq=1 << 20, heads=32767, view=_view(cap=1 << 22, tokens=1 << 22)) == uns
     assert attend(lq=0) == _native.TMHD_OK
 
 

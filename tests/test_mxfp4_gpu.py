@@ -122,6 +122,49 @@ def test_product_of_views(torch_mod, dev, m):
         assert bool((out == 7.0).all())
 
 
+@pytest.mark.parametrize("m", [256, 300])
+def test_rows_far_apart(torch_mod, dev, m):
+    """Rows 16 MiB apart: offsets just below 2^32 (tiles) and beyond (rows), of codes, of bf16 rows and of outputs."""
+    from taomate_hd_amd import mxfp4_linear, mxfp4_quant, mxfp4_scaled_mm, mxfp4_scaled_mm_out
+
+    torch, n, k, far = torch_mod, 40, 544, 1 << 24
+    a, sa, w, sw, b, want, slack = _product(torch, dev, m, n, k, 21, True)
+    codes = torch.empty(m, far, dtype=torch.uint8, device=dev)[:, : k // 2]
+    codes.copy_(a)
+    got = mxfp4_scaled_mm(codes, w.t(), sa, sw, bias=b)
+    _close(got, want, slack)
+    out = torch.empty(m, far // 2, dtype=torch.bfloat16, device=dev)[:, 8 : 8 + n]
+    mxfp4_scaled_mm_out(out, codes, w.t(), sa, sw, b)
+    assert torch.equal(out, got)
+    weight = torch.empty(m, far, dtype=torch.uint8, device=dev)[:, : k // 2]  # as the other operand
+    weight.copy_(a)
+    _close(mxfp4_scaled_mm(w, weight.t(), sw, sa), (want - _f64(b)).T, slack.T)
+    x = torch.empty(m, far // 2, dtype=torch.bfloat16, device=dev)[:, :k]
+    x.copy_(_rows(torch, m, k, 22, dev))
+    q, scale = mxfp4_quant(x)
+    for got, same in zip((q, scale), mxfp4_quant(x.contiguous())):
+        assert torch.equal(got, same)
+    assert torch.equal(mxfp4_linear(x, w, sw), mxfp4_scaled_mm(q, w.t(), scale, sw))
+
+
+def test_two_streams_at_once(torch_mod, dev):
+    """Projections of other rows on the same weight, queued on two streams side by side."""
+    from taomate_hd_amd import mxfp4_linear, mxfp4_quant
+
+    torch = torch_mod
+    w, ws = mxfp4_quant(_rows(torch, 5376, 1056, 1, dev))
+    rows = [_rows(torch, m, 1056, m, dev) for m in (900, 1, 333, 16)]
+    want = [mxfp4_linear(x, w, ws) for x in rows]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(10):
+        for i, x in enumerate(rows):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append((i, mxfp4_linear(x, w, ws)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in got)
+
+
 def test_product_with_a_nan_block(torch_mod, dev):
     """A block of NaN makes its row (or column) NaN and nothing else."""
     from taomate_hd_amd import mxfp4_quant, mxfp4_scaled_mm
