@@ -155,6 +155,9 @@ typedef struct tmhd_kv8_call {
 int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim, float scale,
                       void *workspace, int64_t workspace_bytes, void *stream);
 int64_t tmhd_attn_kv8_workspace_bytes(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim);
+/* Query rows of the items (32, 128 or 256) that the first launch of these calls is cut into on a device of `cus` CUs
+ * (0: the current device); -1 for calls that are refused. */
+int tmhd_attn_kv8_item_rows(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim, int32_t cus);
 
 #ifdef __cplusplus
 }

@@ -1199,9 +1199,8 @@ struct Plan8 {
 // over 12,000 (41) 34/44, 400 over 12,000 (67) 48/52.
 // A workgroup takes at least 8 blocks (two for each wave that loads blocks of its
 // own) or 4.
-Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, Call8 *out) {
+Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, int64_t cus, Call8 *out) {
   Plan8 p{32, 0, 0, 0, 0};
-  const int64_t cus = std::max(device_cus(), 8);
   int64_t units32 = 0;
   for (int i = 0; i < n; ++i) {
     p.most = std::max(p.most, calls[i].lq);
@@ -1384,6 +1383,13 @@ extern "C" int tmhd_kv8_token_major(const tmhd_kv8_segment *view, void *k, void 
   return check_launch(what);
 }
 
+extern "C" int tmhd_attn_kv8_item_rows(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim, int32_t cus) {
+  using namespace tmhd;
+  const char *what = "tmhd_attn_kv8_item_rows";
+  if (n <= 0 || !calls || check_heads(what, heads, head_dim) || check_calls(what, calls, n)) return -1;
+  return plan(calls, group_end(calls, n, 0), heads, head_dim, cus > 0 ? cus : std::max(device_cus(), 8), nullptr).rows;
+}
+
 extern "C" int64_t tmhd_attn_kv8_workspace_bytes(const tmhd_kv8_call *calls, int32_t n, int32_t heads, int32_t head_dim) {
   using namespace tmhd;
   if (n <= 0 || !calls || check_heads("tmhd_attn_kv8_workspace_bytes", heads, head_dim) ||
@@ -1392,7 +1398,7 @@ extern "C" int64_t tmhd_attn_kv8_workspace_bytes(const tmhd_kv8_call *calls, int
   int64_t most = 0;
   for (int i = 0; i < n;) {
     const int e = group_end(calls, n, i);
-    most = std::max(most, parts_bytes(plan(calls + i, e - i, heads, head_dim, nullptr), head_dim));
+    most = std::max(most, parts_bytes(plan(calls + i, e - i, heads, head_dim, std::max(device_cus(), 8), nullptr), head_dim));
     i = e;
   }
   return most;
@@ -1409,7 +1415,7 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
   for (int i = 0; i < n;) {
     const int e = group_end(calls, n, i);
     Args8 aa{};
-    const Plan8 p = plan(calls + i, e - i, heads, head_dim, aa.call);
+    const Plan8 p = plan(calls + i, e - i, heads, head_dim, std::max(device_cus(), 8), aa.call);
     // (the merge's workgroups, 1024 / head_dim rows each, within what a launch holds)
     if (p.units > INT32_MAX || p.items * (p.rows * head_dim / 1024) >= 1 << 24)
       return set_error(TMHD_ERR_UNSUPPORTED, "%s: too many query rows and keys", what);

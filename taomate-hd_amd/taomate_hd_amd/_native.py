@@ -288,6 +288,7 @@ _LOWBIT_SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         c_int, [POINTER(KV8Call), c_int32, c_int32, c_int32, c_float, c_void_p, c_int64, c_void_p],
     ),
     "tmhd_attn_kv8_workspace_bytes": (c_int64, [POINTER(KV8Call), c_int32, c_int32, c_int32]),
+    "tmhd_attn_kv8_item_rows": (c_int, [POINTER(KV8Call), c_int32, c_int32, c_int32, c_int32]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)  # of include/tmhd.h

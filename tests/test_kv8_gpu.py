@@ -139,24 +139,25 @@ def test_expand_of_more_rows_than_a_slot_holds(torch_mod, dev, monkeypatch):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_blocks_without_finite_values(torch_mod, dev, fmt):
+@pytest.mark.parametrize("rows,heads,dim,items", [(1, 4, 64, 32), (40, 4, 64, 32), (100, 1900, 64, 128), (200, 1100, 64, 256), (300, 400, 128, 256)])
+def test_blocks_without_finite_values(torch_mod, dev, rows, heads, dim, items, fmt):
     """An infinity or NaN makes its block and head NaN, in every reader, and nothing else."""
     from taomate_hd_amd import segment_attention
     from taomate_hd_amd.slots import expand_views
 
     torch = torch_mod
-    k, v = _kv(torch, 200, 4, 64, 1, dev)
+    assert _item_rows(heads, dim, (rows, [200])) == items
+    k, v = _kv(torch, 200, heads, dim, 1, dev)
     k[70, 1, 3], v[130, 2, 60] = float("inf"), float("nan")
     slot = _slot(torch, k, v, fmt, dev)
     nan = [torch.isnan(t) for t in slot.token_major()]
-    assert int(nan[0].sum()) == 64 * 64 == int(nan[0][64:128, 1].sum())
-    assert int(nan[1].sum()) == 64 * 64 == int(nan[1][128:192, 2].sum())
+    assert int(nan[0].sum()) == 64 * dim == int(nan[0][64:128, 1].sum())
+    assert int(nan[1].sum()) == 64 * dim == int(nan[1][128:192, 2].sum())
     big = expand_views(torch, [slot.view()])[0].slot
-    assert int(torch.isnan(big.k).sum()) == 64 * 64 == int(torch.isnan(big.vt).sum())
-    for rows in (1, 40, 200):
-        q = _kv(torch, rows, 4, 64, 2, dev)[0]
-        bad = torch.isnan(segment_attention(torch, q, [slot.view()], scale=0.125))
-        assert bool(bad[:, 1:3].all()) and not bool(bad[:, [0, 3]].any())
+    assert int(torch.isnan(big.k).sum()) == 64 * dim == int(torch.isnan(big.vt).sum())
+    q = _kv(torch, rows, heads, dim, 2, dev)[0]
+    bad = torch.isnan(segment_attention(torch, q, [slot.view()], scale=0.125))
+    assert bool(bad[:, 1:3].all()) and not bool(bad[:, 0].any()) and not bool(bad[:, 3:].any())
 
 
 def _want(q, segments, scale):
@@ -176,10 +177,27 @@ def _want(q, segments, scale):
     return want, HALF_BF16 * np.abs(want) + 1.02 * weight * size + lost
 
 
+def _item_rows(heads, dim, *calls):
+    """Rows of the items that calls of (rows, segment lengths) are cut into: which kernel they run."""
+    from taomate_hd_amd import _native
+
+    table = (_native.KV8Call * len(calls))()
+    for c, (rows, sizes) in zip(table, calls):
+        c.q, c.o, c.q_token_stride, c.q_head_stride, c.o_token_stride, c.o_head_stride = 4096, 4096, 128, 64, 128, 64
+        c.lq, c.n_segments = rows, len(sizes)
+        for i, n in enumerate(sizes):
+            c.seg[i] = _native.KV8Segment(4096, 4096, 4096, 4096, -(-n // 64) * 64, 0, n, 0)
+    return _native.load().tmhd_attn_kv8_item_rows(table, len(calls), heads, dim, 0)
+
+
+# (rows, heads) whose calls over two blocks take each kernel: a head size of 64, and of 128
+KERNELS = [(3, 2, 64, 32), (100, 3700, 64, 128), (200, 2200, 64, 256), (90, 2500, 128, 128), (300, 800, 128, 256)]
 CASES = [(1, 1, 64, [1]), (1, 3, 128, [33]), (5, 2, 64, [64, 1, 130]), (32, 4, 128, [500]), (33, 2, 128, [65]),
          (64, 3, 64, [1000, 70]), (1, 14, 128, [9000, 777, 64]), (17, 1, 128, [20000]), (40, 1, 128, [30]),
          (100, 5, 128, [64, 700, 33]), (128, 2, 64, [2000]), (129, 3, 128, [1]), (300, 2, 64, [65, 128]),
-         (256, 9, 128, [500, 640]), (700, 1, 128, [5000, 64])]
+         (256, 9, 128, [500, 640]), (700, 1, 128, [5000, 64]), (33, 7300, 64, [65]), (128, 2600, 128, [1, 64]),
+         (97, 40, 128, [6000, 65, 200]), (129, 1000, 128, [65, 1]), (257, 12, 128, [9000, 130, 64, 63]),
+         (513, 3, 64, [17000, 20000])]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -288,6 +306,43 @@ def test_batch_of_unlike_calls(torch_mod, dev, fmt):
     assert bool((out[:, :heads] == 7.0).all()) and bool((o[~touched.to(dev)] == 7.0).all())
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,lengths,items", [(3, (100, 60, 5), 32), (830, (100, 60, 5), 128), (520, (200, 140, 5), 256)])
+def test_batch_in_each_kernel(torch_mod, dev, heads, lengths, items, fmt):
+    """Rows by range and by list (one of them twice in the queries), views inside a slot, strided queries and outputs,
+    a call without rows: rows that belong to no call stay."""
+    from taomate_hd_amd import AttentionCall, segment_attention_batch
+    from taomate_hd_amd.slots import SlotView
+
+    torch, dim = torch_mod, 64
+    sizes = ([130, 60], [150], [300, 150, 300])
+    assert _item_rows(heads, dim, *zip(lengths, sizes)) == items
+    a = _slot(torch, *_kv(torch, 300, heads, dim, 1, dev), fmt, dev)
+    b = _slot(torch, *_kv(torch, 150, heads, dim, 2, dev), fmt, dev)
+    q = _kv(torch, 420, 2 * heads, dim, 4, dev)[0][:, heads:]
+    out = torch.full((420, heads, dim), 7.0, dtype=torch.bfloat16, device=dev)
+    order = torch.randperm(100, generator=torch.Generator().manual_seed(1)) + 10
+    take = torch.cat([order, order])[: lengths[1]].to(dev)
+    put = (torch.randperm(lengths[1], generator=torch.Generator().manual_seed(2)) + 215).to(dev)
+    n = lengths[0]
+    plan = [
+        (AttentionCall(q, [SlotView(a, 130, 64), SlotView(a, 60, 192)], q_row0=1, lq=n, out=out, o_row0=2), q[1 : n + 1],
+         range(2, n + 2)),
+        (AttentionCall(q, [b.view()], q_rows=take, out=out, o_rows=put), q[take], put.tolist()),
+        (AttentionCall(q, [b.view()], lq=0, out=out), q[:0], ()),
+        (AttentionCall(q, [a.view(), b.view(), a.view()], q_row0=415, lq=5, out=out, o_row0=400), q[415:], range(400, 405)),
+    ]
+    segment_attention_batch(torch, [call for call, *_ in plan], scale=0.125)
+    touched = torch.zeros(420, dtype=torch.bool)
+    for call, rows, where in plan:
+        where = list(where)
+        touched[where] = True
+        if where:
+            want, bound = _want(rows, call.segments, 0.125)
+            assert (np.abs(_f64(out[where]) - want) <= bound).all()
+    assert bool((out[~touched.to(dev)] == 7.0).all())
+
+
 def test_more_calls_than_one_launch(torch_mod, dev):
     from taomate_hd_amd import AttentionCall, segment_attention, segment_attention_batch
 
@@ -304,47 +359,50 @@ def test_more_calls_than_one_launch(torch_mod, dev):
         assert (np.abs(_f64(again) - want) <= bound).all()
 
 
-@pytest.mark.parametrize("rows,dim", [(20, 128), (90, 128), (300, 128), (150, 64)])
-def test_large_scores_move_the_running_maximum(torch_mod, dev, rows, dim):
+@pytest.mark.parametrize("rows,heads,dim,items", [(20, 2, 128, 32), (90, 210, 128, 128), (300, 64, 128, 256), (150, 256, 64, 256)])
+def test_large_scores_move_the_running_maximum(torch_mod, dev, rows, heads, dim, items):
     from taomate_hd_amd import segment_attention
 
     torch = torch_mod
-    k, v = _kv(torch, 1500, 2, dim, 1, dev)
+    assert _item_rows(heads, dim, (rows, [1500])) == items
+    k, v = _kv(torch, 1500, heads, dim, 1, dev)
     k = k * torch.linspace(0.1, 6.0, 1500, device=dev).view(-1, 1, 1).to(torch.bfloat16)
     slot = _slot(torch, k, v, "int8", dev)
-    q = 8 * _kv(torch, rows, 2, dim, 2, dev)[0]
+    q = 8 * _kv(torch, rows, heads, dim, 2, dev)[0]
     got = segment_attention(torch, q, [slot.view()], scale=dim ** -0.5)
     want, bound = _want(q, [slot.view()], dim ** -0.5)
     assert (np.abs(_f64(got) - want) <= bound).all()
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("rows", [1, 33, 200])
-def test_values_behind_a_view_that_overflow(torch_mod, dev, rows, fmt):
+@pytest.mark.parametrize("rows,heads,dim,items", KERNELS)
+def test_values_behind_a_view_that_overflow(torch_mod, dev, rows, heads, dim, items, fmt):
     """Rows of the view's last block that it does not hold: their scores are infinite, their weights nothing."""
     from taomate_hd_amd import segment_attention
     from taomate_hd_amd.slots import SlotView
 
     torch = torch_mod
-    k, v = _kv(torch, 192, 2, 64, 1, dev)
+    assert _item_rows(heads, dim, (rows, [70])) == items
+    k, v = _kv(torch, 192, heads, dim, 1, dev)
     k[70:], v[70:] = 2.0 ** 100, 2.0 ** 100
     slot = _slot(torch, k, v, fmt, dev)
-    q = 2.0 ** 40 * _kv(torch, rows, 2, 64, 2, dev)[0].abs()
-    for view in (SlotView(slot, 70, 0), SlotView(slot, 6, 64)):
+    q = 2.0 ** 40 * _kv(torch, rows, heads, dim, 2, dev)[0].abs()
+    for view in (SlotView(slot, 70, 0), SlotView(slot, 6, 64)):  # (of two blocks, and of one)
         got = segment_attention(torch, q, [view], scale=2.0 ** -43)
         want, bound = _want(q, [view], 2.0 ** -43)
         assert (np.abs(_f64(got) - want) <= bound).all()
 
 
-@pytest.mark.parametrize("rows", [3, 33, 200])
+@pytest.mark.parametrize("rows,heads,dim,items", KERNELS)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 40.0])
-def test_any_softmax_scale(torch_mod, dev, scale, rows):
+def test_any_softmax_scale(torch_mod, dev, scale, rows, heads, dim, items):
     """No scale (the mean of the values), a negative, a vanishing and a large one, with a ragged last tile."""
     from taomate_hd_amd import segment_attention
 
     torch = torch_mod
-    slot = _slot(torch, *_kv(torch, 71, 2, 64, 1, dev), "int8", dev)
-    q = _kv(torch, rows, 2, 64, 2, dev)[0]
+    assert _item_rows(heads, dim, (rows, [71])) == items
+    slot = _slot(torch, *_kv(torch, 71, heads, dim, 1, dev), "int8", dev)
+    q = _kv(torch, rows, heads, dim, 2, dev)[0]
     got = segment_attention(torch, q, [slot.view()], scale=scale)
     want, bound = _want(q, [slot.view()], scale)
     assert (np.abs(_f64(got) - want) <= bound).all()
@@ -378,15 +436,16 @@ def test_refusals(torch_mod, dev):
         slot.view().to_segment()
 
 
-@pytest.mark.parametrize("rows", [2, 100, 400])
-def test_streams_and_graph(torch_mod, dev, rows):
+@pytest.mark.parametrize("rows,heads,items", [(2, 4, 32), (100, 48, 128), (400, 48, 256)])
+def test_streams_and_graph(torch_mod, dev, rows, heads, items):
     """A pack and a decode call on another stream, and captured and replayed with new K/V between eager calls."""
     from taomate_hd_amd import KVSlot8, segment_attention
 
     torch = torch_mod
-    slot = KVSlot8(torch, heads=4, head_dim=128, capacity=5000, device=dev)
-    k, v = _kv(torch, 5000, 4, 128, 1, dev)
-    q = _kv(torch, rows, 4, 128, 2, dev)[0]
+    assert _item_rows(heads, 128, (rows, [5000])) == items
+    slot = KVSlot8(torch, heads=heads, head_dim=128, capacity=5000, device=dev)
+    k, v = _kv(torch, 5000, heads, 128, 1, dev)
+    q = _kv(torch, rows, heads, 128, 2, dev)[0]
 
     def step():
         slot.pack(k, v)
@@ -403,7 +462,7 @@ def test_streams_and_graph(torch_mod, dev, rows):
     with torch.cuda.graph(graph):
         out = step()
     for seed in (5, 6, 7):
-        nk, nv = _kv(torch, 5000, 4, 128, seed, dev)
+        nk, nv = _kv(torch, 5000, heads, 128, seed, dev)
         k.copy_(nk), v.copy_(nv)
         graph.replay()
         torch.cuda.synchronize()
@@ -415,8 +474,8 @@ def test_two_streams_at_once(torch_mod, dev):
     from taomate_hd_amd import segment_attention
 
     torch = torch_mod
-    slot = _slot(torch, *_kv(torch, 9000, 4, 128, 1, dev), "e4m3", dev)
-    queries = [_kv(torch, rows, 4, 128, rows, dev)[0] for rows in (1, 700, 100, 5)]
+    slot = _slot(torch, *_kv(torch, 9000, 8, 128, 1, dev), "e4m3", dev)
+    queries = [_kv(torch, rows, 8, 128, rows, dev)[0] for rows in (1, 700, 100, 5)]
     want = [segment_attention(torch, q, [slot.view()], scale=0.1) for q in queries]
     torch.cuda.synchronize()
     streams, got = [torch.cuda.Stream() for _ in range(2)], []
@@ -434,17 +493,18 @@ def test_end_of_the_longest_slot(torch_mod, dev, fmt):
     from taomate_hd_amd import KVSlot8, segment_attention
     from taomate_hd_amd.slots import MAX_SLOT_CAPACITY, SlotView, expand_views
 
-    torch, heads, dim, n = torch_mod, 5, 128, 130
+    torch, heads, dim, n = torch_mod, 5, 128, 46010
     assert MAX_SLOT_CAPACITY * heads * dim > 1 << 32
     slot = KVSlot8(torch, heads=heads, head_dim=dim, capacity=MAX_SLOT_CAPACITY, device=dev, fmt=fmt)
     k, v = _kv(torch, n, heads, dim, 3, dev)
-    at = MAX_SLOT_CAPACITY - 192
+    at = MAX_SLOT_CAPACITY - 46016
     slot.pack(k, v, dst=at)
     near = _slot(torch, k, v, fmt, dev)
     view = SlotView(slot, n, at)
     for a, b in zip(expand_views(torch, [view])[0].slot.token_major(n), near.token_major()):
         assert torch.equal(a, b)
-    for rows in (2, 300):
+    for rows, items in ((2, 32), (128, 128), (300, 256)):
+        assert _item_rows(heads, dim, (rows, [n])) == items
         q = _kv(torch, rows, heads, dim, 4, dev)[0]
         got = segment_attention(torch, q, [view], scale=0.1)
         assert torch.equal(got, segment_attention(torch, q, [near.view()], scale=0.1))

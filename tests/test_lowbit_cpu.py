@@ -208,3 +208,24 @@ def test_mxfp4_forms():
     assert _form(12252, 13824, 5120) in (n.MXFP4_128X64, n.MXFP4_128X128)  # behind ten rounds of 256 x 256
     for bad in ((0, 16, 32), (1, 0, 32), (1, 16, 0), (1, 16, 48)):
         assert _form(*bad) == -1
+
+
+def test_kv8_item_rows():
+    """The rule's choices at sizes whose forms were all timed (256 CUs), and for calls that are refused."""
+    from taomate_hd_amd import _native
+
+    def rows(lq, heads, tokens, dim=128, calls=1, **change):
+        cap = -(-tokens // 64) * 64
+        c = _native.KV8Call(q=4096, q_token_stride=128, q_head_stride=64, lq=lq, o=4096, o_token_stride=128,
+                            o_head_stride=64, n_segments=1)
+        c.seg[0] = _view(cap=cap, tokens=tokens, **change)
+        return _native.load().tmhd_attn_kv8_item_rows((_native.KV8Call * calls)(*[c] * calls), calls, heads, dim, 256)
+
+    assert rows(1, 14, 40788) == rows(32, 40, 100000) == 32
+    assert rows(256, 14, 2800) == rows(400, 40, 1500) == rows(128, 14, 12000) == 32
+    assert rows(91, 40, 12000) == rows(128, 14, 41000) == 128
+    assert rows(256, 40, 6000) == rows(1024, 14, 41000) == 256
+    assert rows(300, 14, 11000, dim=64) == 32 and rows(300, 14, 41000, dim=64) == 256
+    assert rows(100, 14, 2800, calls=12) == 128  # (together as large as one long call)
+    assert rows(0, 14, 2800) == 32 and rows(-1, 14, 2800) == -1 and rows(1, 14, 2800, dim=96) == -1
+    assert rows(1, 0, 2800) == -1 and rows(1, 14, 2800, row0=32) == -1
