@@ -293,6 +293,7 @@ struct Args8 {
   Seg8 seg[kMaxSegs];
   int32_t n_calls, heads;
   int32_t units, wgs;  // the launch's units of work, and the workgroups they are dealt to
+  int32_t whole;       // an item to a workgroup
   float scale2;        // |softmax scale| times log2 e
   int32_t flip;        // sign bits to change in Q: a negative scale's
   float *ws;
@@ -300,10 +301,17 @@ struct Args8 {
 
 // The work is one item per (call, head, tile of query rows), of its call's 64-token
 // blocks each; the items' blocks in a row are dealt evenly to the workgroups,
-// which so all end at about the same time.  An item that lies in one workgroup's
+// which so all end at about the same time (short items of 32 rows go whole to one each:
+// kWholeBlocks).  An item that lies in one workgroup's
 // range is written out; the parts of a cut one go to ws, two slots a workgroup
 // (its range may begin and end inside an item), and are merged afterwards.
 __device__ __forceinline__ int range_begin(const Args8 &aa, int wg) { return (int)((int64_t)aa.units * wg / aa.wgs); }
+// First unit of item `item` of the launch, all of its units for the item behind the last
+__device__ __forceinline__ int item_begin(const Args8 &aa, int item) {
+  int ci = 0;
+  while (ci < aa.n_calls && item >= aa.heads * aa.call[ci].row_tiles) item -= aa.heads * aa.call[ci++].row_tiles;
+  return ci < aa.n_calls ? aa.call[ci].first + item * aa.call[ci].blocks : aa.units;
+}
 
 // The range of a workgroup where neighbouring ranges share keys: runs on one XCD
 __device__ __forceinline__ int xcd_wg(int wgs) {
@@ -417,7 +425,8 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
   __shared__ __attribute__((aligned(16))) float stage[kWaves8 * 32 * RS];
   __shared__ float stat[2][kWaves8][32];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, g = lane >> 5;
-  const int x0 = range_begin(aa, blockIdx.x), end = range_begin(aa, blockIdx.x + 1);
+  const int x0 = aa.whole ? item_begin(aa, blockIdx.x) : range_begin(aa, blockIdx.x);
+  const int end = aa.whole ? item_begin(aa, blockIdx.x + 1) : range_begin(aa, blockIdx.x + 1);
   for (int x = x0; x < end;) {
     const Piece pc = piece_at(aa, x, end);
     const Call8 &cl = aa.call[pc.call];
@@ -1181,12 +1190,19 @@ int blocks_of(const tmhd_kv8_call &c) {
   return (int)std::min<int64_t>(b, INT32_MAX);
 }
 
+// Items of 32 rows of up to so many blocks go to a workgroup whole: nothing to merge, a
+// launch and a workspace less.  us, whole against dealt evenly: 14 heads of 128, 1 row
+// over 700 tokens (11 blocks) 17.7/22.4, 2,717 (43) 19.7/22.5, 5,000 (79) 29.6/21.7; 40
+// heads, 3 calls of 20 rows over 2,717 32.5/37.7.
+constexpr int kWholeBlocks = 48;
+
 // Rows of an item, the units of work (item, block) and the workgroups they are dealt to.
 struct Plan8 {
   int rows;
   int64_t items, units;
   int wgs;
-  int most;  // query rows of the longest call
+  int most;    // query rows of the longest call
+  bool whole;  // an item to a workgroup, nothing to merge
 };
 
 // The calls of one launch: items of 32 rows (two workgroups a CU) for up to 32 rows, or
@@ -1200,10 +1216,12 @@ struct Plan8 {
 // A workgroup takes at least 8 blocks (two for each wave that loads blocks of its
 // own) or 4.
 Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, int64_t cus, Call8 *out) {
-  Plan8 p{32, 0, 0, 0, 0};
+  Plan8 p{32, 0, 0, 0, 0, false};
+  int longest = 0;  // blocks of an item
   int64_t units32 = 0;
   for (int i = 0; i < n; ++i) {
     p.most = std::max(p.most, calls[i].lq);
+    longest = std::max(longest, calls[i].lq > 0 ? blocks_of(calls[i]) : 0);
     units32 += (int64_t)heads * (((int64_t)calls[i].lq + 31) / 32) * blocks_of(calls[i]);
   }
   p.rows = p.most <= 32 || units32 <= 2 * cus * 28 * 128 / D ? 32 : p.most <= 128 ? 128 : 256;
@@ -1217,8 +1235,10 @@ Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, int64_t cus, Cal
     p.units += (int64_t)heads * c.row_tiles * c.blocks;
     if (out) out[i] = c;
   }
+  p.whole = p.rows == 32 && longest <= kWholeBlocks;
   const int64_t room = cus * (p.rows == 256 ? 1 : 2), least = p.rows == 32 ? 2 * kWaves8 : 4;
   p.wgs = (int)std::min<int64_t>(room, (p.units + least - 1) / least);
+  if (p.whole) p.wgs = (int)std::min<int64_t>(p.items, INT32_MAX);
   return p;
 }
 
@@ -1252,7 +1272,7 @@ int check_calls(const char *what, const tmhd_kv8_call *calls, int n) {
 
 template <int D, int ROWS>
 void launch_merge(const Args8 &aa, const Plan8 &p, hipStream_t s) {
-  if (p.wgs <= 1) return;
+  if (p.wgs <= 1 || p.whole) return;
   const int rows = std::min(p.most, ROWS);
   // Items of many parts: a row to a workgroup, its parts shared by 1024 / D threads; else
   // 1024 / D rows to a workgroup.  Whole call of 14 heads of 128 over 40,788 tokens (36
@@ -1282,7 +1302,7 @@ void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
 }
 
 // two slots for each workgroup (none if one takes all)
-int64_t parts_bytes(const Plan8 &p, int D) { return p.wgs > 1 ? (int64_t)p.wgs * 2 * p.rows * (D + 2) * 4 : 0; }
+int64_t parts_bytes(const Plan8 &p, int D) { return p.wgs > 1 && !p.whole ? (int64_t)p.wgs * 2 * p.rows * (D + 2) * 4 : 0; }
 
 }  // namespace
 }  // namespace tmhd
@@ -1424,7 +1444,7 @@ extern "C" int tmhd_attn_fwd_kv8(const tmhd_kv8_call *calls, int32_t n, int32_t 
                        (long long)parts_bytes(p, head_dim));
     aa.n_calls = e - i;
     aa.heads = heads;
-    aa.units = (int32_t)p.units, aa.wgs = p.wgs;
+    aa.units = (int32_t)p.units, aa.wgs = p.wgs, aa.whole = p.whole;
     aa.scale2 = fabsf(scale) * 1.4426950408889634f;
     aa.flip = scale < 0.f ? (int32_t)0x80008000u : 0;
     aa.ws = (float *)workspace;

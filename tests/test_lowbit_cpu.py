@@ -229,3 +229,17 @@ def test_kv8_item_rows():
     assert rows(100, 14, 2800, calls=12) == 128  # (together as large as one long call)
     assert rows(0, 14, 2800) == 32 and rows(-1, 14, 2800) == -1 and rows(1, 14, 2800, dim=96) == -1
     assert rows(1, 0, 2800) == -1 and rows(1, 14, 2800, row0=32) == -1
+
+
+def test_kv8_workspace():
+    """Short items of 32 rows are not cut, longer ones are."""
+    from taomate_hd_amd import _native
+
+    def need(lq, tokens, heads=14):
+        c = _native.KV8Call(q=4096, q_token_stride=128, q_head_stride=64, lq=lq, o=4096, o_token_stride=128,
+                            o_head_stride=64, n_segments=1)
+        c.seg[0] = _view(cap=1 << 16, tokens=tokens)
+        return _native.load().tmhd_attn_kv8_workspace_bytes((_native.KV8Call * 1)(c), 1, heads, 128)
+
+    assert need(1, 1) == need(32, 48 * 64) == need(0, 60000) == need(-1, 64) == 0
+    assert need(1, 48 * 64 + 1) > 0 and need(40, 60000) > 0
