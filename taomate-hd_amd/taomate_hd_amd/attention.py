@@ -274,9 +274,11 @@ class AttentionCall:
     rows_checked: bool = False
 
 
-def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: list[Any]) -> tuple[Any, list[SlotView]]:
+def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: list[Any],
+               new: Any | None = None) -> tuple[Any, list[SlotView]]:
     """Check one call and fill its C arguments (``AttnArgs``, or ``KV8Call`` for
-    8-bit segments read in place); returns its output and segments."""
+    8-bit segments read in place); returns its output (``new``, if it fits a
+    call without one) and segments."""
     query, out, q_rows, o_rows, lq = call.query, call.out, call.q_rows, call.o_rows, call.lq
     q_row0, o_row0 = int(call.q_row0), int(call.o_row0)
     _validate_tokens_major(torch, query, "query")
@@ -293,7 +295,9 @@ def _call_args(torch: Any, call: AttentionCall, args: Any, scale: float, keep: l
         lq = rows_in - q_row0
     lq = int(lq)
     if out is None:
-        out = torch.empty((lq, heads, head_dim), dtype=torch.bfloat16, device=device)
+        out = new
+        if out is None or out.shape != (lq, heads, head_dim):
+            out = torch.empty((lq, heads, head_dim), dtype=torch.bfloat16, device=device)
         o_rows, o_row0 = None, 0
     else:
         _validate_tokens_major(torch, out, "out")
@@ -366,12 +370,23 @@ def _in_place_formats(calls: Sequence[AttentionCall]) -> list[str | None]:
     return [_in_place_format(call) if n <= KV8_ROWS or work <= KV8_WORK else None for n, call in zip(rows, calls)]
 
 
+def _new_outputs(calls: Sequence[AttentionCall]) -> dict[int, Any]:
+    """The outputs of calls that bring none, side by side in one allocation (1.7 us of host time each)."""
+    at = [i for i, call in enumerate(calls) if call.out is None]
+    rows = [_call_rows(calls[i]) for i in at]
+    if len(at) < 2 or min(rows) < 0:
+        return {}
+    query = calls[at[0]].query
+    return dict(zip(at, query.new_empty((sum(rows), *query.shape[1:])).split(rows)))
+
+
 def _attend_in_place(torch: Any, calls: Sequence[AttentionCall], scale: float, timer: ComponentTimer | None) -> list[Any]:
     """Calls over 8-bit segments of one format, in one launch (per 16 calls and 24 segments)."""
     keep: list[Any] = []
     n = len(calls)
     args = (_native.KV8Call * n)()
-    outs = [_call_args(torch, call, args[i], scale, keep)[0] for i, call in enumerate(calls)]
+    new = _new_outputs(calls)
+    outs = [_call_args(torch, call, args[i], scale, keep, new.get(i))[0] for i, call in enumerate(calls)]
     query = calls[0].query
     device, shape = query.device, query.shape[1:]
     for call, out in zip(calls, outs):
@@ -433,7 +448,8 @@ def segment_attention_batch(
     attention, or a packed sequence's documents, none of which alone fills the
     GPU's last round of workgroups.  The calls share heads, head_dim and the
     query and output strides; their output rows must not overlap.  Returns
-    their outputs, and with ``return_quant`` the INT8-QK operand views."""
+    their outputs (those of a batch over 8-bit segments may lie in one
+    allocation), and with ``return_quant`` the INT8-QK operand views."""
     if backend not in BACKENDS:
         raise ValueError(f"unknown attention backend {backend!r}")
     if not calls:
