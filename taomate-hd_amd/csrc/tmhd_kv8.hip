@@ -407,10 +407,8 @@ __device__ __forceinline__ int in_branch(int keys) {
   return keys;
 }
 
-constexpr int kWaves8 = 4;
-
-// 32 query rows an item.  The four waves of a workgroup take an item's
-// blocks in turn and merge through LDS.  Per 32 keys a lane loads the 16-byte
+// 32 query rows an item.  The W waves of a workgroup take an item's blocks in
+// turn and merge through LDS.  Per 32 keys a lane loads the 16-byte
 // chunks that are its MFMA operands (no LDS on the way: each code is used once)
 // and turns them into bf16, exactly; S^T = K Q^T leaves 16 keys of one query in a
 // lane, in the order in which the V chunks hold them, so P feeds the second
@@ -418,12 +416,12 @@ constexpr int kWaves8 = 4;
 // the conversion (e4m3) or P (int8).  Bound by HBM over a long cache: two waves a SIMD
 // keep two tiles each in flight.  One row of 14 heads of 128 over 40,788 tokens, e4m3: 26
 // to 28 us (5.2 to 5.6 TB/s), 36 with the merge and the launches.
-template <int D, bool E4M3>
-__global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_rows_kernel(const Args8 aa) {
+template <int D, int W, bool E4M3>
+__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_rows_kernel(const Args8 aa) {
   constexpr int KC = D / 32;  // 16-byte K chunks of a lane per 32 keys, and V chunks (32-channel blocks)
   constexpr int RS = D + 4;   // floats of a staged row
-  __shared__ __attribute__((aligned(16))) float stage[kWaves8 * 32 * RS];
-  __shared__ float stat[2][kWaves8][32];
+  __shared__ __attribute__((aligned(16))) float stage[W * 32 * RS];
+  __shared__ float stat[2][W][32];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, g = lane >> 5;
   const int x0 = aa.whole ? item_begin(aa, blockIdx.x) : range_begin(aa, blockIdx.x);
   const int end = aa.whole ? item_begin(aa, blockIdx.x + 1) : range_begin(aa, blockIdx.x + 1);
@@ -474,7 +472,7 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
       if (t == 0 && left > 32) {
         t = 1, left -= 32, kp += 32 * D, vp += 32 * D;
       } else {
-        b += kWaves8;
+        b += W;
         if (b < pc.b_end) locate();
       }
       f32x16 s;
@@ -545,7 +543,7 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
       for (int j = 0; j < KC; ++j) vr[j] = *(const i32x4 *)(vp + j * 1024);
     }
 
-    // merge of the four waves, in wave order
+    // merge of the waves, in their order
     const float l = sum + __shfl_xor(sum, 32);
     if (g == 0) stat[0][w][lr] = mx, stat[1][w][lr] = l;
 #pragma unroll
@@ -555,14 +553,14 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
         *(f32x4 *)&stage[(w * 32 + lr) * RS + d * 32 + 8 * u + 4 * g] =
             f32x4{acc[d][4 * u], acc[d][4 * u + 1], acc[d][4 * u + 2], acc[d][4 * u + 3]};
     __syncthreads();
-    // thread: row tid / 8, channels 4 (tid % 8) + 32 j ..
-    const int r = threadIdx.x >> 3, dq = threadIdx.x & 7, row = r0 + r;
+    // thread: row tid / 2 W, channels 4 (tid % 2 W) + 8 W j ..
+    const int r = threadIdx.x / (2 * W), dq = threadIdx.x % (2 * W), row = r0 + r;
     if (row < cl.lq) {
-      float m = stat[0][0][r], f[kWaves8], ls = 0.f;
+      float m = stat[0][0][r], f[W], ls = 0.f;
 #pragma unroll
-      for (int i = 1; i < kWaves8; ++i) m = fmaxf(m, stat[0][i][r]);
+      for (int i = 1; i < W; ++i) m = fmaxf(m, stat[0][i][r]);
 #pragma unroll
-      for (int i = 0; i < kWaves8; ++i) {
+      for (int i = 0; i < W; ++i) {
         // a wave without blocks has the reference -inf and sums 0
         f[i] = stat[0][i][r] == m ? 1.0f : __builtin_amdgcn_exp2f(stat[0][i][r] - m);
         ls += f[i] * stat[1][i][r];
@@ -578,11 +576,11 @@ __global__ void __launch_bounds__(kWaves8 * 64) __attribute__((amdgpu_waves_per_
         ws[32 * (D + 1) + r] = ls;
       }
 #pragma unroll
-      for (int j = 0; j < KC; ++j) {
-        const int d = 32 * j + 4 * dq;
+      for (int j = 0; j < D / (8 * W); ++j) {
+        const int d = 8 * W * j + 4 * dq;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kWaves8; ++i) v += f[i] * *(const f32x4 *)&stage[(i * 32 + r) * RS + d];
+        for (int i = 0; i < W; ++i) v += f[i] * *(const f32x4 *)&stage[(i * 32 + r) * RS + d];
         if (op)
           *(i32x2 *)(op + d) = pack4(v, inv);
         else
@@ -1193,7 +1191,9 @@ int blocks_of(const tmhd_kv8_call &c) {
 // Items of 32 rows of up to so many blocks go to a workgroup whole: nothing to merge, a
 // launch and a workspace less.  us, whole against dealt evenly: 14 heads of 128, 1 row
 // over 700 tokens (11 blocks) 17.7/22.4, 2,717 (43) 19.7/22.5, 5,000 (79) 29.6/21.7; 40
-// heads, 3 calls of 20 rows over 2,717 32.5/37.7.
+// heads, 3 calls of 20 rows over 2,717 32.5/37.7.  Of eight waves where there are no more
+// of them than CUs (against four: 14 heads, 200 rows over 2,717 18.2/21.9, 40 heads, 1
+// row 21.0/24.9; but 400 items 44.3/37.5).
 constexpr int kWholeBlocks = 48;
 
 // Rows of an item, the units of work (item, block) and the workgroups they are dealt to.
@@ -1203,6 +1203,7 @@ struct Plan8 {
   int wgs;
   int most;    // query rows of the longest call
   bool whole;  // an item to a workgroup, nothing to merge
+  bool eight;  // of eight waves
 };
 
 // The calls of one launch: items of 32 rows (two workgroups a CU) for up to 32 rows, or
@@ -1216,7 +1217,7 @@ struct Plan8 {
 // A workgroup takes at least 8 blocks (two for each wave that loads blocks of its
 // own) or 4.
 Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, int64_t cus, Call8 *out) {
-  Plan8 p{32, 0, 0, 0, 0, false};
+  Plan8 p{32, 0, 0, 0, 0, false, false};
   int longest = 0;  // blocks of an item
   int64_t units32 = 0;
   for (int i = 0; i < n; ++i) {
@@ -1236,9 +1237,9 @@ Plan8 plan(const tmhd_kv8_call *calls, int n, int heads, int D, int64_t cus, Cal
     if (out) out[i] = c;
   }
   p.whole = p.rows == 32 && longest <= kWholeBlocks;
-  const int64_t room = cus * (p.rows == 256 ? 1 : 2), least = p.rows == 32 ? 2 * kWaves8 : 4;
+  const int64_t room = cus * (p.rows == 256 ? 1 : 2), least = p.rows == 32 ? 8 : 4;
   p.wgs = (int)std::min<int64_t>(room, (p.units + least - 1) / least);
-  if (p.whole) p.wgs = (int)std::min<int64_t>(p.items, INT32_MAX);
+  if (p.whole) p.wgs = (int)std::min<int64_t>(p.items, INT32_MAX), p.eight = p.items <= cus;
   return p;
 }
 
@@ -1290,7 +1291,10 @@ void launch_merge(const Args8 &aa, const Plan8 &p, hipStream_t s) {
 template <int D, bool E4M3>
 void launch_attn(const Args8 &aa, const Plan8 &p, hipStream_t s) {
   if (p.rows == 32) {
-    hipLaunchKernelGGL((kv8_rows_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(kWaves8 * 64), 0, s, aa);
+    if (p.eight)
+      hipLaunchKernelGGL((kv8_rows_kernel<D, 8, E4M3>), dim3((unsigned)p.wgs), dim3(512), 0, s, aa);
+    else
+      hipLaunchKernelGGL((kv8_rows_kernel<D, 4, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
     launch_merge<D, 32>(aa, p, s);
   } else if (p.rows == 128) {
     hipLaunchKernelGGL((kv8_tile_kernel<D, E4M3>), dim3((unsigned)p.wgs), dim3(256), 0, s, aa);
