@@ -197,7 +197,7 @@ CASES = [(1, 1, 64, [1]), (1, 3, 128, [33]), (5, 2, 64, [64, 1, 130]), (32, 4, 1
          (100, 5, 128, [64, 700, 33]), (128, 2, 64, [2000]), (129, 3, 128, [1]), (300, 2, 64, [65, 128]),
          (256, 9, 128, [500, 640]), (700, 1, 128, [5000, 64]), (33, 7300, 64, [65]), (128, 2600, 128, [1, 64]),
          (97, 40, 128, [6000, 65, 200]), (129, 1000, 128, [65, 1]), (257, 12, 128, [9000, 130, 64, 63]),
-         (513, 3, 64, [17000, 20000])]
+         (513, 3, 64, [17000, 20000]), (33, 200, 64, [65, 100]), (3, 300, 128, [700])]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -304,6 +304,23 @@ def test_batch_of_unlike_calls(torch_mod, dev, fmt):
             want, bound = _want(q[where], [SlotView(_Held(s.slot), s.tokens, s.row0) for s in call.segments], 0.125)
             assert (np.abs(_f64(o[where]) - want) <= bound).all()
     assert bool((out[:, :heads] == 7.0).all()) and bool((o[~touched.to(dev)] == 7.0).all())
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+def test_more_segments_than_one_launch(torch_mod, dev, rows):
+    """Then they are expanded and the oldest copied together: the call over bf16 slots of the same values."""
+    from taomate_hd_amd import KVSlot, segment_attention
+
+    torch, heads, dim = torch_mod, 2, 64
+    views, plain = [], []
+    for i in range(21):
+        slot = _slot(torch, *_kv(torch, 20 + 13 * i, heads, dim, i, dev), FORMATS[i % 2], dev)
+        views.append(slot.view())
+        plain.append(KVSlot(torch, heads=heads, head_dim=dim, capacity=slot.capacity, device=dev))
+        plain[-1].pack(*slot.token_major())
+    q = _kv(torch, rows, heads, dim, 99, dev)[0]
+    got = segment_attention(torch, q, views, scale=0.125)
+    assert torch.equal(got, segment_attention(torch, q, [p.view() for p in plain], scale=0.125))
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
