@@ -596,10 +596,11 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 
 // into MFMA operand order in LDS (chunks of 16 bytes, a wave's read 1 KiB in a row);
 // then every wave multiplies its rows with it.  Two buffers: while block b is
 // multiplied, block b + 1 (in registers since the block before) is converted and
-// block b + 2 loaded; one barrier a block.  Bound by the latencies between a block's
-// load, conversion, products and barrier, which the CU's other workgroup only
-// half fills: 14 heads of 128 over 40,788 tokens, e4m3: 64 rows 60 us (2.4 TB/s), 128
-// rows 76 us (490 TFLOPS); 40 heads, 91 rows over 11,232 tokens, int8: 55 us.
+// block b + 2 loaded; one barrier a block.  14 heads of 128 over 40,788 tokens, e4m3: 64
+// rows 57 us (2.6 TB/s), 128 rows 76 (490 TFLOPS); 40 heads, 91 rows over 11,232 tokens,
+// int8: 57.  Bound by a block's steps that follow each other, which the CU's other
+// workgroup only half fills: of the last 57 us, 20 go without the products and the
+// softmax, 10 without the conversion, 7 without the loads, 4 without the barrier.
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_tile_kernel(const Args8 aa) {
   constexpr int KC = D / 32, T = 256, ROWS = 128;
@@ -643,19 +644,21 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
     // K chunk (tile, 16 channels, key): two chunks of 8 channels, 512 bytes apart; V
     // chunk (tile, 32 channels, key group, channel): two of 8 keys, 1 KiB apart
+    // A block without finite values makes every output NaN: by way of `poison`, not of its values.
+    float poison = 0.f;
     auto convert = [&](int buf) {
+      const float fk = scale_of(kb), fv = scale_of(vb);
+      poison += fk + fv == fk + fv ? 0.f : fk + fv;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = i * T + tid;
         const bool is_v = c >= KCH;
         asm volatile("" : "+v"(raw[i]));  // (converted here, not where it was loaded: four times the registers)
-        const uint32_t byte = is_v ? vb : kb;
-        const float f = scale_of(byte);
-        const bool nan = byte == 255u;
+        const float f = is_v ? fv : fk;
         i32x4 o[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const i32x2 lo = decode4<E4M3>((uint32_t)raw[i][2 * m], f, nan), hi = decode4<E4M3>((uint32_t)raw[i][2 * m + 1], f, nan);
+          const i32x2 lo = decode4<E4M3>((uint32_t)raw[i][2 * m], f, false), hi = decode4<E4M3>((uint32_t)raw[i][2 * m + 1], f, false);
           o[m] = i32x4{lo[0], lo[1], hi[0], hi[1]};
         }
         const int cc = is_v ? c - KCH : c;
@@ -754,7 +757,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
       left = next_left;
     }
 
-    const float l = sum + __shfl_xor(sum, 32);
+    const float l = sum + __shfl_xor(sum, 32) + poison;
     const int row = r0 + lr;
     if (row < cl.lq) {
       if (pc.whole) {
