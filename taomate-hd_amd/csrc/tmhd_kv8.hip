@@ -834,7 +834,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, g = lane >> 5;
   const int x0 = range_begin(aa, xcd_wg(aa.wgs)), end = range_begin(aa, xcd_wg(aa.wgs) + 1);
   // (-inf, a masked score, times it stays -inf)
-  const float scale2 = fmaxf(aa.scale2, __uint_as_float(1u));
+  const float scale2 = aa.scale2 == 0.f ? __uint_as_float(1u) : aa.scale2;
   for (int x = x0; x < end;) {
     const Piece pc = piece_at(aa, x, end);
     const Call8 &cl = aa.call[pc.call];

@@ -425,6 +425,17 @@ def test_any_softmax_scale(torch_mod, dev, scale, rows, heads, dim, items):
     assert (np.abs(_f64(got) - want) <= bound).all()
 
 
+@pytest.mark.parametrize("rows,heads,dim,items", KERNELS)
+def test_scale_that_is_no_number(torch_mod, dev, rows, heads, dim, items):
+    from taomate_hd_amd import segment_attention
+
+    torch = torch_mod
+    assert _item_rows(heads, dim, (rows, [71])) == items
+    slot = _slot(torch, *_kv(torch, 71, heads, dim, 1, dev), "e4m3", dev)
+    q = _kv(torch, rows, heads, dim, 2, dev)[0]
+    assert bool(torch.isnan(segment_attention(torch, q, [slot.view()], scale=float("nan"))).all())
+
+
 def test_refusals(torch_mod, dev):
     from taomate_hd_amd import KVSlot8, fused_qkv_qk_norm_rope_stage_, segment_attention
 
