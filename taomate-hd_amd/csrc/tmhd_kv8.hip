@@ -407,6 +407,20 @@ __device__ __forceinline__ int in_branch(int keys) {
   return keys;
 }
 
+// A row's reference before its first score: a number, so that scores of -inf (sums that
+// overflowed) weigh 2^(-inf - kLeast) = 0 and not NaN
+constexpr float kLeast = -3.402823466e38f;
+
+// A score times the scale, rounded, less the reference, which is the largest such
+// product: what one rounding less (a fused multiply-add) leaves of the largest itself
+// is up to 2^-24 of it, and of products beyond 2^31 its power of two is infinite.
+__device__ __forceinline__ float below(float s, float scale, float reference) {
+#pragma clang fp contract(off)
+  return s * scale - reference;
+}
+// References up to which the fused form does (2^28: off by at most 2^4)
+constexpr float kFused = 268435456.f;
+
 // 32 query rows an item.  The W waves of a workgroup take an item's blocks in
 // turn and merge through LDS.  Per 32 keys a lane loads the 16-byte
 // chunks that are its MFMA operands (no LDS on the way: each code is used once)
@@ -433,7 +447,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 
     bf16x8 qf[2 * KC];
     load_q<D, true>(aa, cl, h, r0, lr, g, qf);
     f32x16 acc[KC];
-    float mx = -__builtin_inff(), sum = 0.f;
+    float mx = kLeast, sum = 0.f;
 #pragma unroll
     for (int d = 0; d < KC; ++d)
 #pragma unroll
@@ -514,7 +528,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 
       }
       float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], kc, -mx));
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(below(s[i], kc, mx));
       if (here < 32) {
         const int keys = in_branch(here) - 4 * g;
 #pragma unroll
@@ -561,7 +575,7 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 
       for (int i = 1; i < W; ++i) m = fmaxf(m, stat[0][i][r]);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        // a wave without blocks has the reference -inf and sums 0
+        // a wave without blocks has the reference kLeast and sums 0
         f[i] = stat[0][i][r] == m ? 1.0f : __builtin_amdgcn_exp2f(stat[0][i][r] - m);
         ls += f[i] * stat[1][i][r];
       }
@@ -619,7 +633,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
     bf16x8 qf[2 * KC];
     load_q<D, false>(aa, cl, h, r0, lr, g, qf);
     f32x16 acc[KC];
-    float mx = -__builtin_inff(), sum = 0.f;
+    float mx = kLeast, sum = 0.f;
+    bool large = false;  // references beyond kFused: the scores are brought below them one by one
 #pragma unroll
     for (int d = 0; d < KC; ++d)
 #pragma unroll
@@ -719,13 +734,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))
           for (int d = 0; d < KC; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+          large = __any(fabsf(mx) > kFused);
+        }
+        float mul = aa.scale2, ref = mx;
+        if (large) {
+          mul = 1.0f, ref = 0.f;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = below(s[t][i], aa.scale2, mx);
         }
         bf16x8 pf[2][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           float p[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], aa.scale2, -mx));
+          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, -ref));
           if (left < kBlock) {
             const int keys = in_branch(left) - 4 * g;
 #pragma unroll
@@ -845,7 +869,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
 #pragma unroll
     for (int i = 0; i < NQ; ++i) asm volatile("" : "+a"(qf[0][i]), "+a"(qf[1][i]));
     f32x16 acc[2][KC];
-    float mx[2] = {-__builtin_inff(), -__builtin_inff()}, sum[2] = {0.f, 0.f};
+    float mx[2] = {kLeast, kLeast}, sum[2] = {0.f, 0.f};
+    float mul = scale2, ref[2] = {kLeast, kLeast};  // (as in kv8_tile_kernel)
+    bool large = false;
 #pragma unroll
     for (int d = 0; d < KC; ++d)
 #pragma unroll
@@ -898,7 +924,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
       for (int i = 1; i < 16; ++i) m = fmaxf(m, sc[i]);
       return m;
     };
-    auto move = [&](float (&top)[2]) {  // (as in kv8_rows_kernel)
+    auto move = [&](float (&top)[2], f32x16 (&sc)[2]) {  // (as in kv8_rows_kernel; sc: the scores)
       top[0] *= scale2, top[1] *= scale2;
       if (__any(top[0] > mx[0] + 8.0f || top[1] > mx[1] + 8.0f)) {
         settle<KC>(acc);
@@ -914,6 +940,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
             for (int i = 0; i < 16; ++i) acc[rb][d][i] *= f;
         }
         settle<KC>(acc);
+        large = __any(fabsf(mx[0]) > kFused || fabsf(mx[1]) > kFused);
+        mul = large ? 1.0f : scale2;
+        ref[0] = large ? 0.f : mx[0], ref[1] = large ? 0.f : mx[1];
+      }
+      if (large) {
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[rb][i] = below(sc[rb][i], scale2, mx[rb]);
       }
     };
 
@@ -940,8 +975,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
         for (int u = 0; u < 16; ++u) {
           const int st = u >> 3, b = (u >> 2) & 1, q = u & 3;
           if (pair_at(u) == r) {
-            pe[u][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][8 * st + 2 * q], scale2, -mx[b]));
-            pe[u][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][8 * st + 2 * q + 1], scale2, -mx[b]));
+            pe[u][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][8 * st + 2 * q], mul, -ref[b]));
+            pe[u][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][8 * st + 2 * q + 1], mul, -ref[b]));
             asm volatile("" : "+v"(pe[u][0]), "+v"(pe[u][1]));
           }
           if (pair_at(u) + 1 == r) {
@@ -983,7 +1018,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
         mask(nx, left);
         top[0] = largest(nx[0]), top[1] = largest(nx[1]);
       }
-      move(top);
+      move(top, nx);
     };
 
     // K of blocks 0 and 1, V of block 0; the codes of block 2's K and block 1's V
@@ -1018,7 +1053,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))
     if (left0 < 32) mask(sa, left0);
     {
       float top[2] = {largest(sa[0]), largest(sa[1])};
-      move(top);
+      move(top, sa);
     }
     int k0 = 0, k1 = HALF, k2 = 2 * HALF;  // the K buffers of blocks b, b + 1, b + 2
 #pragma unroll

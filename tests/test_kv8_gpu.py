@@ -426,6 +426,46 @@ def test_any_softmax_scale(torch_mod, dev, scale, rows, heads, dim, items):
 
 
 @pytest.mark.parametrize("rows,heads,dim,items", KERNELS)
+def test_first_scores_below_every_number(torch_mod, dev, rows, heads, dim, items):
+    """Scores of a call's first block that overflow to -inf weigh nothing, and leave what follows alone."""
+    from taomate_hd_amd import segment_attention
+    from taomate_hd_amd.slots import SlotView
+
+    torch = torch_mod
+    assert _item_rows(heads, dim, (rows, [71])) == items
+    k, v = _kv(torch, 71, heads, dim, 1, dev)
+    k[:64] = -(2.0 ** 100)
+    slot = _slot(torch, k, v, "int8", dev)
+    q = 2.0 ** 40 * (1 + _kv(torch, rows, heads, dim, 2, dev)[0].abs())
+    got = segment_attention(torch, q, [slot.view()], scale=2.0 ** -43)
+    want, bound = _want(q, [SlotView(slot, 7, 64)], 2.0 ** -43)
+    assert (np.abs(_f64(got) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rows,heads,dim,items", KERNELS)
+def test_scores_beyond_every_fraction(torch_mod, dev, rows, heads, dim, items, sign):
+    """Equal scores of 2^44 and more, all of an fp32's bits above the point: the mean of the values, then one larger
+    score that outweighs them all."""
+    from taomate_hd_amd import segment_attention
+    from taomate_hd_amd.slots import SlotView
+
+    torch = torch_mod
+    assert _item_rows(heads, dim, (rows, [71])) == items
+    k, v = _kv(torch, 71, heads, dim, 1, dev)
+    k[:] = sign * 2.0 ** 20
+    k[70] = 2.0 ** 21
+    slot = _slot(torch, k, v, "int8", dev)
+    q = 2.0 ** 24 * (1 + _kv(torch, rows, heads, dim, 2, dev)[0].abs())
+    values = _f64(slot.token_major()[1])
+    for view, want in ((SlotView(slot, 70, 0), values[:70].mean(0)), (SlotView(slot, 6, 64), values[64:70].mean(0)),
+                       (slot.view(), values[70])):
+        got = _f64(segment_attention(torch, q, [view], scale=0.9))
+        size = np.abs(values).max(0)
+        assert (np.abs(got - want) <= HALF_BF16 * np.abs(want) + 1.02 * (HALF_BF16 + 2.0 ** -20) * size).all()
+
+
+@pytest.mark.parametrize("rows,heads,dim,items", KERNELS)
 def test_scale_that_is_no_number(torch_mod, dev, rows, heads, dim, items):
     from taomate_hd_amd import segment_attention
 
