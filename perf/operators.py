@@ -15,7 +15,6 @@ package.  ``exact`` gives the same outputs in 64 bits.
 """
 
 import sys
-from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -28,9 +27,7 @@ E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 TOP = {"e4m3": (0.875, 9), "int8": (0.9921875, 7)}
 
 
-@lru_cache(maxsize=1)
 def _package():
-    """The package of the repository this runs in, imported once as a user's program does."""
     root = str(Path("taomate-hd_amd").resolve())
     if root not in sys.path:
         sys.path.insert(1, root)
