@@ -126,9 +126,12 @@ int tmhd_kv8_token_major(const tmhd_kv8_segment *view, void *k, void *v, int32_t
 
 /*
  * One attention call over 8-bit segments: softmax(q k^T * scale) v over the
- * values they stand for, no mask.  Codes are turned into bf16 once for up to 256
- * query rows; calls of many more rows take less time over a slot that
- * tmhd_kv8_expand wrote.  Queries and outputs as in tmhd_attn_args.
+ * values they stand for, no mask.  Weighted values are summed in fp32 and divided
+ * by the weights' sum at the end, with weights up to 2^8: values above about 2^120 /
+ * tokens may overflow on the way.  Q is not rounded again (scores are scaled in
+ * fp32).  Codes are turned into bf16 once for up to 256 query rows; calls of many more
+ * rows take less time over a slot that tmhd_kv8_expand wrote, whose kernel rounds the
+ * scaled Q to bf16.  Queries and outputs as in tmhd_attn_args.
  */
 typedef struct tmhd_kv8_call {
   const void *q;

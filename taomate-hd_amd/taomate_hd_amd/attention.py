@@ -12,7 +12,7 @@ Segments may lie in slots held in 8 bits (``KVSlot8``).  A ``"bf16"`` call
 whose segments all do, in one format, reads their codes in place
 (``tmhd_attn_fwd_kv8``) where it has up to ``KV8_ROWS`` query rows or the batch
 is small; for any other call they are expanded to bf16 first, which is exact,
-and the call runs as over bf16 slots.
+and the call runs as over bf16 slots, whose kernel rounds the scaled Q to bf16.
 """
 
 from __future__ import annotations
@@ -26,17 +26,20 @@ from .profiling import ComponentTimer, maybe_region
 from .slots import KV_TILE, KVSlot, KVSlot8, SlotView, expand_views, round_up, vt_columns
 
 BACKENDS = ("bf16", "i8qk")
-# 8-bit segments are read in place by calls of up to KV8_ROWS query rows, and by
-# batches of up to KV8_WORK (query row, token, channel) products.  The kernels that
-# read codes turn every block into bf16 for at most 256 rows at a time and multiply at
-# 1.0 PFLOPS; expanding costs a pass over the cache and a launch, the bf16 kernel
-# then runs at up to 1.35.  Measured, e4m3, in place / expanded, us: 14 heads of 128
-# over 41,000 tokens 108/187 at 256 rows, 301/348 at 1,024, 573/613 at 2,048, 1,418/1,227
-# at 5,120; 11,000 tokens 71/76 at 512, 109/106 at 1,024, 143/133 at 1,536; 2,800 tokens
-# 54/54 at 1,024; 700 tokens 35/50 at 1,536 (1.9e9 products), 52/51 at 2,560 (3.2e9); 4
-# heads over 2,800 tokens 30/54 at 2,048 (2.9e9); 14 heads of 64 over 41,000 tokens
-# 127/145 at 512, 222/223 at 1,024, 321/294 at 1,536.  int8 is 5 to 10% slower in place.
-KV8_ROWS = 1024
+# 8-bit segments are read in place by calls of up to KV8_ROWS query rows (more than any
+# chunk's), and by batches of up to KV8_WORK (query row, token, channel) products.  The
+# kernels that read codes multiply Q as it is and the scores by the scale in fp32; the
+# bf16 kernel multiplies Q by the scale first and rounds it to bf16 (2^-8 of a score's
+# products).  So a row's result does not change its accuracy with the rows beside it: off
+# in the 2-norm by 0.0023 to 0.0024 in place and 0.0028 to 0.0030 expanded on N(0, 1) keys,
+# and more apart at larger scores.  What that costs, in place / expanded, us, three
+# segments: 14 heads of 128 over 40,788 tokens, e4m3, 362/369 at 1,024 rows, 645/620 at
+# 2,048, 1,375/1,188 at 4,836, 3,359/2,786 at 12,252, int8 1,560/1,183 at 4,836; over
+# 11,232 tokens 164/141 at 1,536, 441/350 at 4,836; over 2,717 140/122 at 4,836; over 700
+# 34/53 at 2,560 (3.2e9 products); 4 heads over 2,800 24/55 at 2,048; 14 heads of 64 over
+# 40,788 970/798 at 4,836.  Views that expand_views wrote are attended at the bf16
+# kernel's time and rounding.
+KV8_ROWS = 1 << 14
 KV8_WORK = 5 << 29
 
 

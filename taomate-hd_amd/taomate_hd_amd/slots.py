@@ -16,8 +16,9 @@ for the INT8-QK smooth-K mean); attention reads them in place.
 ``KVSlot8`` is the same unit held in 8 bits (e4m3 or int8 codes with a
 power-of-two scale for each 64 tokens of a head; layout in
 include/tmhd_lowbit.h): half the memory, written by its quantizing ``pack``.
-Attention of up to a few hundred query rows reads its codes in place; other
-readers expand it to bf16 first, which is exact.
+Attention reads its codes in place where all of a call's segments are 8-bit
+ones of one format (the rule is at ``attention.KV8_ROWS``); other readers
+expand it to bf16 first, which is exact.
 """
 
 from __future__ import annotations
