@@ -1,8 +1,8 @@
 /*
  * tmhd_lowbit.h - block-scaled low-bit storage: MXFP4 projections and a K/V
  * cache held in 8 bits.  Conventions and status codes are tmhd.h's.  Every
- * scale is a power of two, 2^(byte - 127) (byte 255: NaN), so a stored value
- * times its scale is a bf16 number exactly.
+ * scale is a power of two, 2^(byte - 127) (byte 255: NaN), and a code that these
+ * entries write times its scale is a finite bf16 number exactly.
  *
  * MXFP4 matrix [rows][k], k a multiple of 32
  *   codes : uint8 [rows][k / 2], two e2m1 values a byte, the even column in the
@@ -105,8 +105,10 @@ typedef struct tmhd_kv8_segment {
  * dst .. (dst a multiple of 64), rows up to the next multiple of 64 become zero.
  * Per 64 tokens of a head, K and V apart: e = the least integer, not below
  * -117, with max |x| <= Q 2^e (Q = 448 for e4m3, 127 for int8), code = x 2^-e
- * rounded to nearest even; an infinity or NaN gives the block the scale byte
- * 255 and codes 0.  zero_to of a range is not used.
+ * rounded to nearest even, but not up to one that stands for 2^128 (in e4m3 blocks
+ * with max |x| >= 1.9375 2^127 and int8 blocks that hold the largest finite bf16, the
+ * code below is the last); an infinity or NaN gives the block the scale byte 255 and
+ * codes 0.  zero_to of a range is not used.
  */
 int tmhd_kv8_pack_ranges(const void *k, const void *v, int64_t token_stride, int64_t head_stride,
                          const tmhd_pack_range *ranges, int32_t n_ranges, const tmhd_kv8_segment *slot, int32_t heads,

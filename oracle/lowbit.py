@@ -1,8 +1,8 @@
 """Block-scaled low-bit formats, restated in float64 numpy (formats: include/tmhd_lowbit.h).
 
 MXFP4 by search over its eight magnitudes, 8-bit K/V by rounding to the code's
-own step; scales are found from the definition (a power of two and an
-inequality), not from bit fields.  Values come back as the float64 numbers
+own step, but not up to 2^128, which bf16 does not hold; scales are found from
+the definition (a power of two and an inequality), not from bit fields.  Values come back as the float64 numbers
 that codes and scales stand for, NaN for a block that holds an infinity or NaN.
 """
 
@@ -41,6 +41,7 @@ def mxfp4_values(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
 
 
 KV_TOP = {"e4m3": 448.0, "int8": 127.0}
+KV_BELOW = {256.0: 240.0, 64.0: 63.0}  # the code in front of a power of two, e4m3 and int8
 
 
 def kv8_values(x: np.ndarray, fmt: str) -> tuple[np.ndarray, np.ndarray]:
@@ -65,6 +66,8 @@ def kv8_values(x: np.ndarray, fmt: str) -> tuple[np.ndarray, np.ndarray]:
             y = np.rint(y / step) * step
         else:
             y = np.rint(y)
+        for power, code in KV_BELOW.items():
+            y = np.where((np.abs(y) == power) & (power * scale == 2.0**128), np.copysign(code, y), y)
         y = y * scale
         y[:, bad] = np.nan
         out[64 * i : 64 * i + 64] = y

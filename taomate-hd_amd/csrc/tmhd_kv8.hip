@@ -36,6 +36,22 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
   return (uint32_t)max(E4M3 ? e - 8 + (m > 0x60) : e - 6 + (m > 0x7e), kMinByte);
 }
 
+// Largest scale byte of finite values, and the largest magnitude (bf16 bits) that is
+// encoded under it: codes from the next one on (248 and more halfway to 256 in e4m3,
+// 63.5 halfway to 64 in int8) would stand for 2^128, which bf16 does not hold.
+template <bool E4M3>
+constexpr uint32_t kTopByte = E4M3 ? 247 : 249;
+template <bool E4M3>
+constexpr uint32_t kTopMagnitude = E4M3 ? 0x7f77 : 0x7f7d;
+
+// The magnitudes of 2 bf16 brought down to kTopMagnitude
+template <bool E4M3>
+__device__ __forceinline__ int below_top(int w) {
+  constexpr uint16_t top = kTopMagnitude<E4M3>;
+  const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, (uint32_t)w & 0x7fff7fffu), u16x2{top, top});
+  return (int)(__builtin_bit_cast(uint32_t, m) | ((uint32_t)w & 0x80008000u));
+}
+
 // 8 bf16 -> 8 codes (2 words)
 template <bool E4M3>
 __device__ __forceinline__ i32x2 encode8(const i32x4 &v, uint32_t byte) {
@@ -52,7 +68,7 @@ __device__ __forceinline__ i32x2 encode8(const i32x4 &v, uint32_t byte) {
       c[h] = __builtin_bit_cast(int, p);
     }
   } else {
-    const float inv = __uint_as_float((254u - byte) << 23);  // exact: the byte is 10 .. 248
+    const float inv = __uint_as_float((254u - byte) << 23);  // exact: the byte is 10 .. 249
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t p = 0;
@@ -147,6 +163,12 @@ __global__ void __launch_bounds__(2 * D) kv8_pack_kernel(const PackArgs pa) {
 #pragma unroll
   for (int i = 1; i < T / 64; ++i) amax = max(amax, part[i]);
   const uint32_t byte = scale_byte<E4M3>(amax);
+  if (byte >= kTopByte<E4M3>) {  // (the same for the whole workgroup)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = below_top<E4M3>(v[i][e]);
+  }
   const int64_t blk = pa.r[ri].dst / kBlock + b;  // of the slot
   if (tid == 0) (is_v ? pa.vso : pa.kso)[(int64_t)h * (pa.cap / kBlock) + blk] = (uint8_t)byte;
   i32x2 c[4];

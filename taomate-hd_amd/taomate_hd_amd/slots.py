@@ -225,7 +225,8 @@ class KVSlot8(KVSlot):
     Per 64 slot rows of a head, keys and values apart, the scale is the least
     power of two (not below 2^-117) that brings the largest magnitude to the
     format's range (448 for ``"e4m3"``, 127 for ``"int8"``); codes are rounded
-    to nearest even.  A block that holds an infinity or NaN reads back as NaN.
+    to nearest even, but not up to 2^128: finite values read back as finite bf16
+    values.  A block that holds an infinity or NaN reads back as NaN.
     """
 
     def __init__(self, torch: Any, *, heads: int, head_dim: int, capacity: int, device: Any, fmt: str = "e4m3") -> None:
