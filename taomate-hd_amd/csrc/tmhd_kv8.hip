@@ -211,10 +211,17 @@ struct ExpandArgs {
   View view[kMaxSegs];
 };
 
+// The first n of four bf16 (2 words), the others zero
+__device__ __forceinline__ i32x2 first_of4(const i32x2 &v, int n) {
+  auto word = [](int w, int k) { return k >= 2 ? w : k == 1 ? w & 0xffff : 0; };
+  return i32x2{word(v[0], n), word(v[1], n - 2)};
+}
+
 // One 64-token block of K or V of one head into the bf16 slot format; bound by
 // HBM.  K: lanes run along a token row, so that rows are written whole.  V: the
 // 16 codes of a chunk are two runs of 8 consecutive positions of a transposed row.
-// 40,788 tokens of 14 heads of 128 89 us (4.9 TB/s).
+// Rows behind the view become zero, whatever the slot holds there.  40,788 tokens of
+// 14 heads of 128 89 us (4.9 TB/s).
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(2 * D) kv8_expand_kernel(const ExpandArgs ea) {
   constexpr int T = 2 * D, C = D / 16;
@@ -228,6 +235,7 @@ __global__ void __launch_bounds__(2 * D) kv8_expand_kernel(const ExpandArgs ea) 
   const uint32_t byte = (is_v ? vw.vs : vw.ks)[(int64_t)h * (vw.cap / kBlock) + b];
   const float s = scale_of(byte);
   const bool nan = byte == 255u;
+  const int left = vw.tokens - b * kBlock;  // valid rows of the block, 64 and more for a whole one
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int c = i * T + tid;
@@ -237,7 +245,11 @@ __global__ void __launch_bounds__(2 * D) kv8_expand_kernel(const ExpandArgs ea) 
       uint16_t *o = ea.vt + (int64_t)h * ea.vhs + (int64_t)d * ea.vrs + vw.dst + b * kBlock + tile * 32 + g * 8;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const i32x2 lo = decode4<E4M3>((uint32_t)w[2 * m], s, nan), hi = decode4<E4M3>((uint32_t)w[2 * m + 1], s, nan);
+        i32x2 lo = decode4<E4M3>((uint32_t)w[2 * m], s, nan), hi = decode4<E4M3>((uint32_t)w[2 * m + 1], s, nan);
+        if (left < kBlock) {  // word j of the chunk: tokens 8 j + 4 g ..
+          const int keep = left - tile * 32 - 4 * g - 16 * m;
+          lo = first_of4(lo, keep), hi = first_of4(hi, keep - 8);
+        }
         *(i32x4 *)(o + 16 * m) = i32x4{lo[0], lo[1], hi[0], hi[1]};
       }
     } else {
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(2 * D) kv8_expand_kernel(const ExpandArgs ea) 
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const i32x2 lo = decode4<E4M3>((uint32_t)w[2 * m], s, nan), hi = decode4<E4M3>((uint32_t)w[2 * m + 1], s, nan);
-        *(i32x4 *)(o + 8 * m) = i32x4{lo[0], lo[1], hi[0], hi[1]};
+        *(i32x4 *)(o + 8 * m) = t < left ? i32x4{lo[0], lo[1], hi[0], hi[1]} : i32x4{0, 0, 0, 0};
       }
     }
   }
