@@ -116,8 +116,8 @@ int tmhd_kv8_pack_ranges(const void *k, const void *v, int64_t token_stride, int
 
 /*
  * The values of n views (all of one head count and head_dim) in bf16, into the
- * slot format of tmhd.h: view i at slot rows dst[i] .. (multiples of 64), zero up
- * to the next multiple of 64.  Exact.
+ * slot format of tmhd.h: view i at slot rows dst[i] .. (multiples of 64; no two views
+ * in one 64-row block), zero up to the next multiple of 64.  Exact.
  */
 int tmhd_kv8_expand(const tmhd_kv8_segment *views, const int32_t *dst, int32_t n, void *k_slot, void *vt_slot,
                     int64_t k_head_stride, int64_t vt_head_stride, int32_t vt_row_stride, int32_t heads,

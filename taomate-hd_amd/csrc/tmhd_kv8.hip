@@ -1437,11 +1437,15 @@ extern "C" int tmhd_kv8_expand(const tmhd_kv8_segment *views, const int32_t *dst
   if (!k_slot || !vt_slot || (uintptr_t)k_slot % 16 || (uintptr_t)vt_slot % 16 || k_head_stride % 8 || vt_head_stride % 8 ||
       vt_row_stride % 8 || vt_head_stride < (int64_t)head_dim * vt_row_stride)
     return set_error(TMHD_ERR_INVALID, "%s: null or misaligned slot", what);
+  auto end_of = [&](int i) { return (int64_t)dst[i] + (views[i].tokens + kBlock - 1) / kBlock * kBlock; };
   for (int i = 0; i < n; ++i) {
     if (int st = check_view(what, views[i])) return st;
-    const int64_t end = (int64_t)dst[i] + (views[i].tokens + kBlock - 1) / kBlock * kBlock;
+    const int64_t end = end_of(i);
     if (dst[i] < 0 || dst[i] % kBlock || end > vt_row_stride || end * head_dim > k_head_stride)
       return set_error(TMHD_ERR_INVALID, "%s: view %d of %d rows at slot row %d", what, i, views[i].tokens, dst[i]);
+    for (int j = 0; j < i; ++j)
+      if (dst[j] < end && dst[i] < end_of(j))
+        return set_error(TMHD_ERR_INVALID, "%s: views %d and %d share rows of the slot", what, j, i);
   }
   for (int i = 0; i < n;) {
     ExpandArgs ea{(uint16_t *)k_slot, (uint16_t *)vt_slot, k_head_stride, vt_head_stride, vt_row_stride, 0, {}};
