@@ -437,18 +437,6 @@ __device__ __forceinline__ void orescale(int b, f32x16 &o, float alpha) {
 // code reads it (an 8-pass MFMA completes within 4 * 8 + 2 cycles).
 __device__ __forceinline__ void mfma_drain() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// 16 bytes per lane global -> LDS (saddr form: 64-bit uniform base, 32-bit
-// per-lane offset); the wave's 64 lanes fill the 1 KiB LDS block at m0.
-// Issued as inline asm on purpose: the compiler's wait-count insertion cannot
-// tell the destination block from the tiles being read and would place a
-// vmcnt(0) wait in front of the next LDS read, serialising the prefetch.  The
-// kernel itself waits (vmcnt(0) + barrier) before any read of a loaded tile;
-// extra in-order vector-memory operations unknown to the compiler only make
-// its own vmcnt waits stricter.
-__device__ __forceinline__ void load_lds16(const void *base, uint32_t off, uint32_t lds_addr) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
-}
-
 // Physical 16-byte chunk of chunk c of staged row r (rows of 2 D bytes): the
 // rows that share the 512 bytes of the 128 banks sit next to each other, the
 // others are spread over the chunks.  A staging write (8 bytes per lane, one
@@ -730,20 +718,20 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
     };
     auto load_one = [&](int n, const char *kbase, uint32_t kdst, const char *vbase, uint32_t vdst) {
       if (n < KWL)
-        load_lds16(kbase, koff[n], kdst + kblk(n) * 1024);
+        load_lds16_base(kbase, koff[n], kdst + kblk(n) * 1024);
       else
-        load_lds16(vbase, voff[n - KWL], vdst + vblk(n - KWL) * 1024);
+        load_lds16_base(vbase, voff[n - KWL], vdst + vblk(n - KWL) * 1024);
     };
     auto load_k = [&](const Stream &S, int buf) {
       const char *base = S.kb + (int64_t)S.t * (kBN * KROW);
 #pragma unroll
-      for (int i = 0; i < KWL; ++i) load_lds16(base, koff[i], lds0 + buf * KT + kblk(i) * 1024);
+      for (int i = 0; i < KWL; ++i) load_lds16_base(base, koff[i], lds0 + buf * KT + kblk(i) * 1024);
     };
     auto load_v = [&](const Stream &S, int buf) {
       const char *base = S.vb + S.t * (kBN * 2);
 #pragma unroll
       for (int i = 0; i < VWL; ++i)
-        load_lds16(base, (vrc[i] & 0xfffffu) * S.vrs2 + ((vrc[i] >> 20) << 4),
+        load_lds16_base(base, (vrc[i] & 0xfffffu) * S.vrs2 + ((vrc[i] >> 20) << 4),
                    lds0 + 3 * KT + buf * VT + vblk(i) * 1024);
     };
     auto lds_read = [&](uint32_t off) { return *(const i32x4 *)(smem + off); };
@@ -1244,19 +1232,19 @@ __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_e
     auto load_one = [&](int n, const uint32_t (&t)[8], const char *kbase, uint32_t kdst, const char *vbase,
                         uint32_t vdst) {
       if (n < KWL)
-        load_lds16(kbase, t[n], kdst + kblk(n) * 1024);
+        load_lds16_base(kbase, t[n], kdst + kblk(n) * 1024);
       else
-        load_lds16(vbase, t[n], vdst + vblk(n - KWL) * 1024);
+        load_lds16_base(vbase, t[n], vdst + vblk(n - KWL) * 1024);
     };
     auto load_k = [&](const Stream &S, int buf) {
       const char *base = S.kb + (int64_t)S.t * (kBN * KROW);
 #pragma unroll
-      for (int i = 0; i < KWL; ++i) load_lds16(base, koff_of(i), lds0 + buf * KT + kblk(i) * 1024);
+      for (int i = 0; i < KWL; ++i) load_lds16_base(base, koff_of(i), lds0 + buf * KT + kblk(i) * 1024);
     };
     auto load_v = [&](const Stream &S, int buf) {
       const char *base = S.vb + S.t * (kBN * 2);
 #pragma unroll
-      for (int i = 0; i < VWL; ++i) load_lds16(base, voff_of(i, S.vrs2), lds0 + 3 * KT + buf * VT + vblk(i) * 1024);
+      for (int i = 0; i < VWL; ++i) load_lds16_base(base, voff_of(i, S.vrs2), lds0 + 3 * KT + buf * VT + vblk(i) * 1024);
     };
     auto load_ks = [&](const Stream &S) {
       int idx = S.t >> 1;  // 128-token quant blocks hold two tiles

@@ -1,5 +1,5 @@
-// Pieces that the tiled products share (gfx950): tile order, direct-to-LDS
-// loads and their waits.
+// Pieces that the tiled products share (gfx950): tile order and the waits of their
+// direct-to-LDS loads (load_lds16_base).
 #pragma once
 
 #include "tmhd_internal.h"
@@ -27,11 +27,5 @@ __device__ __forceinline__ void grouped_tile(int L, int tm_count, int tn_count, 
 
 // s_waitcnt immediate that leaves n vector-memory operations in flight (and waits for nothing else)
 constexpr int vmcnt_imm(int n) { return 0x0f70 | (n & 15) | ((n >> 4) << 14); }
-
-// 16 bytes per lane from base + off to LDS at lds_addr (+ 16 lane).  Inline asm, so
-// that the compiler does not wait for it before unrelated LDS reads.
-__device__ __forceinline__ void hload_lds16(const void *base, uint32_t off, uint32_t lds_addr) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
-}
 
 }  // namespace tmhd

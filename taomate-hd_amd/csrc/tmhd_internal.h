@@ -146,6 +146,21 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// 16 bytes per lane from base (uniform) + off to LDS at lds_addr (uniform) + 16 lane.
+// Inline asm on purpose: the compiler's wait-count insertion cannot tell the destination
+// from the LDS that is being read and would wait for the load in front of the next LDS
+// read; kernels wait (vmcnt, barrier) before they read what it loaded.  In exchange the
+// compiler does not keep this instruction's wait states for it: five after a vector
+// instruction that wrote its scalar base (v_readfirstlane, or v_readlane of a scalar that
+// was spilled to a vector lane; a load behind one went to a stray address) and one after
+// the write of m0.  The copy of the base keeps both: a scalar instruction waits for the
+// vector write by itself, and a load may follow a scalar write of its base at once.
+__device__ __forceinline__ void load_lds16_base(const void *base, uint32_t off, uint32_t lds_addr) {
+  const void *copy;
+  asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+               : "=&s"(copy) : "v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
+}
+
 constexpr int kMaxSeg = TMHD_MAX_SEGMENTS;
 
 }  // namespace tmhd

@@ -293,18 +293,6 @@ __global__ void __launch_bounds__(256) mxfp4_rows_kernel(const XArgs xa) {
 // there are zero, 2^-127 on both sides: the products underflow to 0.
 constexpr int KB = 128;  // bytes of a row in a block
 
-// hload_lds16 with the wait states that a vector-memory instruction needs after
-// the vector instruction that wrote its scalar base (five: v_readlane of a
-// spilled register, v_readfirstlane) and after the write of m0 (one).  The
-// compiler keeps those for its own instructions, not for inline asm, and the
-// product kernels hold enough scalars for it to spill some to vector lanes.  The
-// copy of the base is a scalar instruction: it waits for the vector write by
-// itself, and a scalar write needs no wait states before the load.
-__device__ __forceinline__ void load_lds16_any(const void *base, uint32_t off, uint32_t lds_addr) {
-  const void *copy;
-  asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(copy) : "v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
-}
-
 // A wave's sums, rounded to bf16 and stored from registers: rows m0 .., columns n0 ...  A
 // pair of 16-column blocks trades halves between neighbouring lane groups, so that a
 // lane holds 8 consecutive columns of one block (16 bytes).  WHOLE: every row and
@@ -430,11 +418,11 @@ struct TileLoop {
     const uint32_t to = lds0 + (uint32_t)(buf * BUF);
     if (n < DL) {
       const uint32_t dst = to + (n < AL ? (w + 4 * n) * 1024 : BM * KB + (w + 4 * (n - AL)) * 1024);
-      load_lds16_any(n < AL ? xa.a : xa.b, doff[n] + koff, dst);
+      load_lds16_base(n < AL ? xa.a : xa.b, doff[n] + koff, dst);
     } else {
       const int i = n - DL;
       const uint32_t *base = scale_of_a(i) ? xa.as + (int64_t)(d >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(d >> 1) * 4 * xa.bn4;
-      load_lds16_any(base, soff[i], to + sdst[i]);
+      load_lds16_base(base, soff[i], to + sdst[i]);
     }
   }
   __device__ __forceinline__ uint32_t koff_of(int d) const { return (uint32_t)(min(8 * d + lch, chunks - 1) * 16); }
@@ -627,11 +615,11 @@ struct BigLoop {
   }
   // load i of unit j of the block at the load cursor, into ring slot s
   __device__ __forceinline__ void load_data(int s, int j, int i) {
-    load_lds16_any(j & 1 ? bbase : abase, doff[j][i], lds0 + (uint32_t)(s * UNIT + (w + 8 * i) * 1024));
+    load_lds16_base(j & 1 ? bbase : abase, doff[j][i], lds0 + (uint32_t)(s * UNIT + (w + 8 * i) * 1024));
   }
   __device__ __forceinline__ void load_scales() {
     const uint32_t to = lds0 + (uint32_t)(RING + sload * SBUF + w * 1024);
-    load_lds16_any(w < 4 ? xa.as + (int64_t)(lb >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4, soff, to);
+    load_lds16_base(w < 4 ? xa.as + (int64_t)(lb >> 1) * 4 * xa.am4 : xa.bs + (int64_t)(lb >> 1) * 4 * xa.bn4, soff, to);
     sload ^= 1;
   }
   // the load cursor's next block: of this tile, of the workgroup's next one, or

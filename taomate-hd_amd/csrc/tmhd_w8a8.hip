@@ -438,9 +438,9 @@ gemm_i8_wave128_kernel(const GArgs ga) {
     const int j = min(u >> 1, nd - 1), h = u & 1, i = n & 3;
     const uint32_t dst = lds0 + (uint32_t)((u % HRING) * HUNIT) + (w + 4 * i) * 1024;
     if (n < 4)
-      hload_lds16(abase + (int64_t)j * HKD, aoff[h][i], dst);
+      load_lds16_base(abase + (int64_t)j * HKD, aoff[h][i], dst);
     else
-      hload_lds16(bbase + (int64_t)j * HKD, boff[h][i], dst + HUNIT / 2);
+      load_lds16_base(bbase + (int64_t)j * HKD, boff[h][i], dst + HUNIT / 2);
   };
   // operand read offsets within a unit's operand part, k-step q (0..1) of the
   // block: 16x16x64 operand lane (i, g4) = lane % 16, lane / 16 holds 16 bytes
@@ -818,7 +818,7 @@ gemm_i8_tile_kernel(const GArgs ga) {
   // last block repeat it, into a slot nobody reads
   auto load_one = [&](int j, int h, int slot, int i) {
     const uint32_t at = i < AL ? (w + 4 * i) * 1024 : MH * HKD + (w + 4 * (i - AL)) * 1024;
-    hload_lds16((i < AL ? ga.a : ga.b) + (int64_t)min(j, nd - 1) * HKD, soff[h][i], lds0 + (uint32_t)(slot * UNIT) + at);
+    load_lds16_base((i < AL ? ga.a : ga.b) + (int64_t)min(j, nd - 1) * HKD, soff[h][i], lds0 + (uint32_t)(slot * UNIT) + at);
   };
   // operand reads: 16x16x64 lane (i, g4) holds 16 bytes of row i at logical chunk 4 q + g4
   const int li = lane & 15, lg = lane >> 4;
