@@ -308,6 +308,12 @@ __global__ void __launch_bounds__(2 * D) kv8_token_major_kernel(const View vw, u
 }
 
 // ---- attention
+//
+// Scores, maxima and sums are fp32.  Weights go into the second product rounded to bf16,
+// the MFMA's operand type (each off by at most 2^-8; the values are bf16 numbers already),
+// while their sum takes them unrounded.  Results are off by 0.0023 in the 2-norm on N(0, 1)
+// keys, the rounding of the result alone by 0.0017; a second bf16 term of each weight would
+// double that product's MFMAs.
 
 struct Seg8 {
   const uint8_t *k, *v, *ks, *vs;
@@ -645,10 +651,11 @@ __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 
 // then every wave multiplies its rows with it.  Two buffers: while block b is
 // multiplied, block b + 1 (in registers since the block before) is converted and
 // block b + 2 loaded; one barrier a block.  14 heads of 128 over 40,788 tokens, e4m3: 64
-// rows 57 us (2.6 TB/s), 128 rows 76 (490 TFLOPS); 40 heads, 91 rows over 11,232 tokens,
-// int8: 57.  Bound by a block's steps that follow each other, which the CU's other
-// workgroup only half fills: of the last 57 us, 20 go without the products and the
-// softmax, 10 without the conversion, 7 without the loads, 4 without the barrier.
+// rows 53 to 57 us (2.6 TB/s), 128 rows 66 to 76 (490 TFLOPS); 40 heads, 91 rows over
+// 11,232 tokens, int8: 52 to 57 (the lower figures of a faster card).  Bound by a block's
+// steps that follow each other, which the CU's other workgroup only half fills: of the
+// last 57 us, 20 go without the products and the softmax, 10 without the conversion, 7
+// without the loads, 4 without the barrier.
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) kv8_tile_kernel(const Args8 aa) {
   constexpr int KC = D / 32, T = 256, ROWS = 128;
@@ -876,8 +883,9 @@ __device__ __forceinline__ void settle(f32x16 (&o)[2][KC]) {  // (and after vect
 // of three; then this tile's outputs, with the last weights, the next tile's maximum
 // and the conversion of block b + 2's K or block b + 1's V (loaded an iteration before)
 // in front of the MFMAs.  K in three buffers, V in two, one barrier for 64 keys.
-// 14 heads of 128 over 40,788 tokens, e4m3 (int8): 256 rows 102 us (108), 1,024 rows 305
-// (332; 983 TFLOPS), 4,836 rows 1,383 (1,479).  Bound by issue: MFMAs busy 48% of the
+// 14 heads of 128 over 40,788 tokens, e4m3 (int8): 256 rows 97 to 102 us (104 to 108),
+// 1,024 rows 284 to 305 (308 to 332; 983 TFLOPS), 4,836 rows 1,283 to 1,383 (1,380 to
+// 1,479), the lower figures of a faster card.  Bound by issue: MFMAs busy 48% of the
 // time, instructions issuing 59%; without the conversion (16 cycles for two values) 13%
 // less time, without the exponentials 9%, without the barrier 3%.  Eight waves of 32 rows
 // took 104, 339 and 1,356 us (int8 108, 353, 1,459) and read LDS for as long as they

@@ -296,7 +296,10 @@ constexpr int KB = 128;  // bytes of a row in a block
 // A wave's sums, rounded to bf16 and stored from registers: rows m0 .., columns n0 ...  A
 // pair of 16-column blocks trades halves between neighbouring lane groups, so that a
 // lane holds 8 consecutive columns of one block (16 bytes).  WHOLE: every row and
-// column is inside the matrix and rows are 16-byte aligned: one address a row.
+// column is inside the matrix and rows are 16-byte aligned: one address a row.  Rows of
+// another alignment (a width that is not a multiple of 8) are stored two bytes at a
+// time: 12,252 x 9,001 x 832 271 us, 9,008 columns 83; 4,836 x 10,751 x 5,376 222, 10,752
+// columns 132; 331 x 10,751 x 5,376 22 and 15.
 template <int NB, int MB, bool BIAS, bool WHOLE>
 __device__ __forceinline__ void store_blocks(const XArgs &xa, const f32x4 (&acc)[NB][MB], int m0, int n0, int li, int lg) {
   const int n1 = n0 + (lg & 1) * 16 + 8 * (lg >> 1);  // first of the lane's stored columns
@@ -544,8 +547,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
 // bytes), behind the wait for that block and the barrier, which come when step 1's
 // operands have long arrived.  Step 0 loads the first unit of block d + 2 (the ninth
 // slot), step 1 the other three and their scale words.
-// 12,252 x 13,824 x 5,120 404 us (4,290 TFLOPS), 4,836 x 10,752 x 5,376 132 us (4,220,
-// the last round in smaller tiles).  Four waves of 128 x 128, each step's operands read
+// 12,252 x 13,824 x 5,120 397 to 425 us by card (404: 4,290 TFLOPS), 4,836 x 10,752 x
+// 5,376 132 us (4,220), the last round in smaller tiles in both; under a profiler, ten
+// calls with pauses, 430 to 453.  Four waves of 128 x 128, each step's operands read
 // a step ahead into a second set of registers, took 411 and 137 us, 2,717 x 5,376 x
 // 5,376 47 against 43.  Without stores it takes 352 us, without loads and stores 294, and
 // the MFMAs alone take 243 at the clock that the power limit leaves them: what the tile

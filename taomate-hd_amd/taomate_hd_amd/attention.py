@@ -33,12 +33,12 @@ BACKENDS = ("bf16", "i8qk")
 # products).  So a row's result does not change its accuracy with the rows beside it: off
 # in the 2-norm by 0.0023 to 0.0024 in place and 0.0028 to 0.0030 expanded on N(0, 1) keys,
 # and more apart at larger scores.  What that costs, in place / expanded, us, three
-# segments: 14 heads of 128 over 40,788 tokens, e4m3, 362/369 at 1,024 rows, 645/620 at
-# 2,048, 1,375/1,188 at 4,836, 3,359/2,786 at 12,252, int8 1,560/1,183 at 4,836; over
-# 11,232 tokens 164/141 at 1,536, 441/350 at 4,836; over 2,717 140/122 at 4,836; over 700
-# 34/53 at 2,560 (3.2e9 products); 4 heads over 2,800 24/55 at 2,048; 14 heads of 64 over
-# 40,788 970/798 at 4,836.  Views that expand_views wrote are attended at the bf16
-# kernel's time and rounding.
+# segments, both sides in turn: 14 heads of 128 over 40,788 tokens, e4m3, 98/181 at 256
+# rows, 285/338 at 1,024, 553/592 at 2,048, 1,301/1,153 at 4,836, 3,151/2,706 at 12,252,
+# int8 1,387/1,156 at 4,836; over 11,232 tokens 136/131 at 1,536, 378/335 at 4,836; over
+# 2,717 133/111 at 4,836; over 700 29/42 at 2,560 (3.2e9 products), 129/90 at 12,252
+# (15e9); 4 heads over 2,800 19/45 at 2,048; 14 heads of 64 over 40,788 967/787 at 4,836.
+# Views that expand_views wrote are attended at the bf16 kernel's time and rounding.
 KV8_ROWS = 1 << 14
 KV8_WORK = 5 << 29
 
