@@ -97,3 +97,40 @@ def test_a_row_keeps_its_accuracy_in_a_larger_call(torch_mod, dev, fmt):
     # the same roundings of weights and results in another order of sums: the norms of n = 153,600 nearly independent
     # errors differ by about (2 n)^-1/2 = 0.2%
     assert abs(off[1] - off[0]) <= 0.02 * off[0], off
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,heads,tokens,beside", [(None, 2, 1301, 0), (70, 3, 333, 90)])
+def test_expanded_calls(torch_mod, dev, rows, heads, tokens, beside, fmt):
+    """Calls beyond the in-place rule, and calls with a bf16 segment: within fp64's bound and what rounding the scaled Q
+    to bf16 adds, 2^-8 of a score's products, twice (score and sum of weights)."""
+    from taomate_hd_amd import KVSlot, attention, segment_attention
+
+    torch, dim = torch_mod, 64
+    rows = rows or attention.KV8_ROWS + 1
+    assert beside or rows * heads * dim * tokens > attention.KV8_WORK
+    k, v = (_randn(torch, dev, tokens + beside, heads, dim, seed=s) for s in (1, 2))
+    slot = _slot(torch, k[:tokens], v[:tokens], fmt, dev)
+    views = [slot.view()]
+    kv = [_f64(t) for t in slot.token_major()]
+    if beside:
+        plain = KVSlot(torch, heads=heads, head_dim=dim, capacity=beside, device=dev)
+        plain.pack(k[tokens:], v[tokens:])
+        views.append(plain.view())
+        kv = [np.concatenate([a, _f64(b[tokens:])]) for a, b in zip(kv, (k, v))]
+    q = _randn(torch, dev, rows, heads, dim, seed=3)
+    got = _f64(segment_attention(torch, q, views, scale=dim ** -0.5))
+    qv = _f64(q)
+    want = lowbit.attention(qv, *kv, dim ** -0.5)
+    for i in range(heads):
+        s = np.abs(qv[:, i]) @ np.abs(kv[0][:, i]).T * dim ** -0.5  # the size of a score's products
+        p = np.exp(qv[:, i] @ kv[0][:, i].T * dim ** -0.5)
+        p /= p.sum(-1, keepdims=True)
+        # each score off by at most 2^-8 of its products (and 2^-15 of fp32's roundings): a weight by a factor of up to
+        # e^that, the sum of weights by the largest of them; then as in _want
+        off = np.exp(HALF_BF16 * s + 2.0 ** -15) - 1
+        off = off + off.max(-1, keepdims=True) + HALF_BF16 + 2.0 ** -12
+        bound = HALF_BF16 * np.abs(want[:, i]) + 1.05 * (p * off) @ np.abs(kv[1][:, i])
+        assert (np.abs(got[:, i] - want[:, i]) <= bound).all()
+    err = np.linalg.norm(got - want, axis=-1) / np.linalg.norm(want, axis=-1)
+    assert np.median(err) <= 2.0 ** -7
